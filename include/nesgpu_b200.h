@@ -585,6 +585,46 @@ int nes_binarized_conv_epilogue(const int32_t* counts, const uint16_t* bias_half
 int nes_binarized_int_threshold(const uint16_t* bias_half, const uint16_t* bias_noise_half, int32_t* out,
                                 int64_t P, int64_t N, int offset, nes_stream_t stream);
 
+/* ------------------------------------------------------- microscaled blocks (no counterpart in the reference)
+ * A microscaled matrix holds every row in blocks of 32 elements that share one power of two.  Elements are e2m1
+ * (NES_MXFP4: two to a byte, even column in the low half) or e4m3 (NES_MXFP8); a scale is one byte c of value
+ * 2^(c - 127), 255 for NaN.  Quantisation: c - 127 = floor(log2 max|x|) - (2 | 8), at least -127; elements are
+ * x * 2^(127 - c) rounded to nearest even and saturated; a zero block has c = 0; a block with a NaN or an
+ * infinity has c = 255 and zero elements.
+ * Layout: row-major, rows padded with zero codes and zero scales to whole groups of 128 elements: with
+ * G = ceil(cols / 128), codes (rows, 64 G | 128 G) bytes, 16-byte aligned, scales (rows, 4 G) bytes. */
+
+enum nes_dtype { NES_F32 = 0, NES_BF16 = 1, NES_F16 = 2 };
+enum nes_mx_format { NES_MXFP4 = 4, NES_MXFP8 = 8 };
+
+/* x (rows, cols) of nes_dtype `dtype` -> codes and scales. */
+int nes_mx_quantize(const void* x, int dtype, void* codes, uint8_t* scales, int64_t rows, int64_t cols,
+                    int format, nes_stream_t stream);
+/* codes and scales -> y (rows, cols) of nes_dtype `dtype`. */
+int nes_mx_dequantize(const void* codes, const uint8_t* scales, void* y, int dtype, int64_t rows, int64_t cols,
+                      int format, nes_stream_t stream);
+/* NES_MXFP4 codes -> y (rows, cols) e4m3 bytes of the same values, without scales and padding. */
+int nes_mx_elements(const void* codes, uint8_t* y, int64_t rows, int64_t cols, nes_stream_t stream);
+
+/* y[t, n] = sum_k x[t, k] w[n, k] + bias[n] with microscaled operands, fp32 accumulation, rounded once to `y_dtype`.
+ * w: codes and scales of (N, K).  x: with x_scales given, codes and scales of (M, K) in x_format; with x_scales NULL,
+ * a (M, K) matrix of nes_dtype x_dtype, which is quantised to x_format into `scratch` first (scratch_bytes() of it;
+ * none is needed otherwise).  Formats (x, w): (4, 4), (8, 4), (8, 8).  bias (N) may be NULL. */
+int64_t nes_mx_linear_fwd_scratch_bytes(int64_t M, int64_t N, int64_t K, int x_format);
+int nes_mx_linear_fwd(const void* x, const uint8_t* x_scales, int x_dtype, int x_format, const void* w_codes,
+                      const uint8_t* w_scales, int w_format, const float* bias, void* y, int y_dtype,
+                      int64_t M, int64_t N, int64_t K, void* scratch, int64_t scratch_bytes, nes_stream_t stream);
+
+/* RMS norm of population rows, with the residual's addition:
+ *   h = x + residual;  y = h / sqrt(mean(h^2) + eps) * (gain + s(r) * noise[d]),  row = r * members + d
+ * x, residual, residual_out (rows, cols) of nes_dtype `dtype`; residual and residual_out are both NULL or both given,
+ * residual_out receives h rounded to `dtype` and may not overlap x or residual.  gain (cols) and noise
+ * (members, cols) are fp32, either may be NULL (gain 1, no noise).  format 0: y (rows, cols) of `dtype`;
+ * otherwise y and y_scales receive the codes and scales of that microscaled format. */
+int nes_rms_norm_fwd(const void* x, const void* residual, void* residual_out, const float* gain, const float* noise,
+                     void* y, uint8_t* y_scales, int64_t rows, int64_t cols, int64_t members, int antithetic,
+                     int dtype, int format, float eps, nes_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -98,6 +98,13 @@ SIGNATURES = {
     "nes_binarized_linear_fwd": [c_ptr] * 5 + [c_i64] * 3 + [c_int] * 4 + [c_ptr, c_i64, c_ptr],
     "nes_binarized_conv_epilogue": [c_ptr] * 4 + [c_i64] * 3 + [c_int] * 4 + [c_ptr, c_ptr],
     "nes_binarized_int_threshold": [c_ptr, c_ptr, c_ptr, c_i64, c_i64, c_int, c_ptr],
+    "nes_mx_quantize": [c_ptr, c_int, c_ptr, c_ptr, c_i64, c_i64, c_int, c_ptr],
+    "nes_mx_dequantize": [c_ptr, c_ptr, c_ptr, c_int, c_i64, c_i64, c_int, c_ptr],
+    "nes_mx_elements": [c_ptr, c_ptr, c_i64, c_i64, c_ptr],
+    "nes_mx_linear_fwd_scratch_bytes": [c_i64] * 3 + [c_int],
+    "nes_mx_linear_fwd": [c_ptr, c_ptr, c_int, c_int, c_ptr, c_ptr, c_int, c_ptr, c_ptr, c_int] + [c_i64] * 3
+                         + [c_ptr, c_i64, c_ptr],
+    "nes_rms_norm_fwd": [c_ptr] * 7 + [c_i64] * 3 + [c_int] * 3 + [c_f32, c_ptr],
 }
 _RETURNS = {
     "nes_status_string": ctypes.c_char_p,
@@ -123,6 +130,7 @@ _RETURNS = {
     "nes_conv2d_fwd_bf16x3_scratch_bytes": c_i64,
     "nes_binarized_update_scratch_bytes": c_i64,
     "nes_binarized_linear_fwd_scratch_bytes": c_i64,
+    "nes_mx_linear_fwd_scratch_bytes": c_i64,
 }
 _NO_STATUS = set(_RETURNS) | {"nes_abi_version"}
 

@@ -18,6 +18,7 @@ from torch import nn
 from torch.nn.modules.utils import _pair
 
 from . import _cabi as C
+from . import microscaling
 
 _F32 = torch.float32
 
@@ -411,21 +412,40 @@ class Permuted(Perturbed):
 
 
 _TC_MODES = {"3xtf32": 3, "tf32": 1}
+# microscaled modes of the base product: (activations, weights)
+_MX_MODES = {"mxfp4": ("mxfp4", "mxfp4"), "mxfp8": ("mxfp8", "mxfp8"), "mxfp8_mxfp4": ("mxfp8", "mxfp4")}
 
 
 class _LinearMixin:
-    def _tensor_core_base(self, x, y):
+    MICROSCALED = False        # whether the layer's base product has the microscaled modes
+
+    def _microscaled_base(self, input, out=None):
+        """``x W^T + b`` with both operands in the blocks of ``options["tc"]`` (``"mxfp4"``, ``"mxfp8"`` or
+        ``"mxfp8_mxfp4"``: 8-bit activations, 4-bit weights).  The weight is quantised as it is at this call."""
+        activations, weights = _MX_MODES[self.options["tc"]]
+        if isinstance(input, microscaling.MicroscaledTensor) and input.format != activations:
+            raise NotImplementedError('options["tc"] = "%s" takes %s activations, got %s'
+                                      % (self.options["tc"], activations, input.format))
+        return microscaling.linear(input, microscaling.quantize(self.weight.detach(), weights), self.bias, activations,
+                                   _F32, out)
+
+    def _tensor_core_base(self, x, y, input=None):
         """y = x W^T + b on the tensor cores when the layer's ``options["tc"]`` allows it.
 
         ``"3xtf32"`` (default; error-compensated, fp32-level accuracy), ``"tf32"`` (plain TF32,
-        relative error ~1e-3: a stated reduced-precision mode) or ``"fp32"`` (CUDA cores).
+        relative error ~1e-3: a stated reduced-precision mode) or ``"fp32"`` (CUDA cores); the microscaled modes
+        of :meth:`_microscaled_base` (4-bit operands are ~1e-1 apart from their fp32 values, 8-bit ones ~3e-2) read
+        ``input`` itself when it is microscaled already.
         Returns False when the CUDA-core kernel has to be used (mode "fp32" or a row length that is
         not a multiple of 4, which the TMA descriptors cannot express)."""
         mode = self.options.get("tc", "3xtf32")
-        if mode == "fp32" or self.in_features % 4 or x.shape[0] == 0:
+        if mode in _MX_MODES and x.shape[0]:
+            self._microscaled_base(input if isinstance(input, microscaling.MicroscaledTensor) else x, y)
+            return True
+        if mode == "fp32" or x.shape[0] == 0 or (self.in_features % 4 and mode not in _MX_MODES):
             return False
         if mode not in _TC_MODES:
-            raise NotImplementedError('options["tc"] must be "3xtf32", "tf32" or "fp32"')
+            raise NotImplementedError('options["tc"] must be "3xtf32", "tf32", "fp32", "mxfp4", "mxfp8" or "mxfp8_mxfp4"')
         M, N, K = x.shape[0], self.out_features, self.in_features
         nbytes = C.call("nes_linear_fwd_tc_scratch_bytes", M, N, K, _TC_MODES[mode])
         buf = C.scratch(nbytes, x.device)
@@ -434,12 +454,20 @@ class _LinearMixin:
         return True
 
     def _flatten_rows(self, input):
+        if isinstance(input, microscaling.MicroscaledTensor):
+            if not self.MICROSCALED or self.options.get("tc") not in _MX_MODES:
+                raise NotImplementedError('microscaled inputs need a layer with options["tc"] = "mxfp4", "mxfp8" or '
+                                          '"mxfp8_mxfp4"')
+            input = input.dequantize()
         x = C.require_cuda(input, "input", _F32)
         if x.shape[-1] != self.in_features:
             raise RuntimeError("expected last dimension %d, got %d" % (self.in_features, x.shape[-1]))
         return x.reshape(-1, self.in_features), x.shape[:-1]
 
     def _plain_forward(self, input):
+        if self.MICROSCALED and self.options.get("tc") in _MX_MODES:
+            mx = isinstance(input, microscaling.MicroscaledTensor)
+            return self._microscaled_base(input if mx else C.require_cuda(input, "input", _F32))
         x, lead = self._flatten_rows(input)
         y = torch.empty((x.shape[0], self.out_features), device=x.device, dtype=_F32)
         C.call("nes_linear_fwd", C.ptr(x), C.ptr(_opt(self.weight)), C.ptr(_opt(self.bias)), C.ptr(y),
@@ -450,6 +478,8 @@ class _LinearMixin:
 class PerturbedLinear(nn.Linear, _LinearMixin, Perturbed):
     """``y = x W^T + b + s * (x E_d^T + beta_d)`` with one dense noise matrix per member
     (reference ``base.py:349-381``)."""
+
+    MICROSCALED = True
 
     def __init__(self, in_features, out_features, directions, bias=True, antithetic=False, options={}):
         nn.Linear.__init__(self, in_features, out_features, bias)
@@ -465,7 +495,7 @@ class PerturbedLinear(nn.Linear, _LinearMixin, Perturbed):
         beta = C.require_cuda(self.bias_noise, "bias_noise", _F32) if self.bias is not None else None
         y = torch.empty((x.shape[0], self.out_features), device=x.device, dtype=_F32)
         self.last_path = "fp32"
-        if not direct and self._tensor_core_base(x, y):
+        if not direct and self._tensor_core_base(x, y, input):
             direct = 2          # y now holds x W^T + b; the streaming kernel adds the per-member term
             self.last_path = self.options.get("tc", "3xtf32")
         C.call("nes_perturbed_linear_fwd", C.ptr(x), C.ptr(_opt(self.weight)), C.ptr(_opt(self.bias)),
@@ -484,6 +514,8 @@ class SparsePerturbedLinear(nn.Linear, _LinearMixin, Perturbed):
     with standard deviation ``noise_scale * sqrt(in / k)`` so that the per-row noise energy
     matches the dense layer.  Forward and update equal :class:`PerturbedLinear` on the
     densified noise."""
+
+    MICROSCALED = True
 
     def __init__(self, in_features, out_features, directions, bias=True, antithetic=False, options={}, k=1):
         nn.Linear.__init__(self, in_features, out_features, bias)
@@ -521,7 +553,7 @@ class SparsePerturbedLinear(nn.Linear, _LinearMixin, Perturbed):
         idx = C.require_cuda(self.noise_indices, "noise_indices", torch.int32)
         beta = C.require_cuda(self.bias_noise, "bias_noise", _F32) if self.bias is not None else None
         y = torch.empty((x.shape[0], self.out_features), device=x.device, dtype=_F32)
-        if self._tensor_core_base(x, y):
+        if self._tensor_core_base(x, y, input):
             # base product on the tensor cores (3xTF32 unless options["tc"] says otherwise), then the k-entry gather
             self.last_path = self.options.get("tc", "3xtf32")
             C.call("nes_sparse_noise_add", C.ptr(y), C.ptr(x), C.ptr(idx), C.ptr(val), C.ptr(beta), self.directions, R,
@@ -1126,3 +1158,32 @@ class PerturbedAffine(nn.Module, Perturbed):
         C.call("nes_affine_fwd", C.ptr(x), C.ptr(scale), C.ptr(shift), C.ptr(y), y.numel(), max(scale.numel(), 1),
                C.stream())
         return y
+
+
+class PerturbedRMSNorm(nn.Module, Perturbed):
+    """RMS norm over the last dimension with one gain vector per member (no counterpart in the reference):
+    ``y = h / sqrt(mean(h^2) + eps) * (weight + s * noise[d])``, ``h = input + residual``; rows are laid out
+    ``b = r * directions + d`` as for the linear layers.
+
+    ``forward(input)`` returns ``y``, ``forward(input, residual)`` the pair ``(y, h)``.  Inputs are float32, bfloat16
+    or float16.  ``options["output"]`` = ``"mxfp8"`` or ``"mxfp4"`` makes ``y`` a
+    :class:`nesgpu_b200.microscaling.MicroscaledTensor`, which a linear layer with a microscaled ``options["tc"]`` reads
+    as it is.  Noise, update and gradients of the gain are those of :class:`Perturbed`."""
+
+    def __init__(self, normalized_shape, directions, eps=1e-6, antithetic=False, options={}):
+        nn.Module.__init__(self)
+        self.weight = nn.Parameter(torch.ones(normalized_shape))
+        self.register_parameter("bias", None)
+        if self.weight.dim() != 1:
+            raise NotImplementedError("PerturbedRMSNorm normalises the last dimension only")
+        if options.get("direct"):
+            raise NotImplementedError("direct storage is not defined for PerturbedRMSNorm")
+        self.eps = eps
+        Perturbed.__init__(self, directions, antithetic, options)
+
+    def forward(self, input, residual=None):
+        noise = None
+        if self.perturbed_flag:
+            noise = C.require_cuda(self.weight_noise, "weight_noise", _F32)
+        return microscaling.rms_norm(input, self.weight, self.eps, residual, noise, self.antithetic,
+                                     self.options.get("output"))

@@ -1,0 +1,95 @@
+"""Microscaled operators without a GPU: the oracle against torch's own 8-bit types, refusals, host-side layer logic."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import microscaled_ref as O
+
+
+def test_oracle_e4m3_table_is_torchs():
+    got = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy()
+    want = O.e4m3_values()
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.array_equal(got[~np.isnan(got)], want[~np.isnan(want)])
+
+
+def test_oracle_e4m3_rounding_is_torchs():
+    g = torch.Generator().manual_seed(0)
+    x = torch.cat([torch.randn(20000, generator=g) * torch.exp2(torch.randint(-12, 9, (20000,), generator=g).float()),
+                   torch.arange(-4480, 4481) / 10, torch.arange(-600, 601) * 2.0 ** -10]).clamp(-448, 448)
+    want = x.to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+    assert np.array_equal(O.element_codes(x.double().numpy(), "mxfp8"), want)
+
+
+def test_oracle_e2m1_ties_go_to_the_even_code():
+    ties = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.9])
+    assert O.elements(O.element_codes(ties, "mxfp4"), "mxfp4").tolist() == [0, 1, 1, 2, 2, 4, 4, 6, 6]
+    assert O.element_codes(-ties[:1], "mxfp4").tolist() == [8]
+
+
+@pytest.mark.parametrize("form,emax", [("mxfp4", 2), ("mxfp8", 8)])
+def test_oracle_scale_codes(form, emax):
+    largest = np.array([0.0, 1.0, 1.999, 2.0, 2.0 ** -149, 2.0 ** 127 * 1.5, np.inf, np.nan])
+    assert O.scale_codes(largest, form).tolist() == [0, 127 - emax, 127 - emax, 128 - emax, 0, 254 - emax, 255, 255]
+
+
+def test_refusals():
+    from nesgpu_b200 import microscaling as ms
+    x = torch.zeros(2, 64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ms.quantize(x)
+    with pytest.raises(NotImplementedError, match="format"):
+        ms.quantize(x, "mxfp6")
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ms.rms_norm(x)
+    with pytest.raises(RuntimeError, match="MicroscaledTensor"):
+        ms.linear(x, x)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ms.MicroscaledTensor(torch.zeros(2, 64, dtype=torch.uint8), torch.zeros(2, 4, dtype=torch.uint8), 64)
+    with pytest.raises(NotImplementedError, match="4-bit weights"):
+        ms.MicroscaledLinear(64, 64, format="mxfp8", activations="mxfp4")
+
+
+def test_c_entry_refusals():
+    """Bad extents, formats, pointers and workspaces come back as statuses; nothing is launched."""
+    from nesgpu_b200 import _cabi
+    L = _cabi.lib
+    p = 4096                                        # stands for a device pointer; no call gets as far as using it
+    assert L.nes_mx_quantize(p, 0, p, p, -1, 64, 4, None) == -1
+    assert L.nes_mx_quantize(p, 0, p, p, 2, 64, 5, None) == -2
+    assert L.nes_mx_quantize(p, 3, p, p, 2, 64, 4, None) == -2
+    assert L.nes_mx_quantize(None, 0, p, p, 2, 64, 4, None) == -1
+    assert L.nes_mx_quantize(p, 0, p + 8, p, 2, 64, 4, None) == -1
+    assert L.nes_mx_quantize(None, 0, None, None, 0, 64, 4, None) == 0
+    assert L.nes_mx_dequantize(p, p, None, 0, 2, 64, 8, None) == -1
+    assert L.nes_mx_elements(p, None, 2, 64, None) == -1
+    assert L.nes_rms_norm_fwd(p, p, None, p, None, p, None, 2, 64, 0, 0, 0, 0, 1e-6, None) == -1      # residual, no output
+    assert L.nes_rms_norm_fwd(p, None, None, p, None, p, None, 2, 64, 0, 0, 0, 8, 1e-6, None) == -1   # no scales
+    assert L.nes_rms_norm_fwd(p, None, None, p, p, p, None, 3, 64, 2, 0, 0, 0, 1e-6, None) == -1      # 3 rows, 2 members
+    assert L.nes_mx_linear_fwd(p, p, 0, 4, p, p, 8, None, p, 0, 2, 64, 64, None, 0, None) == -2       # 4-bit x, 8-bit w
+    assert L.nes_mx_linear_fwd(p, p, 0, 4, p, p, 4, None, p, 0, 2, 64, 0, None, 0, None) == -1        # no columns
+    assert L.nes_mx_linear_fwd(p, p, 0, 4, p + 4, p, 4, None, p, 0, 2, 64, 64, None, 0, None) == -1   # misaligned
+    need = L.nes_mx_linear_fwd_scratch_bytes(200, 64, 64, 8)
+    assert need >= 200 * (128 + 4)
+    assert L.nes_mx_linear_fwd(p, None, 0, 8, p, p, 4, None, p, 0, 200, 64, 64, p, need - 1, None) == -5
+    assert L.nes_mx_linear_fwd(p, None, 7, 8, p, p, 4, None, p, 0, 200, 64, 64, p, need, None) == -2
+    assert L.nes_mx_linear_fwd(None, None, 0, 8, None, None, 4, None, None, 0, 0, 64, 64, None, 0, None) == 0
+
+
+def test_norm_layer_state_follows_the_other_layers():
+    from nesgpu_b200 import base
+    import modules.base as mb
+    assert mb.PerturbedRMSNorm is base.PerturbedRMSNorm
+    layer = base.PerturbedRMSNorm(48, 6)
+    assert layer.weight_noise is None and layer.bias is None and not layer.perturbed_flag
+    layer.allocate_memory()
+    assert layer.weight_noise.shape == (6, 48)
+    layer.free_memory()
+    assert layer.weight_noise is None
+    assert [n for n, _ in layer.named_parameters()] == ["weight"]
+    with pytest.raises(NotImplementedError, match="last dimension"):
+        base.PerturbedRMSNorm((4, 8), 2)
+    with pytest.raises(NotImplementedError, match="direct"):
+        base.PerturbedRMSNorm(8, 2, options={"direct": True})
+    pm = base.PerturbedModel(torch.nn.Sequential(layer, base.PerturbedLinear(48, 5, 6, options={"tc": "mxfp4"})), 6)
+    assert len(pm.perturbed_layers) == 2
