@@ -548,21 +548,23 @@ int conv_tc_error_word(int* v, bool clear);
 int conv_bf16_error_word(int* v, bool clear);
 int conv_pool_error_word(int* v, bool clear);
 int permuted_out_error_word(int* v, bool clear);
+int mx_linear_error_word(int* v, bool clear);
 } }
 
 // Reads the error words of all tensor-core translation units, reports the first non-zero code and clears
 // them, so that a later call reports only what has happened since this one.
 extern "C" int nes_tc_error_flag(int* flag) {
   NES_REQUIRE(flag != nullptr, NES_ERR_BAD_ARG, "tc_error_flag: null pointer");
-  int v[5] = {0, 0, 0, 0, 0};
+  int v[6] = {0, 0, 0, 0, 0, 0};
   int rc = read_error_word(&v[0], true, "tc_error_flag");
   if (rc != NES_OK) return rc;
   if ((rc = nes::tc::conv_tc_error_word(&v[1], true)) != NES_OK) return rc;
   if ((rc = nes::tc::conv_bf16_error_word(&v[2], true)) != NES_OK) return rc;
   if ((rc = nes::tc::conv_pool_error_word(&v[3], true)) != NES_OK) return rc;
   if ((rc = nes::tc::permuted_out_error_word(&v[4], true)) != NES_OK) return rc;
+  if ((rc = nes::tc::mx_linear_error_word(&v[5], true)) != NES_OK) return rc;
   *flag = 0;
-  for (int i = 0; i < 5; ++i)
+  for (int i = 0; i < 6; ++i)
     if (v[i]) { *flag = v[i]; break; }
   return NES_OK;
 }

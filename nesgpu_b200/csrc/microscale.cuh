@@ -26,6 +26,7 @@ __host__ __device__ constexpr int64_t scale_pitch(int64_t cols) { return padded(
 
 inline bool known_format(int f) { return f == NES_MXFP4 || f == NES_MXFP8; }
 inline bool known_dtype(int t) { return t == NES_F32 || t == NES_BF16 || t == NES_F16; }
+inline bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
 inline int64_t dtype_bytes(int t) { return t == NES_F32 ? 4 : 2; }
 
 template <typename T> __device__ __forceinline__ float to_float(T v);

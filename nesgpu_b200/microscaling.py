@@ -73,8 +73,10 @@ class MicroscaledTensor:
                 codes.shape[0] != scales.shape[0]:
             raise RuntimeError("codes and scales of %d columns in %s must be (rows, %d) and (rows, %d), got %s and %s"
                                % (cols, format, pitch, spitch, tuple(codes.shape), tuple(scales.shape)))
-        if self.codes.data_ptr() % 16:
-            self.codes = self.codes.clone()          # the kernels read codes in 16-byte pieces
+        if self.codes.data_ptr() % 32:
+            self.codes = self.codes.clone()          # the kernels read codes in aligned 16- and 32-byte pieces
+        if self.scales.data_ptr() % 4:
+            self.scales = self.scales.clone()
         self.cols = cols
         self.format = format
         lead = (codes.shape[0],) if shape is None else tuple(int(s) for s in shape)
