@@ -23,27 +23,28 @@ struct NormArgs {
   uint8_t* scales;
   int64_t rows, cols, members;
   int antithetic;
-  float eps, width;                 // width: cols as fp32
+  float eps;
+  double inv_cols;
   bool vec, vec_gain;
 };
 
-// 1 / sqrt(v) as hi + lo: one Newton step on the hardware's approximation, with the residual 1 - v hi^2 formed exactly.
-// A reciprocal root that is zero or infinite keeps lo = 0.
-__device__ __forceinline__ float2 rsqrt_pair(float v) {
-  const float r = rsqrtf(v);
+// 1 / sqrt(v) as hi + lo: one Newton step on the hardware's approximation.  A reciprocal root that is zero or
+// infinite keeps lo = 0.
+__device__ __forceinline__ float2 rsqrt_pair(double v) {
+  const float r = rsqrtf(float(v));
   if (!(r > 0.f) || r > 3.0e38f) return make_float2(r, 0.f);
-  const float p = v * r, pe = fmaf(v, r, -p);
-  const float e = fmaf(-p, r, 1.f) - pe * r;
-  return make_float2(r, 0.5f * r * e);
+  return make_float2(r, 0.5f * r * float(1.0 - v * (double(r) * double(r))));
 }
 
-// h * (r.x + r.y) * g with one rounding: the products' own rounding errors are carried along, so that an output
-// that is quantised afterwards falls on the wrong side of a rounding border only through the sum of squares
+// h * (r.x + r.y) * g, the products' rounding errors carried along.  SHARP leaves the fp32 result rounded to odd (cut
+// off, lowest bit set), so that a rounding to fewer bits afterwards decides as it would on the unrounded value; a
+// value exactly on a border does not occur except for a zero.  Otherwise the result is rounded to nearest.
+template <bool SHARP>
 __device__ __forceinline__ float scaled(float h, float2 r, float g) {
-  const float t = h * r.x, te = fmaf(h, r.x, -t) + h * r.y;
-  const float p = t * g, pe = fmaf(t, g, -p);
-  const float y = p + fmaf(te, g, pe);
-  return fabsf(p) < 3.0e38f && fabsf(t) < 3.0e38f ? y : p;       // infinities have no error terms
+  const float t = h * r.x, te = fmaf(h, r.y, fmaf(h, r.x, -t));
+  const float p = t * g, c = fmaf(te, g, fmaf(t, g, -p));
+  if (SHARP) return __uint_as_float(__float_as_uint(__fadd_rz(p, c)) | 1u);
+  return fabsf(p) < 3.0e38f && fabsf(t) < 3.0e38f ? p + c : p;       // infinities have no error terms
 }
 
 __device__ __forceinline__ void load_gain(const NormArgs& a, int64_t row, int64_t c, float (&g)[UNIT]) {
@@ -83,7 +84,7 @@ __device__ __forceinline__ void emit(const NormArgs& a, int64_t row, int64_t uni
     float g[UNIT];
     load_gain(a, row, unit * UNIT, g);
 #pragma unroll
-    for (int i = 0; i < UNIT; ++i) y[i] = scaled(h[i], r, g[i]);
+    for (int i = 0; i < UNIT; ++i) y[i] = scaled<OUT != 0>(h[i], r, g[i]);
   } else {
 #pragma unroll
     for (int i = 0; i < UNIT; ++i) y[i] = 0.f;
@@ -100,18 +101,20 @@ __device__ __forceinline__ void emit(const NormArgs& a, int64_t row, int64_t uni
   }
 }
 
-// Sum over the THREADS threads that share a row (all of a block unless THREADS == 32), the same in every thread.
+// Sum over the THREADS threads that share a row (all of a block unless THREADS == 32), the same in every thread.  The
+// threads' partial sums are joined in 64 bits: the last few additions carry the whole row's rounding.
 template <int THREADS>
-__device__ __forceinline__ float row_sum(float s) {
+__device__ __forceinline__ double row_sum(float mine) {
+  double s = mine;
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if (THREADS > 32) {
-    __shared__ float part[THREADS / 32];
+    __shared__ double part[THREADS / 32];
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
     __syncthreads();
-    s = (threadIdx.x & 31) < THREADS / 32 ? part[threadIdx.x & 31] : 0.f;
+    s = part[0];
 #pragma unroll
-    for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    for (int i = 1; i < THREADS / 32; ++i) s += part[i];
   }
   return s;
 }
@@ -144,7 +147,7 @@ __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) rms_norm_kernel
     const int64_t c = int64_t(t + u * THREADS) * UNIT;
     if (a.h && c < a.cols) store_unit(static_cast<T*>(a.h) + row * a.cols, c, a.cols, a.vec, v[u]);
   }
-  const float2 r = rsqrt_pair(row_sum<THREADS>(s) / a.width + a.eps);
+  const float2 r = rsqrt_pair(row_sum<THREADS>(s) * a.inv_cols + double(a.eps));
 #pragma unroll
   for (int u = 0; u < UNITS; ++u) emit<T, OUT>(a, row, t + u * THREADS, units, v[u], r);
 }
@@ -164,7 +167,7 @@ __global__ void __launch_bounds__(THREADS) rms_norm_long_kernel(const NormArgs a
     s += q;
     if (a.h) store_unit(static_cast<T*>(a.h) + row * a.cols, c, a.cols, a.vec, v);
   }
-  const float2 r = rsqrt_pair(row_sum<THREADS>(s) / a.width + a.eps);
+  const float2 r = rsqrt_pair(row_sum<THREADS>(s) * a.inv_cols + double(a.eps));
   for (int64_t u0 = 0; u0 < units; u0 += THREADS) {
     const int64_t unit = u0 + threadIdx.x;
     float v[UNIT];
@@ -220,7 +223,7 @@ extern "C" int nes_rms_norm_fwd(const void* x, const void* residual, void* resid
   NormArgs a;
   a.x = x; a.residual = residual; a.h = residual_out; a.gain = gain; a.noise = noise; a.y = y; a.scales = y_scales;
   a.rows = rows; a.cols = cols; a.members = members > 0 ? members : 1; a.antithetic = antithetic;
-  a.eps = eps; a.width = float(cols);
+  a.eps = eps; a.inv_cols = 1.0 / double(cols);
   a.vec = vec_rows && aligned16(x) && (!residual || (aligned16(residual) && aligned16(residual_out))) && (format != 0 || aligned16(y));
   a.vec_gain = cols % 4 == 0 && (!gain || aligned16(gain)) && (!noise || aligned16(noise));
   cudaStream_t st = as_stream(stream);

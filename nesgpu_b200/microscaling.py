@@ -9,7 +9,7 @@ infinity has ``c = 255`` and reads as NaN throughout.
 Like the other ops of this package the functions take CUDA tensors, launch on the stream that is current at call time
 on the tensors' device, and record no autograd graph; there is no CPU path.
 """
-import contextlib
+import math
 
 import torch
 from torch import nn
@@ -39,17 +39,17 @@ def _pitches(cols, format):
     return groups * (64 if format == "mxfp4" else 128), groups * 4
 
 
-def _on(device):
-    """Makes ``device`` current for the launches of a call (nothing to do when it already is)."""
+def _launch(name, device, *args):
+    """Calls an entry point on ``device`` and the stream that is current there."""
     if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+        return C.call(name, *args, C.stream())
+    with torch.cuda.device(device):
+        return C.call(name, *args, C.stream())
 
 
-def _same_device(device, **tensors):
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise RuntimeError("nesgpu_b200: %s is on %s, expected %s" % (name, t.device, device))
+def _same_device(device, name, t):
+    if t is not None and t.device != device:
+        raise RuntimeError("nesgpu_b200: %s is on %s, expected %s" % (name, t.device, device))
 
 
 class MicroscaledTensor:
@@ -60,79 +60,77 @@ class MicroscaledTensor:
     contiguous CUDA tensors whose padding is zero.  ``shape`` gives the leading dimensions if there are several (their
     product is ``rows``).  The object refers to the tensors it is given."""
 
+    __slots__ = ("codes", "scales", "shape", "rows", "cols", "format")
+
     def __init__(self, codes, scales, cols, format="mxfp4", shape=None):
         _format(format)
         cols = int(cols)
         if cols < 1:
             raise RuntimeError("a microscaled tensor needs at least one column")
-        self.codes = C.require_cuda(codes, "codes", torch.uint8)
-        self.scales = C.require_cuda(scales, "scales", torch.uint8)
-        _same_device(codes.device, scales=scales)
+        codes = C.require_cuda(codes, "codes", torch.uint8)
+        scales = C.require_cuda(scales, "scales", torch.uint8)
+        _same_device(codes.device, "scales", scales)
         pitch, spitch = _pitches(cols, format)
-        if codes.dim() != 2 or scales.dim() != 2 or codes.shape[1] != pitch or scales.shape[1] != spitch or \
-                codes.shape[0] != scales.shape[0]:
+        rows = codes.shape[0] if codes.dim() else 0
+        if codes.shape != (rows, pitch) or scales.shape != (rows, spitch):
             raise RuntimeError("codes and scales of %d columns in %s must be (rows, %d) and (rows, %d), got %s and %s"
                                % (cols, format, pitch, spitch, tuple(codes.shape), tuple(scales.shape)))
-        if self.codes.data_ptr() % 32:
-            self.codes = self.codes.clone()          # the kernels read codes in aligned 16- and 32-byte pieces
-        if self.scales.data_ptr() % 4:
-            self.scales = self.scales.clone()
-        self.cols = cols
-        self.format = format
-        lead = (codes.shape[0],) if shape is None else tuple(int(s) for s in shape)
-        rows = 1
-        for s in lead:
-            rows *= s
-        if rows != codes.shape[0]:
-            raise RuntimeError("leading dimensions %s do not match %d rows" % (lead, codes.shape[0]))
-        self._lead = lead
+        if codes.data_ptr() % 32:                # the kernels read codes in aligned 16- and 32-byte pieces
+            codes = codes.clone()
+        if scales.data_ptr() % 4:
+            scales = scales.clone()
+        lead = (rows,) if shape is None else tuple(int(s) for s in shape)
+        if math.prod(lead) != rows:
+            raise RuntimeError("leading dimensions %s do not match %d rows" % (lead, rows))
+        self._set(codes, scales, lead, rows, cols, format)
 
-    @property
-    def shape(self):
-        return torch.Size(self._lead + (self.cols,))
+    def _set(self, codes, scales, lead, rows, cols, format):
+        self.codes, self.scales = codes, scales
+        self.shape = torch.Size((*lead, cols))
+        self.rows, self.cols, self.format = rows, cols, format
+        return self
 
     @property
     def device(self):
         return self.codes.device
 
-    @property
-    def rows(self):
-        return self.codes.shape[0]
-
     def __repr__(self):
         return "MicroscaledTensor(shape=%s, format=%s, device=%s)" % (tuple(self.shape), self.format, self.device)
 
+    def _view(self, t, width):
+        """The first ``width`` columns of a row-major byte matrix, with this tensor's leading dimensions."""
+        if t.shape[1] != width:
+            t = t.narrow(1, 0, width)
+        return t if len(self.shape) == 2 else t.unflatten(0, self.shape[:-1])
+
     def block_scales(self):
         """``(..., ceil(cols / 32))`` scales as ``torch.float8_e8m0fnu`` (a view)."""
-        blocks = -(-self.cols // BLOCK)
-        return self.scales.view(*self._lead, -1)[..., :blocks].view(torch.float8_e8m0fnu) if self.rows else \
-            self.scales.new_empty(self._lead + (blocks,)).view(torch.float8_e8m0fnu)
+        return self._view(self.scales, -(-self.cols // BLOCK)).view(torch.float8_e8m0fnu)
 
     def elements(self):
         """``(..., cols)`` element values before the scale, as ``torch.float8_e4m3fn``: a view for ``"mxfp8"``,
         unpacked for ``"mxfp4"`` (every e2m1 value is an e4m3 value)."""
-        if self.format == "mxfp4" or not self.rows:
-            out = torch.empty(self.shape, dtype=torch.uint8, device=self.device)
-            if self.rows:
-                with _on(self.device):
-                    C.call("nes_mx_elements", C.ptr(self.codes), C.ptr(out), self.rows, self.cols, C.stream())
-            return out.view(torch.float8_e4m3fn)
-        return self.codes.view(*self._lead, -1)[..., :self.cols].view(torch.float8_e4m3fn)
+        if self.format == "mxfp8":
+            return self._view(self.codes, self.cols).view(torch.float8_e4m3fn)
+        out = self.codes.new_empty(self.shape, dtype=torch.float8_e4m3fn)
+        _launch("nes_mx_elements", self.codes.device, self.codes.data_ptr(), out.data_ptr(), self.rows, self.cols)
+        return out
 
     def dequantize(self, dtype=torch.float32):
         """The values ``element * scale`` (exact in fp32; rounded to nearest even in bfloat16 and float16)."""
         kind = _dtype(dtype, "the result")
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        with _on(self.device):
-            C.call("nes_mx_dequantize", C.ptr(self.codes), C.ptr(self.scales), C.ptr(out), kind, self.rows, self.cols,
-                   FORMATS[self.format], C.stream())
+        out = self.codes.new_empty(self.shape, dtype=dtype)
+        _launch("nes_mx_dequantize", self.codes.device, self.codes.data_ptr(), self.scales.data_ptr(), out.data_ptr(), kind,
+                self.rows, self.cols, FORMATS[self.format])
         return out
 
 
-def _empty(lead, rows, cols, format, device):
+def _empty(x, rows, cols, format):
+    """Uninitialised blocks for ``rows`` rows, with the leading dimensions and on the device of ``x``."""
     pitch, spitch = _pitches(cols, format)
-    return MicroscaledTensor(torch.empty((rows, pitch), dtype=torch.uint8, device=device),
-                             torch.empty((rows, spitch), dtype=torch.uint8, device=device), cols, format, lead)
+    return MicroscaledTensor.__new__(MicroscaledTensor)._set(
+        x.new_empty((rows, pitch), dtype=torch.uint8), x.new_empty((rows, spitch), dtype=torch.uint8), x.shape[:-1],
+        rows, cols, format)
 
 
 def _rows(t, name):
@@ -148,10 +146,10 @@ def quantize(input, format="mxfp4"):
     """``(..., cols)`` float32 / bfloat16 / float16 -> :class:`MicroscaledTensor`."""
     kind = _format(format)
     x, rows = _rows(input, "input")
-    q = _empty(x.shape[:-1], rows, x.shape[-1], format, x.device)
-    with _on(x.device):
-        C.call("nes_mx_quantize", C.ptr(x), _DTYPES[x.dtype], C.ptr(q.codes), C.ptr(q.scales), rows, q.cols, kind,
-               C.stream())
+    cols = x.shape[-1]
+    q = _empty(x, rows, cols, format)
+    _launch("nes_mx_quantize", x.device, x.data_ptr(), _DTYPES[x.dtype], q.codes.data_ptr(), q.scales.data_ptr(), rows,
+            cols, kind)
     return q
 
 
@@ -165,33 +163,38 @@ def linear(input, weight, bias=None, activations="mxfp8", dtype=None, out=None):
     if not isinstance(weight, MicroscaledTensor) or len(weight.shape) != 2:
         raise RuntimeError("weight must be a MicroscaledTensor of (out_features, in_features)")
     out_features, in_features = weight.shape
+    x_scales, x_kind = None, 0
     if isinstance(input, MicroscaledTensor):
-        activations, x, x_scales, x_kind = input.format, input.codes, input.scales, 0
-        rows, dtype = input.rows, dtype or (torch.float32 if out is None else out.dtype)
+        x, rows, activations, default = input.codes, input.rows, input.format, torch.float32
+        x_scales = input.scales.data_ptr()
     else:
         x, rows = _rows(input, "input")
-        x_scales, x_kind, dtype = None, _DTYPES[x.dtype], dtype or (x.dtype if out is None else out.dtype)
-    x_format, w_format, y_kind = _format(activations, "activations"), FORMATS[weight.format], _dtype(dtype, "the result")
+        x_kind, default = _DTYPES[x.dtype], x.dtype
+    if dtype is None:
+        dtype = default if out is None else out.dtype
+    x_format, y_kind = _format(activations, "activations"), _dtype(dtype, "the result")
+    device = x.device
     if input.shape[-1] != in_features:
         raise RuntimeError("expected last dimension %d, got %d" % (in_features, input.shape[-1]))
+    _same_device(device, "weight", weight.codes)
     if bias is not None:
-        bias = C.require_cuda(bias.detach(), "bias", torch.float32)
-        if tuple(bias.shape) != (out_features,):
+        bias = C.require_cuda(bias, "bias", torch.float32)
+        if bias.shape != (out_features,):
             raise RuntimeError("bias must have shape (%d,), got %s" % (out_features, tuple(bias.shape)))
-    _same_device(x.device, weight=weight, bias=bias)
+        _same_device(device, "bias", bias)
     y = out
     if out is None:
-        y = torch.empty(input.shape[:-1] + (out_features,), dtype=dtype, device=x.device)
-    elif out.device != x.device or out.dtype != dtype or not out.is_contiguous() or out.numel() != rows * out_features:
-        raise RuntimeError("out must be a contiguous %s tensor of %d elements on %s" % (dtype, rows * out_features, x.device))
-    nbytes = 0 if x_scales is not None else C.call("nes_mx_linear_fwd_scratch_bytes", rows, out_features, in_features,
-                                                   x_format)
-    # a buffer of this call's own: calls captured into different graphs share nothing
-    buf = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-    with _on(x.device):
-        C.call("nes_mx_linear_fwd", C.ptr(x), C.ptr(x_scales), x_kind, x_format, C.ptr(weight.codes),
-               C.ptr(weight.scales), w_format, C.ptr(bias), C.ptr(y), y_kind, rows, out_features, in_features,
-               C.ptr(buf), nbytes, C.stream())
+        y = x.new_empty((*input.shape[:-1], out_features), dtype=dtype)
+    elif out.device != device or out.dtype != dtype or not out.is_contiguous() or out.numel() != rows * out_features:
+        raise RuntimeError("out must be a contiguous %s tensor of %d elements on %s" % (dtype, rows * out_features, device))
+    buf, nbytes = None, 0
+    if x_scales is None:
+        nbytes = C.call("nes_mx_linear_fwd_scratch_bytes", rows, out_features, in_features, x_format)
+        if nbytes:      # a buffer of this call's own: calls captured into different graphs share nothing
+            buf = x.new_empty(nbytes, dtype=torch.uint8)
+    _launch("nes_mx_linear_fwd", device, x.data_ptr(), x_scales, x_kind, x_format, weight.codes.data_ptr(),
+            weight.scales.data_ptr(), FORMATS[weight.format], C.ptr(bias), y.data_ptr(), y_kind, rows, out_features,
+            in_features, C.ptr(buf), nbytes)
     return y
 
 
@@ -204,38 +207,38 @@ def rms_norm(input, weight=None, eps=1e-6, residual=None, noise=None, antithetic
     second half of the repeats with ``antithetic``).  ``output`` is None for a ``y`` of the input's type, or
     ``"mxfp8"`` / ``"mxfp4"`` for a :class:`MicroscaledTensor`."""
     x, rows = _rows(input, "input")
-    cols = x.shape[-1]
+    cols, device = x.shape[-1], x.device
     kind = 0 if output is None or output == x.dtype else _format(output, "output")
     if not eps >= 0:
         raise RuntimeError("eps must not be negative, got %r" % (eps,))
-    h = members = None
+    h, members = None, 0
     if residual is not None:
         if not isinstance(residual, torch.Tensor) or residual.shape != x.shape:
             raise RuntimeError("residual must have the input's shape %s" % (tuple(x.shape),))
         residual = C.require_cuda(residual, "residual", x.dtype)
+        _same_device(device, "residual", residual)
         h = torch.empty_like(x)
     if weight is not None:
-        weight = C.require_cuda(weight.detach(), "weight", torch.float32)
-        if tuple(weight.shape) != (cols,):
+        weight = C.require_cuda(weight, "weight", torch.float32)
+        if weight.shape != (cols,):
             raise RuntimeError("weight must have shape (%d,), got %s" % (cols, tuple(weight.shape)))
+        _same_device(device, "weight", weight)
     if noise is not None:
         noise = C.require_cuda(noise, "noise", torch.float32)
-        if noise.dim() != 2 or noise.shape[1] != cols or noise.shape[0] == 0:
+        members = noise.shape[0] if noise.dim() else 0
+        if not members or noise.shape != (members, cols):
             raise RuntimeError("noise must have shape (members, %d), got %s" % (cols, tuple(noise.shape)))
-        members = noise.shape[0]
         if rows % members:
             raise RuntimeError("batch size %d is not a multiple of directions %d" % (rows, members))
-    _same_device(x.device, residual=residual, weight=weight, noise=noise)
+        _same_device(device, "noise", noise)
     if kind:
-        y = _empty(x.shape[:-1], rows, cols, output, x.device)
-        data, scales = y.codes, y.scales
+        y = _empty(x, rows, cols, output)
+        data, scales = y.codes.data_ptr(), y.scales.data_ptr()
     else:
-        y = data = torch.empty_like(x)
-        scales = None
-    with _on(x.device):
-        C.call("nes_rms_norm_fwd", C.ptr(x), C.ptr(residual), C.ptr(h), C.ptr(weight), C.ptr(noise), C.ptr(data),
-               C.ptr(scales), rows, cols, members or 0, 1 if antithetic else 0, _DTYPES[x.dtype], kind, float(eps),
-               C.stream())
+        y = torch.empty_like(x)
+        data, scales = y.data_ptr(), None
+    _launch("nes_rms_norm_fwd", device, x.data_ptr(), C.ptr(residual), C.ptr(h), C.ptr(weight), C.ptr(noise), data,
+            scales, rows, cols, members, 1 if antithetic else 0, _DTYPES[x.dtype], kind, eps)
     return y if residual is None else (y, h)
 
 
