@@ -10,7 +10,8 @@
 //     byte (16 elements and 8 empty bytes... per 16-byte piece) by the copy itself.
 //   * Scales are stored row-major (4 bytes per 128 elements); the instruction wants them in tensor memory, one 32-bit
 //     column per 32 rows and 128 elements, repeated in each quarter of the lanes.  Four warps load them for STEP = 512
-//     elements of K at a time, 16 bytes per row, and write them with tcgen05.st: a transposition that costs no shared memory.
+//     elements of K at a time, 16 bytes per row and thread, transpose them on the way into shared memory, and tcgen05.cp
+//     brings them over in the order of the products.
 //   * Few output tiles: a cluster of up to eight CTAs splits K and adds its partial tiles in a fixed order through
 //     distributed shared memory.
 #include <type_traits>
@@ -26,6 +27,7 @@ constexpr int FEATURES = 128;                // accumulator lanes
 constexpr int ROW_BYTES = 128;               // one swizzle row of an operand per stage
 constexpr int STEP = 512;                    // elements of K whose scales are written at once
 constexpr int CHUNKS = STEP / GROUP;         // 32-bit scale words of a row per step
+constexpr int SCALE_TILE = 512;              // scales of 128 rows x 128 elements in shared memory
 constexpr int THREADS_TC = 192;              // warp 0: TMA, warp 1: MMA, warps 2-5: scales, then epilogue
 
 struct Product {
@@ -42,13 +44,14 @@ struct Layout {
   static constexpr int W_BYTES = FEATURES * ROW_BYTES;
   static constexpr int X_BYTES = TOKENS * ROW_BYTES;
   static constexpr int STAGE = W_BYTES + X_BYTES;
-  static constexpr int STAGES = TOKENS >= 256 ? 4 : TOKENS >= 128 ? 6 : 8;
-  static constexpr int X_COLS = TOKENS <= 128 ? 4 : 8;                     // scale columns of x per 128 elements
+  static constexpr int STAGES = TOKENS >= 128 ? 6 : 8;
+  static constexpr int X_COLS = 4;                                         // scale columns of x per 128 elements
   static constexpr int SCALE_COLS = CHUNKS * (4 + X_COLS);                 // one buffer
   static constexpr int SCALE_BASE = TOKENS < 32 ? 32 : TOKENS;
   static constexpr int USED_COLS = SCALE_BASE + 2 * SCALE_COLS;
   static constexpr int TMEM_COLS = USED_COLS <= 128 ? 128 : USED_COLS <= 256 ? 256 : 512;
-  static constexpr size_t SMEM = 1024 + size_t(STAGES) * STAGE + (2 * STAGES + 5) * sizeof(uint64_t) + 16;
+  static constexpr int SCALES = 2 * CHUNKS * SCALE_TILE;                   // a buffer in shared memory: w, then x
+  static constexpr size_t SMEM = 1024 + size_t(STAGES) * STAGE + 2 * SCALES + (2 * STAGES + 5) * sizeof(uint64_t) + 16;
 };
 
 template <int XF, int WF>
@@ -88,36 +91,116 @@ constexpr uint32_t idesc_scaled(int m, int n) {
 __device__ __forceinline__ constexpr uint32_t scale_byte(uint32_t id) { return (id << 29) | (id << 4); }
 
 // 16 scale bytes of a row from 128-element group `group` on; zeros outside the matrix
-__device__ __forceinline__ void load_scale_words(const uint8_t* scales, int row, int rows, int group, int groups, bool vec, uint32_t (&w)[CHUNKS]) {
-#pragma unroll
-  for (int j = 0; j < CHUNKS; ++j) w[j] = 0;
-  if (row >= rows) return;
+__device__ __forceinline__ uint4 load_scale_words(const uint8_t* scales, int row, int rows, int group, int groups, bool vec) {
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  if (row >= rows) return v;
   const uint32_t* p = reinterpret_cast<const uint32_t*>(scales + int64_t(row) * groups * 4) + group;
-  if (vec) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-    w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-  } else {
-#pragma unroll
-    for (int j = 0; j < CHUNKS; ++j) if (group + j < groups) w[j] = __ldg(p + j);
-  }
+  if (vec) return __ldg(reinterpret_cast<const uint4*>(p));
+  v.x = __ldg(p);
+  if (group + 1 < groups) v.y = __ldg(p + 1);
+  if (group + 2 < groups) v.z = __ldg(p + 2);
+  if (group + 3 < groups) v.w = __ldg(p + 3);
+  return v;
+}
+
+// Scales in shared memory: one tile of 512 bytes per 128 rows and 128 elements, the word of row 32 c + l at word 4 l + c,
+// which is the order in which tcgen05.cp (32 lanes x 16 bytes, repeated for the four lane quarters) makes the four
+// 32-bit columns of tensor memory that an instruction reads.  Thread t of the 128 that fill a tile owns word t, so the
+// stores have no bank conflicts.
+__device__ __forceinline__ int scale_row(int t) { return (t & 3) * 32 + (t >> 2); }
+__device__ __forceinline__ void put_scale_words(unsigned char* tiles, int t, const uint4& v) {      // CHUNKS tiles in a row
+  uint32_t* w = reinterpret_cast<uint32_t*>(tiles) + t;
+  w[0] = v.x;
+  w[SCALE_TILE / 4] = v.y;
+  w[2 * SCALE_TILE / 4] = v.z;
+  w[3 * SCALE_TILE / 4] = v.w;
+}
+// descriptor of a scale tile: no swizzle, 8 rows x 16 bytes per core matrix, core matrices 128 bytes apart
+__device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
+  return uint64_t((saddr & 0x3FFFFu) >> 4) | (uint64_t(1) << 16) | (uint64_t(128 >> 4) << 32) | (uint64_t(1) << 46);
+}
+template <int CTAS>
+__device__ __forceinline__ void warp_copy_scales(uint32_t tmem, uint64_t desc) {
+  if (CTAS == 2)
+    asm volatile("{\n.reg .pred pe;\nelect.sync _|pe, 0xffffffff;\n@pe tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n}\n" ::"r"(tmem), "l"(desc) : "memory");
+  else
+    asm volatile("{\n.reg .pred pe;\nelect.sync _|pe, 0xffffffff;\n@pe tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n}\n" ::"r"(tmem), "l"(desc) : "memory");
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
+__device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
   uint32_t remote;
-  float v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+  return remote;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t remote) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
   return v;
 }
 
-__device__ __forceinline__ void store_result(const Product& p, int64_t at, float v) {
-  if (p.y_dtype == NES_F32) static_cast<float*>(p.y)[at] = v;
-  else if (p.y_dtype == NES_BF16) static_cast<__nv_bfloat16*>(p.y)[at] = __float2bfloat16_rn(v);
-  else static_cast<__half*>(p.y)[at] = __float2half_rn(v);
+// Four neighbouring features of one token; `left` of them exist.
+template <typename T>
+__device__ __forceinline__ void store_four(T* y, const float4& v, int left, bool vec) {
+  if (vec && left >= 4) {
+    if (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(y) = v;
+    } else {
+      using H = typename std::conditional<sizeof(T) == 4, __half, T>::type;
+      *reinterpret_cast<uint2*>(y) = make_uint2(float_to_pair(v.x, v.y, H()), float_to_pair(v.z, v.w, H()));
+    }
+  } else {
+    if (left > 0) y[0] = from_float<T>(v.x);
+    if (left > 1) y[1] = from_float<T>(v.y);
+    if (left > 2) y[2] = from_float<T>(v.z);
+    if (left > 3) y[3] = from_float<T>(v.w);
+  }
+}
+
+// Adds the partial tiles ([token][feature] fp32 at the same shared-memory address of every CTA of the cluster) in rank
+// order and stores this CTA's share of the tokens: token = rank + splits * i, four features per lane.
+template <typename T>
+__device__ __forceinline__ void join_tiles(const Product& p, uint32_t part, int n0, int m0, int tokens, int rank, int splits, int warp, int lane) {
+  const int n = n0 + lane * 4, left = p.N - n;
+  if (left <= 0) return;
+  float4 bias = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (p.bias) {
+    bias.x = __ldg(p.bias + n);
+    if (left > 1) bias.y = __ldg(p.bias + n + 1);
+    if (left > 2) bias.z = __ldg(p.bias + n + 2);
+    if (left > 3) bias.w = __ldg(p.bias + n + 3);
+  }
+  uint32_t source[8];
+#pragma unroll
+  for (int r = 0; r < 8; ++r) source[r] = r < splits ? map_rank(part, r) : 0u;
+  const bool vec = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0;
+  constexpr int AT_ONCE = 4;                                     // tokens whose loads are in flight together
+  for (int t0 = rank + splits * warp; t0 < tokens; t0 += splits * 4 * AT_ONCE) {
+    float4 sum[AT_ONCE];
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) sum[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      if (r >= splits) break;
+#pragma unroll
+      for (int i = 0; i < AT_ONCE; ++i) {
+        const int t = t0 + i * splits * 4;
+        if (t >= tokens) continue;
+        const float4 v = ld_cluster4(source[r] + uint32_t(t * FEATURES + lane * 4) * 4u);
+        sum[i].x += v.x; sum[i].y += v.y; sum[i].z += v.z; sum[i].w += v.w;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const int t = t0 + i * splits * 4;
+      if (t >= tokens) continue;
+      sum[i].x += bias.x; sum[i].y += bias.y; sum[i].z += bias.z; sum[i].w += bias.w;
+      store_four(static_cast<T*>(p.y) + int64_t(m0 + t) * p.N + n, sum[i], left, vec);
+    }
+  }
 }
 
 template <int XF, int WF, int TOKENS>
@@ -127,7 +210,8 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
   const unsigned int timeouts_at_start = timeouts_so_far();
   const uint32_t raw = smem_u32(dyn_raw);
   unsigned char* tiles = dyn_raw + (((raw + 1023u) & ~1023u) - raw);
-  uint64_t* full = reinterpret_cast<uint64_t*>(tiles + size_t(L::STAGES) * L::STAGE);
+  unsigned char* scale_tiles = tiles + size_t(L::STAGES) * L::STAGE;
+  uint64_t* full = reinterpret_cast<uint64_t*>(scale_tiles + 2 * L::SCALES);
   uint64_t* empty = full + L::STAGES;
   uint64_t* sf_full = empty + L::STAGES;
   uint64_t* sf_empty = sf_full + 2;
@@ -177,6 +261,7 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
   } else if (warp == 1) {
     constexpr uint32_t idesc = idesc_scaled<XF, WF>(FEATURES, TOKENS);
     const uint64_t desc0 = smem_desc_sw128(smem_u32(tiles));
+    const uint64_t sdesc0 = scale_desc(smem_u32(scale_tiles));
     int s = 0;
     uint32_t ph = 0, sf_ph = 0, accumulate = 0;
     int kt = kt0;
@@ -185,7 +270,12 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
       ok = warp_mbar_wait(&sf_full[b], sf_ph, 2);
       if (!ok) break;
       if (b) sf_ph ^= 1u;
+      tc_fence_after();
       const uint32_t sfa = tmem + L::SCALE_BASE + b * L::SCALE_COLS, sfb = sfa + CHUNKS * 4;
+#pragma unroll
+      for (int j = 0; j < 2 * CHUNKS; ++j)              // four columns each: w, then x
+        warp_copy_scales<1>(sfa + 4 * j, sdesc0 + uint64_t((b * L::SCALES + j * SCALE_TILE) >> 4));
+      warp_mma_commit(&sf_empty[b]);
 #pragma unroll
       for (int i = 0; i < STAGES_PER_STEP; ++i, ++kt) {
         if (kt >= kt1) break;
@@ -204,106 +294,379 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
         warp_mma_commit(&empty[s]);
         if (++s == L::STAGES) { s = 0; ph ^= 1u; }
       }
-      warp_mma_commit(&sf_empty[b]);
     }
     warp_mma_commit(accum);
   } else {
     const int q = warp & 3;
     const uint32_t lanes = uint32_t(q * 32) << 16;
-    uint32_t wr[4][CHUNKS], xr[L::X_COLS][CHUNKS];
-    auto load = [&](int step) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) load_scale_words(p.w_scales, n0 + c * 32 + lane, p.N, step * CHUNKS, p.groups, p.vec_scales, wr[c]);
-#pragma unroll
-      for (int c = 0; c < L::X_COLS; ++c)
-        load_scale_words(p.x_scales, c * 32 < TOKENS ? m0 + c * 32 + lane : p.M, p.M, step * CHUNKS, p.groups, p.vec_scales, xr[c]);
+    const int t = threadIdx.x - 64, row = scale_row(t);
+    uint4 wv[2], xv[2];                              // two steps in flight
+    auto load = [&](int step, uint4& wo, uint4& xo) {
+      if (step >= step1) return;
+      wo = load_scale_words(p.w_scales, n0 + row, p.N, step * CHUNKS, p.groups, p.vec_scales);
+      xo = load_scale_words(p.x_scales, row < TOKENS ? m0 + row : p.M, p.M, step * CHUNKS, p.groups, p.vec_scales);
     };
-    uint32_t ph = 0;
-    if (step0 < step1) load(step0);
-    for (int step = step0; step < step1; ++step) {
-      const int b = (step - step0) & 1;
-      uint32_t r[16], t[CHUNKS * L::X_COLS];
+    load(step0, wv[0], xv[0]);
+    load(step0 + 1, wv[1], xv[1]);
+    uint32_t ph = 1;
+    for (int step = step0; step < step1 && ok; step += 2, ph ^= 1u) {
 #pragma unroll
-      for (int j = 0; j < CHUNKS; ++j) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) r[j * 4 + c] = wr[c][j];
-#pragma unroll
-        for (int c = 0; c < L::X_COLS; ++c) t[j * L::X_COLS + c] = xr[c][j];
+      for (int b = 0; b < 2; ++b) {
+        if (step + b >= step1) break;
+        ok = warp_mbar_wait(&sf_empty[b], ph, 4);
+        if (!ok) break;
+        unsigned char* to = scale_tiles + b * L::SCALES;
+        put_scale_words(to, t, wv[b]);
+        put_scale_words(to + CHUNKS * SCALE_TILE, t, xv[b]);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sf_full[b]);
+        load(step + b + 2, wv[b], xv[b]);
       }
-      if (step + 1 < step1) load(step + 1);
-      ok = warp_mbar_wait(&sf_empty[b], ph ^ 1, 4);
-      if (!ok) break;
-      if (b) ph ^= 1u;
-      tc_fence_after();
-      const uint32_t base = tmem + lanes + L::SCALE_BASE + b * L::SCALE_COLS;
-      tmem_st16(base, r);
-#pragma unroll
-      for (int c = 0; c < CHUNKS * L::X_COLS; c += 16) {
-        uint32_t u[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) u[i] = t[c + i];
-        tmem_st16(base + CHUNKS * 4 + c, u);
-      }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sf_full[b]);
     }
     ok = warp_mbar_wait(accum, 0, 3) && ok;
     tc_fence_after();
     const bool good = __all_sync(0xffffffffu, ok && timeouts_so_far() == timeouts_at_start);
-    const int f = q * 32 + lane, n = n0 + f;
-    if (splits == 1) {
-      if (good) {
-        const float bias = p.bias && n < p.N ? __ldg(p.bias + n) : 0.f;
+    float* part = reinterpret_cast<float*>(tiles) + q * 32 + lane;           // every stage has been consumed
 #pragma unroll 1
-        for (int c = 0; c < TOKENS; c += 16) {
-          if (m0 + c >= p.M) break;
-          uint32_t r[16];
-          tmem_ld16_nowait(tmem + lanes + c, r);
-          tmem_ld_wait();
-          if (n < p.N) {
+    for (int c = 0; c < TOKENS; c += 16) {
+      if (m0 + c >= p.M) break;
+      uint32_t r[16];
+      tmem_ld16_nowait(tmem + lanes + c, r);
+      tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (m0 + c + j < p.M) store_result(p, int64_t(m0 + c + j) * p.N + n, __uint_as_float(r[j]) + bias);
-          }
-        }
-      }
-    } else {
-      float* part = reinterpret_cast<float*>(tiles);           // [token][feature]; every stage has been consumed
-#pragma unroll 1
-      for (int c = 0; c < TOKENS; c += 16) {
-        if (m0 + c >= p.M) break;
-        uint32_t r[16];
-        tmem_ld16_nowait(tmem + lanes + c, r);
-        tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 16; ++j) part[(c + j) * FEATURES + f] = good ? __uint_as_float(r[j]) : 0.f;
-      }
+      for (int j = 0; j < 16; ++j) part[(c + j) * FEATURES] = good ? __uint_as_float(r[j]) : 0.f;
     }
   }
   __syncwarp();
-  if (splits > 1) {
-    cluster_sync_all();
-    if (warp >= 2) {
-      const int f = (warp & 3) * 32 + lane, n = n0 + f;
-      const bool good = timeouts_so_far() == timeouts_at_start;
-      const float bias = p.bias && n < p.N ? __ldg(p.bias + n) : 0.f;
-      for (int t = rank; t < TOKENS && m0 + t < p.M; t += splits) {
-        const uint32_t at = smem_u32(tiles) + uint32_t(t * FEATURES + f) * 4u;
-        float v = 0.f;
-        for (int r = 0; r < splits; ++r) v += ld_cluster(at, r);
-        if (good && n < p.N) store_result(p, int64_t(m0 + t) * p.N + n, v + bias);
-      }
-    }
-    __syncwarp();
-    cluster_sync_all();                                        // partial tiles stay until everyone has read them
+  if (splits > 1) cluster_sync_all(); else __syncthreads();
+  if (warp >= 2 && timeouts_so_far() == timeouts_at_start) {
+    const int tokens = min(TOKENS, p.M - m0);
+    if (p.y_dtype == NES_F32) join_tiles<float>(p, smem_u32(tiles), n0, m0, tokens, rank, splits, warp - 2, lane);
+    else if (p.y_dtype == NES_BF16) join_tiles<__nv_bfloat16>(p, smem_u32(tiles), n0, m0, tokens, rank, splits, warp - 2, lane);
+    else join_tiles<__half>(p, smem_u32(tiles), n0, m0, tokens, rank, splits, warp - 2, lane);
   }
+  __syncwarp();
+  if (splits > 1) cluster_sync_all();                          // partial tiles stay until everyone has read them
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, L::TMEM_COLS);
+  }
+}
+
+
+// ------------------------------------------------------------------------------------------ many tokens: CTA pairs
+//
+// Two CTAs share a tile of 256 features x 192 tokens (tcgen05 with cta_group::2): each holds 128 weight rows and half of
+// the tokens' rows and keeps the accumulator of its own features, so an SM reads (128 + 96) rows per stage where it
+// would need 128 + 192 alone.  The grid is persistent: 192 columns fit tensor memory twice beside two buffers of
+// scales (2 * 192 + 2 * 48 = 480 of 512 columns), so the epilogue of a tile runs under the products of the next.
+// Results go through shared memory to TMA stores, which clip at the matrix's edges.
+
+constexpr int PAIR_TOKENS = 192;
+constexpr int PAIR_FEATURES = 2 * FEATURES;
+constexpr int THREADS_PAIR = 320;            // warp 0: TMA, 1: MMA (leading CTA), 2-5: scales, 6-9: epilogue
+
+struct PairLayout {
+  static constexpr int W_BYTES = FEATURES * ROW_BYTES;
+  static constexpr int X_BYTES = PAIR_TOKENS / 2 * ROW_BYTES;
+  static constexpr int STAGE = W_BYTES + X_BYTES;
+  static constexpr int STAGES = 6;
+  static constexpr int X_COLS = 8;                                         // six in use
+  static constexpr int SCALE_COLS = CHUNKS * (4 + X_COLS);
+  static constexpr int SCALE_BASE = 2 * PAIR_TOKENS;
+  static constexpr int OUT_TOKENS = 32;                                    // tokens of one output box
+  static constexpr int OUT_BYTES = OUT_TOKENS * 32 * 4;                    // one warp's box
+  static constexpr int SCALES = 3 * CHUNKS * SCALE_TILE;                   // a buffer in shared memory: w, x rows 0-127, x rows 128-191
+  static constexpr size_t SMEM = 1024 + size_t(STAGES) * STAGE + 8 * OUT_BYTES + 2 * SCALES + (2 * STAGES + 8) * sizeof(uint64_t) + 16;
+};
+static_assert(PairLayout::SCALE_BASE + 2 * PairLayout::SCALE_COLS <= 512, "tensor memory");
+static_assert(PairLayout::SMEM <= 227 * 1024, "shared memory");
+
+struct PairMaps { CUtensorMap w, x, y; };
+
+template <int XF, int WF>
+__device__ __forceinline__ void warp_mma_scaled_pair(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb,
+                                                     uint32_t accumulate) {
+  if (XF == NES_MXFP4)
+    asm volatile(
+        "{\n"
+        ".reg .pred p, pe;\n"
+        "elect.sync _|pe, 0xffffffff;\n"
+        "setp.ne.b32 p, %6, 0;\n"
+        "@pe tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n"
+        "}\n"
+        ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n"
+        ".reg .pred p, pe;\n"
+        "elect.sync _|pe, 0xffffffff;\n"
+        "setp.ne.b32 p, %6, 0;\n"
+        "@pe tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n"
+        "}\n"
+        ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+// arrives at the barrier of the same address in both CTAs once the products issued so far are done
+__device__ __forceinline__ void warp_commit_pair(uint64_t* bar) {
+  asm volatile(
+      "{\n"
+      ".reg .pred pe;\n"
+      "elect.sync _|pe, 0xffffffff;\n"
+      "@pe tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n"
+      "}\n"
+      ::"r"(smem_u32(bar)), "h"(uint16_t(3)) : "memory");
+}
+// load into this CTA's shared memory, counted by a barrier of the leading CTA
+__device__ __forceinline__ void tma_load_pair(void* dst, const CUtensorMap* map, uint32_t leader_bar, int c0, int c1) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(leader_bar), "r"(c0), "r"(c1)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+               ::"l"(map), "r"(smem_u32(src)), "r"(c0), "r"(c1) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t (&r)[32]) {
+  tmem_ld16_nowait(taddr, r);
+  tmem_ld16_nowait(taddr + 16, r + 16);
+}
+
+// One warp's box of 32 tokens x 32 features: lane = feature, r[j] = token j.
+template <typename T>
+__device__ __forceinline__ void box_to_smem(unsigned char* box, int lane, const uint32_t (&r)[32], float bias) {
+  T* out = reinterpret_cast<T*>(box) + lane;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) out[j * 32] = from_float<T>(__uint_as_float(r[j]) + bias);
+}
+template <typename T>
+__device__ __forceinline__ void box_to_global(const Product& p, int m, int n, const uint32_t (&r)[32], float bias) {
+  if (n >= p.N) return;
+  T* out = static_cast<T*>(p.y) + int64_t(m) * p.N + n;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) {
+    if (m + j < p.M) *out = from_float<T>(__uint_as_float(r[j]) + bias);
+    out += p.N;
+  }
+}
+
+template <int XF, int WF>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS_PAIR, 1)
+mx_pair_kernel(const __grid_constant__ PairMaps maps, const Product p, int ftiles, int tiles, int tma_out) {
+  using L = PairLayout;
+  extern __shared__ unsigned char dyn_raw[];
+  const unsigned int timeouts_at_start = timeouts_so_far();
+  const uint32_t raw = smem_u32(dyn_raw);
+  unsigned char* stages = dyn_raw + (((raw + 1023u) & ~1023u) - raw);
+  unsigned char* boxes = stages + size_t(L::STAGES) * L::STAGE;
+  unsigned char* scale_tiles = boxes + 8 * L::OUT_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(scale_tiles + 2 * L::SCALES);
+  uint64_t* empty = full + L::STAGES;
+  uint64_t* sf_full = empty + L::STAGES;
+  uint64_t* sf_empty = sf_full + 2;
+  uint64_t* acc_full = sf_empty + 2;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = int(cluster_rank());
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  constexpr int STAGE_GROUPS = XF == NES_MXFP4 ? 2 : 1;
+  constexpr int STAGES_PER_STEP = CHUNKS / STAGE_GROUPS;
+  const int steps = (p.groups + CHUNKS - 1) / CHUNKS;
+  const int kts = (p.groups + STAGE_GROUPS - 1) / STAGE_GROUPS;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < L::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&sf_full[s], 8); mbar_init(&sf_empty[s], 1);       // four scale warps of each CTA
+      mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 8);     // four epilogue warps of each CTA
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                                              // both CTAs' barriers exist
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  bool ok = true;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      constexpr uint32_t W_TX = XF == NES_MXFP8 && WF == NES_MXFP4 ? L::W_BYTES / 2 : L::W_BYTES;   // a spreading copy counts what it reads
+      const uint32_t full0 = map_rank(smem_u32(full), 0);
+      int s = 0;
+      uint32_t ph = 0;
+      for (int tile = pair; tile < tiles && ok; tile += pairs) {
+        const int n0 = (tile % ftiles) * PAIR_FEATURES + rank * FEATURES, m0 = (tile / ftiles) * PAIR_TOKENS + rank * (PAIR_TOKENS / 2);
+        for (int kt = 0; kt < kts; ++kt) {
+          ok = mbar_wait(&empty[s], ph ^ 1, 1);
+          if (!ok) break;
+          unsigned char* st = stages + size_t(s) * L::STAGE;
+          if (rank == 0) mbar_expect_tx(&full[s], 2 * (W_TX + L::X_BYTES));
+          const uint32_t bar = full0 + uint32_t(s) * 8u;
+          tma_load_pair(st, &maps.w, bar, kt * ROW_BYTES, n0);
+          tma_load_pair(st + L::W_BYTES, &maps.x, bar, kt * ROW_BYTES, m0);
+          if (++s == L::STAGES) { s = 0; ph ^= 1u; }
+        }
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (rank == 0) {
+      constexpr uint32_t idesc = idesc_scaled<XF, WF>(PAIR_FEATURES, PAIR_TOKENS);
+      const uint64_t desc0 = smem_desc_sw128(smem_u32(stages));
+      const uint64_t sdesc0 = scale_desc(smem_u32(scale_tiles));
+      int s = 0, b = 0, acc = 0;
+      uint32_t ph = 0, sf_ph = 0, acc_ph = 0;
+      for (int tile = pair; tile < tiles && ok; tile += pairs) {
+        ok = warp_mbar_wait(&acc_empty[acc], acc_ph ^ 1, 2);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t d = tmem + acc * PAIR_TOKENS;
+        uint32_t accumulate = 0;
+        int kt = 0;
+        for (int step = 0; step < steps && ok; ++step) {
+          ok = warp_mbar_wait(&sf_full[b], sf_ph, 2);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t sfa = tmem + L::SCALE_BASE + b * L::SCALE_COLS, sfb = sfa + CHUNKS * 4;
+          const uint64_t sdesc = sdesc0 + uint64_t((b * L::SCALES) >> 4);
+#pragma unroll
+          for (int j = 0; j < CHUNKS; ++j) {
+            warp_copy_scales<2>(sfa + 4 * j, sdesc + uint64_t((j * SCALE_TILE) >> 4));
+            warp_copy_scales<2>(sfb + L::X_COLS * j, sdesc + uint64_t(((CHUNKS + j) * SCALE_TILE) >> 4));
+            warp_copy_scales<2>(sfb + L::X_COLS * j + 4, sdesc + uint64_t(((2 * CHUNKS + j) * SCALE_TILE) >> 4));
+          }
+          warp_commit_pair(&sf_empty[b]);
+#pragma unroll
+          for (int i = 0; i < STAGES_PER_STEP; ++i, ++kt) {
+            if (kt >= kts) break;
+            ok = warp_mbar_wait(&full[s], ph, 2);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t a = desc0 + uint64_t(uint32_t(s) * uint32_t(L::STAGE >> 4)), x = a + (L::W_BYTES >> 4);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const int j = XF == NES_MXFP4 ? i * 2 + (k >> 1) : i;
+              const uint32_t id = XF == NES_MXFP4 ? (k & 1) * 2 : k;
+              if (XF != NES_MXFP4 || kt * 2 + (k >> 1) < p.groups)
+                warp_mma_scaled_pair<XF, WF>(d, a + 2 * k, x + 2 * k, idesc | scale_byte(id), sfa + 4 * j, sfb + L::X_COLS * j, accumulate);
+              accumulate = 1;
+            }
+            warp_commit_pair(&empty[s]);
+            if (++s == L::STAGES) { s = 0; ph ^= 1u; }
+          }
+          if (b) sf_ph ^= 1u;
+          b ^= 1;
+        }
+        warp_commit_pair(&acc_full[acc]);
+        if (acc) acc_ph ^= 1u;
+        acc ^= 1;
+      }
+    }
+  } else if (warp < 6) {
+    const uint32_t sf_full0 = map_rank(smem_u32(sf_full), 0);
+    const int t = threadIdx.x - 64, row = scale_row(t);
+    uint4 v[2][3];                                   // two steps in flight
+    int tile = pair, step = 0;                       // of the next load
+    auto load = [&](uint4 (&o)[3]) {
+      if (tile >= tiles) return;
+      const int n0 = (tile % ftiles) * PAIR_FEATURES + rank * FEATURES, m0 = (tile / ftiles) * PAIR_TOKENS;
+      o[0] = load_scale_words(p.w_scales, n0 + row, p.N, step * CHUNKS, p.groups, p.vec_scales);
+      o[1] = load_scale_words(p.x_scales, m0 + row, p.M, step * CHUNKS, p.groups, p.vec_scales);
+      o[2] = load_scale_words(p.x_scales, row < PAIR_TOKENS - 128 ? m0 + 128 + row : p.M, p.M, step * CHUNKS, p.groups, p.vec_scales);
+      if (++step == steps) { step = 0; tile += pairs; }
+    };
+    load(v[0]);
+    load(v[1]);
+    const int64_t total = pair < tiles ? int64_t((tiles - 1 - pair) / pairs + 1) * steps : 0;
+    uint32_t ph = 1;
+    for (int64_t i = 0; i < total && ok; i += 2, ph ^= 1u) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        if (i + b >= total) break;
+        ok = warp_mbar_wait(&sf_empty[b], ph, 4);
+        if (!ok) break;
+        unsigned char* to = scale_tiles + b * L::SCALES;
+#pragma unroll
+        for (int h = 0; h < 3; ++h) put_scale_words(to + h * CHUNKS * SCALE_TILE, t, v[b][h]);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(sf_full0 + b * 8);
+        load(v[b]);
+      }
+    }
+  } else {
+    const int q = warp & 3;
+    const uint32_t lanes = uint32_t(q * 32) << 16;
+    const uint32_t acc_empty0 = map_rank(smem_u32(acc_empty), 0);
+    unsigned char* box = boxes + (warp - 6) * 2 * L::OUT_BYTES;
+    int acc = 0, side = 0;
+    uint32_t ph = 0;
+    for (int tile = pair; tile < tiles; tile += pairs) {
+      const int n0 = (tile % ftiles) * PAIR_FEATURES + rank * FEATURES + q * 32, m0 = (tile / ftiles) * PAIR_TOKENS;
+      ok = warp_mbar_wait(&acc_full[acc], ph, 3);
+      if (!ok) break;
+      tc_fence_after();
+      const bool good = __all_sync(0xffffffffu, timeouts_so_far() == timeouts_at_start);
+      const float bias = p.bias && n0 + lane < p.N ? __ldg(p.bias + n0 + lane) : 0.f;
+#pragma unroll 1
+      for (int c = 0; c < PAIR_TOKENS; c += L::OUT_TOKENS) {
+        if (m0 + c >= p.M) break;
+        uint32_t r[32];
+        tmem_ld32_nowait(tmem + lanes + acc * PAIR_TOKENS + c, r);
+        tmem_ld_wait();
+        if (!good || n0 >= p.N) continue;
+        if (tma_out) {
+          unsigned char* out = box + side * L::OUT_BYTES;
+          side ^= 1;
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");      // the box's last store has been read
+          __syncwarp();
+          if (p.y_dtype == NES_F32) box_to_smem<float>(out, lane, r, bias);
+          else if (p.y_dtype == NES_BF16) box_to_smem<__nv_bfloat16>(out, lane, r, bias);
+          else box_to_smem<__half>(out, lane, r, bias);
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&maps.y, out, n0, m0 + c);
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+        } else if (p.y_dtype == NES_F32) {
+          box_to_global<float>(p, m0 + c, n0 + lane, r, bias);
+        } else if (p.y_dtype == NES_BF16) {
+          box_to_global<__nv_bfloat16>(p, m0 + c, n0 + lane, r, bias);
+        } else {
+          box_to_global<__half>(p, m0 + c, n0 + lane, r, bias);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(acc_empty0 + acc * 8);
+      if (acc) ph ^= 1u;
+      acc ^= 1;
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync_all();                                              // no CTA leaves while the other may still signal it
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
   }
 }
 
@@ -356,12 +719,43 @@ static int launch_product(const Product& p, const void* x, const void* w, cudaSt
 }
 
 template <int XF, int WF>
+static int launch_pair(const Product& p, const void* x, const void* w, cudaStream_t st) {
+  using L = PairLayout;
+  PairMaps maps;
+  int rc = code_map(&maps.w, w, p.N, p.groups, WF == NES_MXFP4, WF == NES_MXFP4 && XF == NES_MXFP8, FEATURES);
+  if (rc != NES_OK) return rc;
+  if ((rc = code_map(&maps.x, x, p.M, p.groups, XF == NES_MXFP4, false, PAIR_TOKENS / 2)) != NES_OK) return rc;
+  const int size = int(dtype_bytes(p.y_dtype));
+  const int tma_out = (int64_t(p.N) * size) % 16 == 0 && aligned16(p.y);
+  maps.y = maps.x;
+  if (tma_out) {
+    cuuint64_t dims[2] = {(cuuint64_t)p.N, (cuuint64_t)p.M};
+    cuuint64_t strides[1] = {cuuint64_t(p.N) * size};
+    cuuint32_t box[2] = {32, (cuuint32_t)L::OUT_TOKENS};
+    cuuint32_t estr[2] = {1, 1};
+    const CUtensorMapDataType type = p.y_dtype == NES_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : p.y_dtype == NES_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    CUresult r = encode_fn()(&maps.y, type, 2, p.y, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                             CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    NES_REQUIRE(r == CUDA_SUCCESS, NES_ERR_LAUNCH, "mx_linear_fwd: cuTensorMapEncodeTiled failed with %d", (int)r);
+  }
+  const int64_t ftiles = ceil_div<int64_t>(p.N, PAIR_FEATURES), tiles = ftiles * ceil_div<int64_t>(p.M, PAIR_TOKENS);
+  NES_REQUIRE(tiles <= INT32_MAX / 2, NES_ERR_UNSUPPORTED, "mx_linear_fwd: too large");
+  const auto kernel = mx_pair_kernel<XF, WF>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::SMEM);
+  if (e != cudaSuccess) return fail(NES_ERR_LAUNCH, "mx_linear_fwd: shared memory opt-in failed: %s", cudaGetErrorString(e));
+  const int64_t pairs = tiles < sm_count() / 2 ? tiles : sm_count() / 2;
+  kernel<<<unsigned(pairs * 2), THREADS_PAIR, L::SMEM, st>>>(maps, p, int(ftiles), int(tiles), tma_out);
+  return check_launch("mx_linear_fwd");
+}
+
+template <int XF, int WF>
 static int launch_tokens(const Product& p, const void* x, const void* w, cudaStream_t st) {
   if (p.M <= 16) return launch_product<XF, WF, 16>(p, x, w, st);
   if (p.M <= 32) return launch_product<XF, WF, 32>(p, x, w, st);
   if (p.M <= 64) return launch_product<XF, WF, 64>(p, x, w, st);
-  if (p.M <= 128 || ceil_div(p.M, 256) * ceil_div(p.N, FEATURES) < sm_count()) return launch_product<XF, WF, 128>(p, x, w, st);
-  return launch_product<XF, WF, 256>(p, x, w, st);
+  if (p.M <= 128) return launch_product<XF, WF, 128>(p, x, w, st);
+  return launch_pair<XF, WF>(p, x, w, st);
 }
 
 static int64_t align256(int64_t v) { return (v + 255) & ~int64_t(255); }
