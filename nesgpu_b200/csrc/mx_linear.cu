@@ -54,31 +54,6 @@ struct Layout {
   static constexpr size_t SMEM = 1024 + size_t(STAGES) * STAGE + 2 * SCALES + (2 * STAGES + 5) * sizeof(uint64_t) + 16;
 };
 
-template <int XF, int WF>
-__device__ __forceinline__ void warp_mma_scaled(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb,
-                                                uint32_t accumulate) {
-  if (XF == NES_MXFP4)
-    asm volatile(
-        "{\n"
-        ".reg .pred p, pe;\n"
-        "elect.sync _|pe, 0xffffffff;\n"
-        "setp.ne.b32 p, %6, 0;\n"
-        "@pe tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n"
-        "}\n"
-        ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-        : "memory");
-  else
-    asm volatile(
-        "{\n"
-        ".reg .pred p, pe;\n"
-        "elect.sync _|pe, 0xffffffff;\n"
-        "setp.ne.b32 p, %6, 0;\n"
-        "@pe tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n"
-        "}\n"
-        ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-        : "memory");
-}
-
 // Instruction descriptor with block scales: element formats at bits 7 and 10 (kind::mxf4: 1 = e2m1; kind::mxf8f6f4: 0 = e4m3,
 // 5 = e2m1), N >> 3 at bit 17, scale type 1 = E8M0 at bit 23, M >> 4 at bit 24; the byte of the scale columns that an
 // instruction uses is added per instruction (bits 29 for A and 4 for B).
@@ -88,7 +63,58 @@ constexpr uint32_t idesc_scaled(int m, int n) {
   constexpr uint32_t b = XF == NES_MXFP4 ? 1u : 0u;
   return (a << 7) | (b << 10) | (uint32_t(n >> 3) << 17) | (1u << 23) | (uint32_t(m >> 4) << 24);
 }
-__device__ __forceinline__ constexpr uint32_t scale_byte(uint32_t id) { return (id << 29) | (id << 4); }
+__host__ __device__ constexpr uint32_t scale_byte(uint32_t id) { return (id << 29) | (id << 4); }
+
+// The products of one stage: four instructions (two if HALF: a last stage with one 128-element group of 4-bit codes), each 32
+// bytes further along the rows.  They share one elected lane and one asm block: an instruction with an election of its own takes
+// 113 cycles to issue, which is more than a 4-bit product of 192 columns takes to run.
+// kind::mxf4: two instructions per scale word (bytes 0-1 and 2-3), words sfa / sfb and sfa1 / sfb1; otherwise four.
+#define NES_MX_STAGE4(GROUP, KIND, VEC)                                                              \
+  asm volatile(                                                                                      \
+      "{\n"                                                                                          \
+      ".reg .pred p, pe, pt;\n"                                                                      \
+      ".reg .b64 a1, a2, a3, x1, x2, x3;\n"                                                          \
+      "elect.sync _|pe, 0xffffffff;\n"                                                               \
+      "setp.ne.b32 p, %11, 0;\n"                                                                     \
+      "setp.eq.b32 pt, 0, 0;\n"                                                                      \
+      "add.s64 a1, %1, 2;\n"                                                                         \
+      "add.s64 a2, %1, 4;\n"                                                                         \
+      "add.s64 a3, %1, 6;\n"                                                                         \
+      "add.s64 x1, %2, 2;\n"                                                                         \
+      "add.s64 x2, %2, 4;\n"                                                                         \
+      "add.s64 x3, %2, 6;\n"                                                                         \
+      "@pe tcgen05.mma." GROUP "." KIND ".block_scale." VEC " [%0], %1, %2, %3, [%7], [%8], p;\n"    \
+      "@pe tcgen05.mma." GROUP "." KIND ".block_scale." VEC " [%0], a1, x1, %4, [%7], [%8], pt;\n"   \
+      "@pe tcgen05.mma." GROUP "." KIND ".block_scale." VEC " [%0], a2, x2, %5, [%9], [%10], pt;\n"  \
+      "@pe tcgen05.mma." GROUP "." KIND ".block_scale." VEC " [%0], a3, x3, %6, [%9], [%10], pt;\n"  \
+      "}\n" ::"r"(d), "l"(a), "l"(x), "r"(i0), "r"(i1), "r"(i2), "r"(i3), "r"(sfa), "r"(sfb), "r"(sfa1), "r"(sfb1), "r"(accumulate) : "memory")
+#define NES_MX_STAGE2(GROUP)                                                                         \
+  asm volatile(                                                                                      \
+      "{\n"                                                                                          \
+      ".reg .pred p, pe, pt;\n"                                                                      \
+      ".reg .b64 a1, x1;\n"                                                                          \
+      "elect.sync _|pe, 0xffffffff;\n"                                                               \
+      "setp.ne.b32 p, %7, 0;\n"                                                                      \
+      "setp.eq.b32 pt, 0, 0;\n"                                                                      \
+      "add.s64 a1, %1, 2;\n"                                                                         \
+      "add.s64 x1, %2, 2;\n"                                                                         \
+      "@pe tcgen05.mma." GROUP ".kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%5], [%6], p;\n"  \
+      "@pe tcgen05.mma." GROUP ".kind::mxf4.block_scale.scale_vec::2X [%0], a1, x1, %4, [%5], [%6], pt;\n" \
+      "}\n" ::"r"(d), "l"(a), "l"(x), "r"(i0), "r"(i1), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory")
+
+template <int XF, int CTAS, bool HALF = false>
+__device__ __forceinline__ void warp_mma_stage(uint32_t d, uint64_t a, uint64_t x, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t sfa1,
+                                               uint32_t sfb1, uint32_t accumulate) {
+  constexpr bool FOUR = XF == NES_MXFP4;
+  const uint32_t i0 = idesc, i1 = idesc | scale_byte(FOUR ? 2 : 1), i2 = idesc | scale_byte(FOUR ? 0 : 2), i3 = idesc | scale_byte(FOUR ? 2 : 3);
+  if (HALF) {
+    if (CTAS == 2) NES_MX_STAGE2("cta_group::2"); else NES_MX_STAGE2("cta_group::1");
+  } else if (FOUR) {
+    if (CTAS == 2) NES_MX_STAGE4("cta_group::2", "kind::mxf4", "scale_vec::2X"); else NES_MX_STAGE4("cta_group::1", "kind::mxf4", "scale_vec::2X");
+  } else {
+    if (CTAS == 2) NES_MX_STAGE4("cta_group::2", "kind::mxf8f6f4", "scale_vec::1X"); else NES_MX_STAGE4("cta_group::1", "kind::mxf8f6f4", "scale_vec::1X");
+  }
+}
 
 // 16 scale bytes of a row from 128-element group `group` on; zeros outside the matrix
 __device__ __forceinline__ uint4 load_scale_words(const uint8_t* scales, int row, int rows, int group, int groups, bool vec) {
@@ -119,12 +145,29 @@ __device__ __forceinline__ void put_scale_words(unsigned char* tiles, int t, con
 __device__ __forceinline__ uint64_t scale_desc(uint32_t saddr) {
   return uint64_t((saddr & 0x3FFFFu) >> 4) | (uint64_t(1) << 16) | (uint64_t(128 >> 4) << 32) | (uint64_t(1) << 46);
 }
-template <int CTAS>
+// CHUNKS tiles, `cols` columns apart in tensor memory
+#define NES_MX_COPY4(GROUP)                                            \
+  asm volatile(                                                        \
+      "{\n"                                                            \
+      ".reg .pred pe;\n"                                               \
+      ".reg .b64 s1, s2, s3;\n"                                        \
+      ".reg .b32 t1, t2, t3;\n"                                        \
+      "elect.sync _|pe, 0xffffffff;\n"                                 \
+      "add.s64 s1, %1, 32;\n"                                          \
+      "add.s64 s2, %1, 64;\n"                                          \
+      "add.s64 s3, %1, 96;\n"                                          \
+      "add.s32 t1, %0, %2;\n"                                          \
+      "add.s32 t2, t1, %2;\n"                                          \
+      "add.s32 t3, t2, %2;\n"                                          \
+      "@pe tcgen05.cp." GROUP ".32x128b.warpx4 [%0], %1;\n"            \
+      "@pe tcgen05.cp." GROUP ".32x128b.warpx4 [t1], s1;\n"            \
+      "@pe tcgen05.cp." GROUP ".32x128b.warpx4 [t2], s2;\n"            \
+      "@pe tcgen05.cp." GROUP ".32x128b.warpx4 [t3], s3;\n"            \
+      "}\n" ::"r"(tmem), "l"(desc), "n"(COLS) : "memory")
+template <int CTAS, int COLS>
 __device__ __forceinline__ void warp_copy_scales(uint32_t tmem, uint64_t desc) {
-  if (CTAS == 2)
-    asm volatile("{\n.reg .pred pe;\nelect.sync _|pe, 0xffffffff;\n@pe tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n}\n" ::"r"(tmem), "l"(desc) : "memory");
-  else
-    asm volatile("{\n.reg .pred pe;\nelect.sync _|pe, 0xffffffff;\n@pe tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n}\n" ::"r"(tmem), "l"(desc) : "memory");
+  static_assert(CHUNKS == 4 && SCALE_TILE == 512, "the copies' offsets");
+  if (CTAS == 2) NES_MX_COPY4("cta_group::2"); else NES_MX_COPY4("cta_group::1");
 }
 
 __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
@@ -270,11 +313,11 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
       ok = warp_mbar_wait(&sf_full[b], sf_ph, 2);
       if (!ok) break;
       if (b) sf_ph ^= 1u;
-      tc_fence_after();
+      fence_proxy_async_smem();                         // here and not in the loading warps: it waits for loads in flight
       const uint32_t sfa = tmem + L::SCALE_BASE + b * L::SCALE_COLS, sfb = sfa + CHUNKS * 4;
-#pragma unroll
-      for (int j = 0; j < 2 * CHUNKS; ++j)              // four columns each: w, then x
-        warp_copy_scales<1>(sfa + 4 * j, sdesc0 + uint64_t((b * L::SCALES + j * SCALE_TILE) >> 4));
+      const uint64_t sdesc = sdesc0 + uint64_t((b * L::SCALES) >> 4);
+      warp_copy_scales<1, 4>(sfa, sdesc);
+      warp_copy_scales<1, L::X_COLS>(sfb, sdesc + uint64_t((CHUNKS * SCALE_TILE) >> 4));
       warp_mma_commit(&sf_empty[b]);
 #pragma unroll
       for (int i = 0; i < STAGES_PER_STEP; ++i, ++kt) {
@@ -283,14 +326,13 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
         if (!ok) break;
         tc_fence_after();
         const uint64_t a = desc0 + uint64_t(uint32_t(s) * uint32_t(L::STAGE >> 4)), x = a + (L::W_BYTES >> 4);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {                 // 32 bytes of a row per instruction
-          const int j = XF == NES_MXFP4 ? i * 2 + (k >> 1) : i;
-          const uint32_t id = XF == NES_MXFP4 ? (k & 1) * 2 : k;
-          if (XF != NES_MXFP4 || kt * 2 + (k >> 1) < p.groups)
-            warp_mma_scaled<XF, WF>(tmem, a + 2 * k, x + 2 * k, idesc | scale_byte(id), sfa + 4 * j, sfb + L::X_COLS * j, accumulate);
-          accumulate = 1;
-        }
+        const int j = i * STAGE_GROUPS;
+        if (STAGE_GROUPS == 1 || kt * 2 + 1 < p.groups)
+          warp_mma_stage<XF, 1>(tmem, a, x, idesc, sfa + 4 * j, sfb + L::X_COLS * j, sfa + 4 * (j + STAGE_GROUPS - 1),
+                                sfb + L::X_COLS * (j + STAGE_GROUPS - 1), accumulate);
+        else
+          warp_mma_stage<XF, 1, true>(tmem, a, x, idesc, sfa + 4 * j, sfb + L::X_COLS * j, 0u, 0u, accumulate);
+        accumulate = 1;
         warp_mma_commit(&empty[s]);
         if (++s == L::STAGES) { s = 0; ph ^= 1u; }
       }
@@ -318,7 +360,6 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
         unsigned char* to = scale_tiles + b * L::SCALES;
         put_scale_words(to, t, wv[b]);
         put_scale_words(to + CHUNKS * SCALE_TILE, t, xv[b]);
-        fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sf_full[b]);
         load(step + b + 2, wv[b], xv[b]);
@@ -359,13 +400,19 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
 
 // ------------------------------------------------------------------------------------------ many tokens: CTA pairs
 //
-// Two CTAs share a tile of 256 features x 192 tokens (tcgen05 with cta_group::2): each holds 128 weight rows and half of
-// the tokens' rows and keeps the accumulator of its own features, so an SM reads (128 + 96) rows per stage where it
-// would need 128 + 192 alone.  The grid is persistent: 192 columns fit tensor memory twice beside two buffers of
-// scales (2 * 192 + 2 * 48 = 480 of 512 columns), so the epilogue of a tile runs under the products of the next.
+// Two CTAs share a tile of 256 features x 256 tokens (tcgen05 with cta_group::2): each holds 128 weight rows and half of
+// the tokens' rows and keeps the accumulator of its own features, so an SM reads 128 + 128 rows per stage where it
+// would need 128 + 256 alone.  256 columns are the widest instruction and the only one near the pipe's rate: measured
+// without loads and epilogue, an e2m1 product of K = 64 takes 170 cycles with 256 columns and as many with 192; an e4m3
+// one of K = 32 takes 143 and 118.
+//
+// The grid is persistent, and the epilogue of a tile runs under the products of the next: two accumulators of 256
+// columns and two buffers of scales (2 * 48) need 608 columns of the 512 there are, so the accumulators overlap by 96
+// (columns 0-255 and 160-415).  The epilogue reads the shared columns first and hands them over; the rest of its
+// work is done while the next tile fills the other accumulator.
 // Results go through shared memory to TMA stores, which clip at the matrix's edges.
 
-constexpr int PAIR_TOKENS = 192;
+constexpr int PAIR_TOKENS = 256;
 constexpr int PAIR_FEATURES = 2 * FEATURES;
 constexpr int THREADS_PAIR = 320;            // warp 0: TMA, 1: MMA (leading CTA), 2-5: scales, 6-9: epilogue
 
@@ -374,43 +421,20 @@ struct PairLayout {
   static constexpr int X_BYTES = PAIR_TOKENS / 2 * ROW_BYTES;
   static constexpr int STAGE = W_BYTES + X_BYTES;
   static constexpr int STAGES = 6;
-  static constexpr int X_COLS = 8;                                         // six in use
+  static constexpr int X_COLS = 8;
   static constexpr int SCALE_COLS = CHUNKS * (4 + X_COLS);
-  static constexpr int SCALE_BASE = 2 * PAIR_TOKENS;
-  static constexpr int OUT_TOKENS = 32;                                    // tokens of one output box
-  static constexpr int OUT_BYTES = OUT_TOKENS * 32 * 4;                    // one warp's box
-  static constexpr int SCALES = 3 * CHUNKS * SCALE_TILE;                   // a buffer in shared memory: w, x rows 0-127, x rows 128-191
-  static constexpr size_t SMEM = 1024 + size_t(STAGES) * STAGE + 8 * OUT_BYTES + 2 * SCALES + (2 * STAGES + 8) * sizeof(uint64_t) + 16;
+  static constexpr int SCALE_BASE = 512 - 2 * SCALE_COLS;
+  static constexpr int ACC_STRIDE = SCALE_BASE - PAIR_TOKENS;              // first column of the second accumulator
+  static constexpr int SHARED_COLS = PAIR_TOKENS - ACC_STRIDE;             // columns both accumulators have
+  static constexpr int OUT_BYTES = 32 * 64;                                // one warp's output box: 32 features x 32 (16-bit) or 16 tokens
+  static constexpr int SCALES = 3 * CHUNKS * SCALE_TILE;                   // a buffer in shared memory: w, x rows 0-127, x rows 128-255
+  static constexpr size_t SMEM = 1024 + size_t(STAGES) * STAGE + 8 * OUT_BYTES + 2 * SCALES + (2 * STAGES + 10) * sizeof(uint64_t) + 16;
 };
-static_assert(PairLayout::SCALE_BASE + 2 * PairLayout::SCALE_COLS <= 512, "tensor memory");
+static_assert(PairLayout::SHARED_COLS == 96 && PairLayout::SHARED_COLS % 32 == 0, "tensor memory");
 static_assert(PairLayout::SMEM <= 227 * 1024, "shared memory");
 
 struct PairMaps { CUtensorMap w, x, y; };
 
-template <int XF, int WF>
-__device__ __forceinline__ void warp_mma_scaled_pair(uint32_t d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb,
-                                                     uint32_t accumulate) {
-  if (XF == NES_MXFP4)
-    asm volatile(
-        "{\n"
-        ".reg .pred p, pe;\n"
-        "elect.sync _|pe, 0xffffffff;\n"
-        "setp.ne.b32 p, %6, 0;\n"
-        "@pe tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n"
-        "}\n"
-        ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-        : "memory");
-  else
-    asm volatile(
-        "{\n"
-        ".reg .pred p, pe;\n"
-        "elect.sync _|pe, 0xffffffff;\n"
-        "setp.ne.b32 p, %6, 0;\n"
-        "@pe tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n"
-        "}\n"
-        ::"r"(d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-        : "memory");
-}
 // arrives at the barrier of the same address in both CTAs once the products issued so far are done
 __device__ __forceinline__ void warp_commit_pair(uint64_t* bar) {
   asm volatile(
@@ -440,12 +464,12 @@ __device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t (&r)[3
   tmem_ld16_nowait(taddr + 16, r + 16);
 }
 
-// One warp's box of 32 tokens x 32 features: lane = feature, r[j] = token j.
+// One warp's 32 tokens x 32 features: lane = feature, r[j] = token j.
 template <typename T>
-__device__ __forceinline__ void box_to_smem(unsigned char* box, int lane, const uint32_t (&r)[32], float bias) {
+__device__ __forceinline__ void box_to_smem(unsigned char* box, int lane, const uint32_t* r, float bias) {
   T* out = reinterpret_cast<T*>(box) + lane;
 #pragma unroll
-  for (int j = 0; j < 32; ++j) out[j * 32] = from_float<T>(__uint_as_float(r[j]) + bias);
+  for (int j = 0; j < int(64 / sizeof(T)); ++j) out[j * 32] = from_float<T>(__uint_as_float(r[j]) + bias);
 }
 template <typename T>
 __device__ __forceinline__ void box_to_global(const Product& p, int m, int n, const uint32_t (&r)[32], float bias) {
@@ -455,6 +479,27 @@ __device__ __forceinline__ void box_to_global(const Product& p, int m, int n, co
   for (int j = 0; j < 32; ++j) {
     if (m + j < p.M) *out = from_float<T>(__uint_as_float(r[j]) + bias);
     out += p.N;
+  }
+}
+// Through shared memory to a TMA store, by turns from two boxes.
+template <typename T>
+__device__ __forceinline__ void box_by_tma(const CUtensorMap* map, unsigned char* boxes, int& side, int lane, int m, int n0, int M,
+                                           const uint32_t (&r)[32], float bias) {
+  constexpr int TOKENS = 64 / sizeof(T);
+#pragma unroll
+  for (int h = 0; h < 32; h += TOKENS) {
+    if (m + h >= M) break;
+    unsigned char* out = boxes + side * PairLayout::OUT_BYTES;
+    side ^= 1;
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");      // the box's last store has been read
+    __syncwarp();
+    box_to_smem<T>(out, lane, r + h, bias);
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_2d(map, out, n0, m + h);
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
   }
 }
 
@@ -472,7 +517,8 @@ mx_pair_kernel(const __grid_constant__ PairMaps maps, const Product p, int ftile
   uint64_t* empty = full + L::STAGES;
   uint64_t* sf_full = empty + L::STAGES;
   uint64_t* sf_empty = sf_full + 2;
-  uint64_t* acc_full = sf_empty + 2;
+  uint64_t* sf_peer = sf_empty + 2;
+  uint64_t* acc_full = sf_peer + 2;
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
 
@@ -487,7 +533,7 @@ mx_pair_kernel(const __grid_constant__ PairMaps maps, const Product p, int ftile
   if (threadIdx.x == 0) {
     for (int s = 0; s < L::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&sf_full[s], 8); mbar_init(&sf_empty[s], 1);       // four scale warps of each CTA
+      mbar_init(&sf_full[s], 4); mbar_init(&sf_empty[s], 1); mbar_init(&sf_peer[s], 1);
       mbar_init(&acc_full[s], 1); mbar_init(&acc_empty[s], 8);     // four epilogue warps of each CTA
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -532,24 +578,26 @@ mx_pair_kernel(const __grid_constant__ PairMaps maps, const Product p, int ftile
       int s = 0, b = 0, acc = 0;
       uint32_t ph = 0, sf_ph = 0, acc_ph = 0;
       for (int tile = pair; tile < tiles && ok; tile += pairs) {
-        ok = warp_mbar_wait(&acc_empty[acc], acc_ph ^ 1, 2);
-        if (!ok) break;
+        // acc_empty[a]: the epilogue has read the shared columns of accumulator a, which the other one starts or ends with;
+        // its own columns were read before that of the tile in between
+        if (tile != pair) {
+          ok = warp_mbar_wait(&acc_empty[acc ^ 1], acc_ph, 2);
+          if (!ok) break;
+          if (!acc) acc_ph ^= 1u;
+        }
         tc_fence_after();
-        const uint32_t d = tmem + acc * PAIR_TOKENS;
+        const uint32_t d = tmem + acc * L::ACC_STRIDE;
         uint32_t accumulate = 0;
         int kt = 0;
         for (int step = 0; step < steps && ok; ++step) {
-          ok = warp_mbar_wait(&sf_full[b], sf_ph, 2);
+          ok = warp_mbar_wait(&sf_full[b], sf_ph, 2) && warp_mbar_wait(&sf_peer[b], sf_ph, 2);
           if (!ok) break;
-          tc_fence_after();
+          fence_proxy_async_smem();                     // here and not in the loading warps: it waits for loads in flight
           const uint32_t sfa = tmem + L::SCALE_BASE + b * L::SCALE_COLS, sfb = sfa + CHUNKS * 4;
           const uint64_t sdesc = sdesc0 + uint64_t((b * L::SCALES) >> 4);
-#pragma unroll
-          for (int j = 0; j < CHUNKS; ++j) {
-            warp_copy_scales<2>(sfa + 4 * j, sdesc + uint64_t((j * SCALE_TILE) >> 4));
-            warp_copy_scales<2>(sfb + L::X_COLS * j, sdesc + uint64_t(((CHUNKS + j) * SCALE_TILE) >> 4));
-            warp_copy_scales<2>(sfb + L::X_COLS * j + 4, sdesc + uint64_t(((2 * CHUNKS + j) * SCALE_TILE) >> 4));
-          }
+          warp_copy_scales<2, 4>(sfa, sdesc);
+          warp_copy_scales<2, L::X_COLS>(sfb, sdesc + uint64_t((CHUNKS * SCALE_TILE) >> 4));
+          warp_copy_scales<2, L::X_COLS>(sfb + 4, sdesc + uint64_t((2 * CHUNKS * SCALE_TILE) >> 4));
           warp_commit_pair(&sf_empty[b]);
 #pragma unroll
           for (int i = 0; i < STAGES_PER_STEP; ++i, ++kt) {
@@ -558,14 +606,13 @@ mx_pair_kernel(const __grid_constant__ PairMaps maps, const Product p, int ftile
             if (!ok) break;
             tc_fence_after();
             const uint64_t a = desc0 + uint64_t(uint32_t(s) * uint32_t(L::STAGE >> 4)), x = a + (L::W_BYTES >> 4);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const int j = XF == NES_MXFP4 ? i * 2 + (k >> 1) : i;
-              const uint32_t id = XF == NES_MXFP4 ? (k & 1) * 2 : k;
-              if (XF != NES_MXFP4 || kt * 2 + (k >> 1) < p.groups)
-                warp_mma_scaled_pair<XF, WF>(d, a + 2 * k, x + 2 * k, idesc | scale_byte(id), sfa + 4 * j, sfb + L::X_COLS * j, accumulate);
-              accumulate = 1;
-            }
+            const int j = i * STAGE_GROUPS;
+            if (STAGE_GROUPS == 1 || kt * 2 + 1 < p.groups)
+              warp_mma_stage<XF, 2>(d, a, x, idesc, sfa + 4 * j, sfb + L::X_COLS * j, sfa + 4 * (j + STAGE_GROUPS - 1),
+                                    sfb + L::X_COLS * (j + STAGE_GROUPS - 1), accumulate);
+            else
+              warp_mma_stage<XF, 2, true>(d, a, x, idesc, sfa + 4 * j, sfb + L::X_COLS * j, 0u, 0u, accumulate);
+            accumulate = 1;
             warp_commit_pair(&empty[s]);
             if (++s == L::STAGES) { s = 0; ph ^= 1u; }
           }
@@ -573,40 +620,48 @@ mx_pair_kernel(const __grid_constant__ PairMaps maps, const Product p, int ftile
           b ^= 1;
         }
         warp_commit_pair(&acc_full[acc]);
-        if (acc) acc_ph ^= 1u;
         acc ^= 1;
+      }
+    } else {
+      // tells the leading CTA of this CTA's scales: a signal across CTAs also waits for its thread's loads in flight
+      const uint32_t sf_peer0 = map_rank(smem_u32(sf_peer), 0);
+      const int64_t total = pair < tiles ? int64_t((tiles - 1 - pair) / pairs + 1) * steps : 0;
+      for (int64_t i = 0; i < total && ok; ++i) {
+        ok = warp_mbar_wait(&sf_full[i & 1], uint32_t(i >> 1) & 1u, 2);
+        if (!ok) break;
+        fence_proxy_async_smem();
+        if (lane == 0) mbar_arrive_cluster(sf_peer0 + uint32_t(i & 1) * 8u);
+        __syncwarp();
       }
     }
   } else if (warp < 6) {
-    const uint32_t sf_full0 = map_rank(smem_u32(sf_full), 0);
     const int t = threadIdx.x - 64, row = scale_row(t);
-    uint4 v[2][3];                                   // two steps in flight
+    uint4 v[4][3];                                   // four steps in flight
     int tile = pair, step = 0;                       // of the next load
     auto load = [&](uint4 (&o)[3]) {
       if (tile >= tiles) return;
       const int n0 = (tile % ftiles) * PAIR_FEATURES + rank * FEATURES, m0 = (tile / ftiles) * PAIR_TOKENS;
       o[0] = load_scale_words(p.w_scales, n0 + row, p.N, step * CHUNKS, p.groups, p.vec_scales);
       o[1] = load_scale_words(p.x_scales, m0 + row, p.M, step * CHUNKS, p.groups, p.vec_scales);
-      o[2] = load_scale_words(p.x_scales, row < PAIR_TOKENS - 128 ? m0 + 128 + row : p.M, p.M, step * CHUNKS, p.groups, p.vec_scales);
+      o[2] = load_scale_words(p.x_scales, m0 + 128 + row, p.M, step * CHUNKS, p.groups, p.vec_scales);
       if (++step == steps) { step = 0; tile += pairs; }
     };
-    load(v[0]);
-    load(v[1]);
-    const int64_t total = pair < tiles ? int64_t((tiles - 1 - pair) / pairs + 1) * steps : 0;
-    uint32_t ph = 1;
-    for (int64_t i = 0; i < total && ok; i += 2, ph ^= 1u) {
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        if (i + b >= total) break;
-        ok = warp_mbar_wait(&sf_empty[b], ph, 4);
+    for (int i = 0; i < 4; ++i) load(v[i]);
+    const int64_t total = pair < tiles ? int64_t((tiles - 1 - pair) / pairs + 1) * steps : 0;
+    for (int64_t i = 0; i < total && ok; i += 4) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (i + u >= total) break;
+        const int b = u & 1;
+        ok = warp_mbar_wait(&sf_empty[b], u < 2 ? 1u : 0u, 4);
         if (!ok) break;
         unsigned char* to = scale_tiles + b * L::SCALES;
 #pragma unroll
-        for (int h = 0; h < 3; ++h) put_scale_words(to + h * CHUNKS * SCALE_TILE, t, v[b][h]);
-        fence_proxy_async_smem();
+        for (int h = 0; h < 3; ++h) put_scale_words(to + h * CHUNKS * SCALE_TILE, t, v[u][h]);
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(sf_full0 + b * 8);
-        load(v[b]);
+        if (lane == 0) mbar_arrive(&sf_full[b]);
+        load(v[u]);
       }
     }
   } else {
@@ -623,38 +678,38 @@ mx_pair_kernel(const __grid_constant__ PairMaps maps, const Product p, int ftile
       tc_fence_after();
       const bool good = __all_sync(0xffffffffu, timeouts_so_far() == timeouts_at_start);
       const float bias = p.bias && n0 + lane < p.N ? __ldg(p.bias + n0 + lane) : 0.f;
+      // the columns shared with the other accumulator first: the last 96 of accumulator 0, the first of accumulator 1
+      const int first = acc ? 0 : L::ACC_STRIDE;
 #pragma unroll 1
-      for (int c = 0; c < PAIR_TOKENS; c += L::OUT_TOKENS) {
-        if (m0 + c >= p.M) break;
-        uint32_t r[32];
-        tmem_ld32_nowait(tmem + lanes + acc * PAIR_TOKENS + c, r);
-        tmem_ld_wait();
-        if (!good || n0 >= p.N) continue;
-        if (tma_out) {
-          unsigned char* out = box + side * L::OUT_BYTES;
-          side ^= 1;
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");      // the box's last store has been read
-          __syncwarp();
-          if (p.y_dtype == NES_F32) box_to_smem<float>(out, lane, r, bias);
-          else if (p.y_dtype == NES_BF16) box_to_smem<__nv_bfloat16>(out, lane, r, bias);
-          else box_to_smem<__half>(out, lane, r, bias);
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_2d(&maps.y, out, n0, m0 + c);
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      for (int i = 0; i < PAIR_TOKENS; i += 32) {
+        const int c = (first + i) & (PAIR_TOKENS - 1);
+        if (m0 + c < p.M) {
+          uint32_t r[32];
+          tmem_ld32_nowait(tmem + lanes + acc * L::ACC_STRIDE + c, r);
+          tmem_ld_wait();
+          if (i == L::SHARED_COLS - 32) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(acc_empty0 + acc * 8);
           }
-        } else if (p.y_dtype == NES_F32) {
-          box_to_global<float>(p, m0 + c, n0 + lane, r, bias);
-        } else if (p.y_dtype == NES_BF16) {
-          box_to_global<__nv_bfloat16>(p, m0 + c, n0 + lane, r, bias);
-        } else {
-          box_to_global<__half>(p, m0 + c, n0 + lane, r, bias);
+          if (!good || n0 >= p.N) continue;
+          if (tma_out) {
+            if (p.y_dtype == NES_F32) box_by_tma<float>(&maps.y, box, side, lane, m0 + c, n0, p.M, r, bias);
+            else if (p.y_dtype == NES_BF16) box_by_tma<__nv_bfloat16>(&maps.y, box, side, lane, m0 + c, n0, p.M, r, bias);
+            else box_by_tma<__half>(&maps.y, box, side, lane, m0 + c, n0, p.M, r, bias);
+          } else if (p.y_dtype == NES_F32) {
+            box_to_global<float>(p, m0 + c, n0 + lane, r, bias);
+          } else if (p.y_dtype == NES_BF16) {
+            box_to_global<__nv_bfloat16>(p, m0 + c, n0 + lane, r, bias);
+          } else {
+            box_to_global<__half>(p, m0 + c, n0 + lane, r, bias);
+          }
+        } else if (i == L::SHARED_COLS - 32) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(acc_empty0 + acc * 8);
         }
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(acc_empty0 + acc * 8);
       if (acc) ph ^= 1u;
       acc ^= 1;
     }
@@ -731,7 +786,7 @@ static int launch_pair(const Product& p, const void* x, const void* w, cudaStrea
   if (tma_out) {
     cuuint64_t dims[2] = {(cuuint64_t)p.N, (cuuint64_t)p.M};
     cuuint64_t strides[1] = {cuuint64_t(p.N) * size};
-    cuuint32_t box[2] = {32, (cuuint32_t)L::OUT_TOKENS};
+    cuuint32_t box[2] = {32, cuuint32_t(64 / size)};
     cuuint32_t estr[2] = {1, 1};
     const CUtensorMapDataType type = p.y_dtype == NES_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                      : p.y_dtype == NES_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;

@@ -245,6 +245,12 @@ def test_linear(rows, cols, outs, activations, weights):
 
 
 @pytest.mark.parametrize("activations,weights", PAIRS)
+@pytest.mark.parametrize("rows,cols,outs", [(2100, 128, 5000), (1300, 1160, 7000), (4500, 700, 2305)])
+def test_linear_more_tiles_than_processors(rows, cols, outs, activations, weights):
+    test_linear(rows, cols, outs, activations, weights)
+
+
+@pytest.mark.parametrize("activations,weights", PAIRS)
 @pytest.mark.parametrize("rows", [1, 16, 40, 150])
 def test_linear_special_scales(rows, activations, weights):
     """A NaN block poisons its own row or column only; scales at both ends of the range meet without overflow."""
