@@ -503,9 +503,17 @@ __device__ __forceinline__ void box_by_tma(const CUtensorMap* map, unsigned char
   }
 }
 
+// Order of the tiles: eight feature tiles wide down all tokens, so that the pairs that run together share both operands' rows.
+constexpr int RASTER = 4;
+__device__ __forceinline__ int2 tile_place(int tile, int ftiles, int ttiles) {
+  const int column = tile / (RASTER * ttiles), within = tile - column * RASTER * ttiles;
+  const int wide = min(RASTER, ftiles - column * RASTER), t = within / wide;
+  return make_int2(column * RASTER + within - t * wide, t);
+}
+
 template <int XF, int WF>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS_PAIR, 1)
-mx_pair_kernel(const __grid_constant__ PairMaps maps, const Product p, int ftiles, int tiles, int tma_out) {
+mx_pair_kernel(const __grid_constant__ PairMaps maps, const Product p, int ftiles, int ttiles, int tma_out) {
   using L = PairLayout;
   extern __shared__ unsigned char dyn_raw[];
   const unsigned int timeouts_at_start = timeouts_so_far();
@@ -524,7 +532,7 @@ mx_pair_kernel(const __grid_constant__ PairMaps maps, const Product p, int ftile
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = int(cluster_rank());
-  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, tiles = ftiles * ttiles;
   constexpr int STAGE_GROUPS = XF == NES_MXFP4 ? 2 : 1;
   constexpr int STAGES_PER_STEP = CHUNKS / STAGE_GROUPS;
   const int steps = (p.groups + CHUNKS - 1) / CHUNKS;
@@ -556,7 +564,8 @@ mx_pair_kernel(const __grid_constant__ PairMaps maps, const Product p, int ftile
       int s = 0;
       uint32_t ph = 0;
       for (int tile = pair; tile < tiles && ok; tile += pairs) {
-        const int n0 = (tile % ftiles) * PAIR_FEATURES + rank * FEATURES, m0 = (tile / ftiles) * PAIR_TOKENS + rank * (PAIR_TOKENS / 2);
+        const int2 at = tile_place(tile, ftiles, ttiles);
+        const int n0 = at.x * PAIR_FEATURES + rank * FEATURES, m0 = at.y * PAIR_TOKENS + rank * (PAIR_TOKENS / 2);
         for (int kt = 0; kt < kts; ++kt) {
           ok = mbar_wait(&empty[s], ph ^ 1, 1);
           if (!ok) break;
@@ -640,7 +649,8 @@ mx_pair_kernel(const __grid_constant__ PairMaps maps, const Product p, int ftile
     int tile = pair, step = 0;                       // of the next load
     auto load = [&](uint4 (&o)[3]) {
       if (tile >= tiles) return;
-      const int n0 = (tile % ftiles) * PAIR_FEATURES + rank * FEATURES, m0 = (tile / ftiles) * PAIR_TOKENS;
+      const int2 at = tile_place(tile, ftiles, ttiles);
+      const int n0 = at.x * PAIR_FEATURES + rank * FEATURES, m0 = at.y * PAIR_TOKENS;
       o[0] = load_scale_words(p.w_scales, n0 + row, p.N, step * CHUNKS, p.groups, p.vec_scales);
       o[1] = load_scale_words(p.x_scales, m0 + row, p.M, step * CHUNKS, p.groups, p.vec_scales);
       o[2] = load_scale_words(p.x_scales, m0 + 128 + row, p.M, step * CHUNKS, p.groups, p.vec_scales);
@@ -672,43 +682,50 @@ mx_pair_kernel(const __grid_constant__ PairMaps maps, const Product p, int ftile
     int acc = 0, side = 0;
     uint32_t ph = 0;
     for (int tile = pair; tile < tiles; tile += pairs) {
-      const int n0 = (tile % ftiles) * PAIR_FEATURES + rank * FEATURES + q * 32, m0 = (tile / ftiles) * PAIR_TOKENS;
+      const int2 at = tile_place(tile, ftiles, ttiles);
+      const int n0 = at.x * PAIR_FEATURES + rank * FEATURES + q * 32, m0 = at.y * PAIR_TOKENS;
       ok = warp_mbar_wait(&acc_full[acc], ph, 3);
       if (!ok) break;
       tc_fence_after();
       const bool good = __all_sync(0xffffffffu, timeouts_so_far() == timeouts_at_start);
       const float bias = p.bias && n0 + lane < p.N ? __ldg(p.bias + n0 + lane) : 0.f;
-      // the columns shared with the other accumulator first: the last 96 of accumulator 0, the first of accumulator 1
-      const int first = acc ? 0 : L::ACC_STRIDE;
-#pragma unroll 1
-      for (int i = 0; i < PAIR_TOKENS; i += 32) {
-        const int c = (first + i) & (PAIR_TOKENS - 1);
-        if (m0 + c < p.M) {
-          uint32_t r[32];
-          tmem_ld32_nowait(tmem + lanes + acc * L::ACC_STRIDE + c, r);
-          tmem_ld_wait();
-          if (i == L::SHARED_COLS - 32) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(acc_empty0 + acc * 8);
-          }
-          if (!good || n0 >= p.N) continue;
-          if (tma_out) {
-            if (p.y_dtype == NES_F32) box_by_tma<float>(&maps.y, box, side, lane, m0 + c, n0, p.M, r, bias);
-            else if (p.y_dtype == NES_BF16) box_by_tma<__nv_bfloat16>(&maps.y, box, side, lane, m0 + c, n0, p.M, r, bias);
-            else box_by_tma<__half>(&maps.y, box, side, lane, m0 + c, n0, p.M, r, bias);
-          } else if (p.y_dtype == NES_F32) {
-            box_to_global<float>(p, m0 + c, n0 + lane, r, bias);
-          } else if (p.y_dtype == NES_BF16) {
-            box_to_global<__nv_bfloat16>(p, m0 + c, n0 + lane, r, bias);
-          } else {
-            box_to_global<__half>(p, m0 + c, n0 + lane, r, bias);
-          }
-        } else if (i == L::SHARED_COLS - 32) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(acc_empty0 + acc * 8);
+      auto emit = [&](int c, const uint32_t (&r)[32]) {
+        if (!good || n0 >= p.N || m0 + c >= p.M) return;
+        if (tma_out) {
+          if (p.y_dtype == NES_F32) box_by_tma<float>(&maps.y, box, side, lane, m0 + c, n0, p.M, r, bias);
+          else if (p.y_dtype == NES_BF16) box_by_tma<__nv_bfloat16>(&maps.y, box, side, lane, m0 + c, n0, p.M, r, bias);
+          else box_by_tma<__half>(&maps.y, box, side, lane, m0 + c, n0, p.M, r, bias);
+        } else if (p.y_dtype == NES_F32) {
+          box_to_global<float>(p, m0 + c, n0 + lane, r, bias);
+        } else if (p.y_dtype == NES_BF16) {
+          box_to_global<__nv_bfloat16>(p, m0 + c, n0 + lane, r, bias);
+        } else {
+          box_to_global<__half>(p, m0 + c, n0 + lane, r, bias);
         }
+      };
+      // the columns shared with the other accumulator go to registers and are handed over before anything else: the
+      // last 96 of accumulator 0, the first of accumulator 1
+      const uint32_t from = tmem + lanes + acc * L::ACC_STRIDE;
+      const int first = acc ? 0 : L::ACC_STRIDE;
+      {
+        uint32_t r[3][32];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) tmem_ld32_nowait(from + first + 32 * i, r[i]);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(acc_empty0 + acc * 8);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) emit(first + 32 * i, r[i]);
+      }
+#pragma unroll 1
+      for (int i = L::SHARED_COLS; i < PAIR_TOKENS; i += 32) {
+        const int c = (first + i) & (PAIR_TOKENS - 1);
+        if (m0 + c >= p.M) continue;
+        uint32_t r[32];
+        tmem_ld32_nowait(from + c, r);
+        tmem_ld_wait();
+        emit(c, r);
       }
       if (acc) ph ^= 1u;
       acc ^= 1;
@@ -794,13 +811,13 @@ static int launch_pair(const Product& p, const void* x, const void* w, cudaStrea
                              CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     NES_REQUIRE(r == CUDA_SUCCESS, NES_ERR_LAUNCH, "mx_linear_fwd: cuTensorMapEncodeTiled failed with %d", (int)r);
   }
-  const int64_t ftiles = ceil_div<int64_t>(p.N, PAIR_FEATURES), tiles = ftiles * ceil_div<int64_t>(p.M, PAIR_TOKENS);
-  NES_REQUIRE(tiles <= INT32_MAX / 2, NES_ERR_UNSUPPORTED, "mx_linear_fwd: too large");
+  const int64_t ftiles = ceil_div<int64_t>(p.N, PAIR_FEATURES), ttiles = ceil_div<int64_t>(p.M, PAIR_TOKENS), tiles = ftiles * ttiles;
+  NES_REQUIRE(tiles <= INT32_MAX / 16, NES_ERR_UNSUPPORTED, "mx_linear_fwd: too large");
   const auto kernel = mx_pair_kernel<XF, WF>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::SMEM);
   if (e != cudaSuccess) return fail(NES_ERR_LAUNCH, "mx_linear_fwd: shared memory opt-in failed: %s", cudaGetErrorString(e));
   const int64_t pairs = tiles < sm_count() / 2 ? tiles : sm_count() / 2;
-  kernel<<<unsigned(pairs * 2), THREADS_PAIR, L::SMEM, st>>>(maps, p, int(ftiles), int(tiles), tma_out);
+  kernel<<<unsigned(pairs * 2), THREADS_PAIR, L::SMEM, st>>>(maps, p, int(ftiles), int(ttiles), tma_out);
   return check_launch("mx_linear_fwd");
 }
 
