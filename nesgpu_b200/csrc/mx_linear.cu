@@ -758,6 +758,28 @@ static int code_map(CUtensorMap* map, const void* base, int64_t rows, int64_t gr
   return NES_OK;
 }
 
+// CTAs that share a tile's K: as many as fill the SMs once, each with a step of its own at least
+static int choose_splits(int64_t tiles, int steps) {
+  int splits = 1;
+  while (splits < 8 && splits * 2 <= steps && tiles * splits * 2 <= sm_count()) splits *= 2;
+  return splits;
+}
+
+// Raises a kernel's dynamic shared memory limit once per device.
+template <auto KERNEL>
+static int allow_smem(size_t bytes) {
+  static unsigned long long done = 0;                      // one bit per device, one word per kernel
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  const unsigned long long bit = 1ULL << (dev & 63);
+  if (e == cudaSuccess && (dev > 63 || !(__atomic_load_n(&done, __ATOMIC_RELAXED) & bit))) {
+    e = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess && dev <= 63) __atomic_fetch_or(&done, bit, __ATOMIC_RELAXED);
+  }
+  NES_REQUIRE(e == cudaSuccess, NES_ERR_LAUNCH, "mx_linear_fwd: shared memory opt-in failed: %s", cudaGetErrorString(e));
+  return NES_OK;
+}
+
 template <int XF, int WF, int TOKENS>
 static int launch_product(const Product& p, const void* x, const void* w, cudaStream_t st) {
   using L = Layout<TOKENS>;
@@ -767,13 +789,9 @@ static int launch_product(const Product& p, const void* x, const void* w, cudaSt
   if ((rc = code_map(&maps.x, x, p.M, p.groups, XF == NES_MXFP4, false, TOKENS)) != NES_OK) return rc;
   const int64_t ftiles = ceil_div<int64_t>(p.N, FEATURES), ttiles = ceil_div<int64_t>(p.M, TOKENS);
   const int steps = ceil_div(p.groups, CHUNKS);
-  int splits = 1;
-  if (TOKENS <= 128)
-    while (splits < 8 && splits * 2 <= steps && ftiles * ttiles * splits * 2 <= sm_count()) splits *= 2;
+  const int splits = choose_splits(ftiles * ttiles, steps);
   NES_REQUIRE(ttiles <= 65535 && ftiles * splits <= INT32_MAX, NES_ERR_UNSUPPORTED, "mx_linear_fwd: too large");
-  const auto kernel = mx_product_kernel<XF, WF, TOKENS>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::SMEM);
-  if (e != cudaSuccess) return fail(NES_ERR_LAUNCH, "mx_linear_fwd: shared memory opt-in failed: %s", cudaGetErrorString(e));
+  if ((rc = allow_smem<mx_product_kernel<XF, WF, TOKENS>>(L::SMEM)) != NES_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(ftiles * splits), unsigned(ttiles));
   cfg.blockDim = dim3(THREADS_TC);
@@ -785,7 +803,7 @@ static int launch_product(const Product& p, const void* x, const void* w, cudaSt
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, kernel, maps, p, splits);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, mx_product_kernel<XF, WF, TOKENS>, maps, p, splits);
   if (e != cudaSuccess) return fail(NES_ERR_LAUNCH, "mx_linear_fwd: %s", cudaGetErrorString(e));
   return check_launch("mx_linear_fwd");
 }
@@ -813,11 +831,9 @@ static int launch_pair(const Product& p, const void* x, const void* w, cudaStrea
   }
   const int64_t ftiles = ceil_div<int64_t>(p.N, PAIR_FEATURES), ttiles = ceil_div<int64_t>(p.M, PAIR_TOKENS), tiles = ftiles * ttiles;
   NES_REQUIRE(tiles <= INT32_MAX / 16, NES_ERR_UNSUPPORTED, "mx_linear_fwd: too large");
-  const auto kernel = mx_pair_kernel<XF, WF>;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)L::SMEM);
-  if (e != cudaSuccess) return fail(NES_ERR_LAUNCH, "mx_linear_fwd: shared memory opt-in failed: %s", cudaGetErrorString(e));
+  if ((rc = allow_smem<mx_pair_kernel<XF, WF>>(L::SMEM)) != NES_OK) return rc;
   const int64_t pairs = tiles < sm_count() / 2 ? tiles : sm_count() / 2;
-  kernel<<<unsigned(pairs * 2), THREADS_PAIR, L::SMEM, st>>>(maps, p, int(ftiles), int(ttiles), tma_out);
+  mx_pair_kernel<XF, WF><<<unsigned(pairs * 2), THREADS_PAIR, L::SMEM, st>>>(maps, p, int(ftiles), int(ttiles), tma_out);
   return check_launch("mx_linear_fwd");
 }
 
@@ -826,8 +842,18 @@ static int launch_tokens(const Product& p, const void* x, const void* w, cudaStr
   if (p.M <= 16) return launch_product<XF, WF, 16>(p, x, w, st);
   if (p.M <= 32) return launch_product<XF, WF, 32>(p, x, w, st);
   if (p.M <= 64) return launch_product<XF, WF, 64>(p, x, w, st);
-  if (p.M <= 128) return launch_product<XF, WF, 128>(p, x, w, st);
-  return launch_pair<XF, WF>(p, x, w, st);
+  // Single CTAs on 128 x 128 tiles, or pairs on 256 x 256: what either takes in ns, from its waves over the SMs.  Measured
+  // with 8-bit activations: a wave of either kind takes 2.5 us per 1024 of K, a wave of single CTAs 4.5 us besides (its
+  // epilogue runs under nothing), the pairs 8 us in all.  512x4096x4096: 14.9 us single, 20.7 us in pairs; 1024x4096x4096:
+  // 28.0 and 21.8 us; 4-bit activations take 1.5 us per 1024 of K.
+  if (p.M > 128) {
+    const int64_t sms = sm_count(), k = int64_t(p.groups) * (XF == NES_MXFP4 ? 190 : 310);
+    const int64_t single = ceil_div<int64_t>(p.M, 128) * ceil_div(p.N, FEATURES), pairs = ceil_div<int64_t>(p.M, PAIR_TOKENS) * ceil_div(p.N, PAIR_FEATURES);
+    const int splits = choose_splits(single, ceil_div(p.groups, CHUNKS));
+    const int64_t single_ns = ceil_div<int64_t>(single * splits, sms) * (4500 + k / splits);
+    if (8000 + ceil_div<int64_t>(pairs, sms / 2) * k < single_ns) return launch_pair<XF, WF>(p, x, w, st);
+  }
+  return launch_product<XF, WF, 128>(p, x, w, st);
 }
 
 static int64_t align256(int64_t v) { return (v + 255) & ~int64_t(255); }
