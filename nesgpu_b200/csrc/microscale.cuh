@@ -60,67 +60,67 @@ __device__ __forceinline__ uint32_t float_to_pair(float a, float b, __half) {
   return w;
 }
 
-// Eight consecutive elements starting at column c of a row, zeros from column `cols` on.  vec: rows and base are
-// 16-byte aligned, so a unit that lies inside the row is one or two 128-bit loads.
-template <typename T>
-__device__ __forceinline__ void load_unit(const T* row, int64_t c, int64_t cols, bool vec, float (&v)[UNIT]) {
-  if (vec && c + UNIT <= cols) {
-    if (sizeof(T) == 4) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(row + c));
-      const float4 b = __ldg(reinterpret_cast<const float4*>(row + c) + 1);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    } else {
-      const uint4 a = __ldg(reinterpret_cast<const uint4*>(row + c));
-      const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-      using H = typename std::conditional<sizeof(T) == 4, __half, T>::type;
+// Eight consecutive elements starting at column c of a row whose start is 16-byte aligned and whose length is a multiple
+// of 16 bytes; zeros from column `cols` on (with fp32 rows a unit may lie half inside).
+__device__ __forceinline__ void load_unit(const float* row, int64_t c, int64_t cols, float (&v)[UNIT]) {
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+  if (c < cols) a = __ldg(reinterpret_cast<const float4*>(row + c));
+  if (c + 4 < cols) b = __ldg(reinterpret_cast<const float4*>(row + c) + 1);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+template <typename H>
+__device__ __forceinline__ void load_unit(const H* row, int64_t c, int64_t cols, float (&v)[UNIT]) {
+  uint4 a = make_uint4(0u, 0u, 0u, 0u);
+  if (c < cols) a = __ldg(reinterpret_cast<const uint4*>(row + c));
+  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 p = pair_to_float(w[i], H());
-        v[2 * i] = p.x;
-        v[2 * i + 1] = p.y;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < UNIT; ++i) v[i] = c + i < cols ? to_float<T>(row[c + i]) : 0.f;
+  for (int i = 0; i < 4; ++i) {
+    const float2 p = pair_to_float(w[i], H());
+    v[2 * i] = p.x;
+    v[2 * i + 1] = p.y;
   }
 }
-
-template <typename T>
-__device__ __forceinline__ void store_unit(T* row, int64_t c, int64_t cols, bool vec, const float (&v)[UNIT]) {
-  if (vec && c + UNIT <= cols) {
-    if (sizeof(T) == 4) {
-      float4* p = reinterpret_cast<float4*>(row + c);
-      p[0] = make_float4(v[0], v[1], v[2], v[3]);
-      p[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-      using H = typename std::conditional<sizeof(T) == 4, __half, T>::type;
-      *reinterpret_cast<uint4*>(row + c) = make_uint4(float_to_pair(v[0], v[1], H()), float_to_pair(v[2], v[3], H()),
-                                                      float_to_pair(v[4], v[5], H()), float_to_pair(v[6], v[7], H()));
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < UNIT; ++i) if (c + i < cols) row[c + i] = from_float<T>(v[i]);
-  }
+__device__ __forceinline__ void store_unit(float* row, int64_t c, int64_t cols, const float (&v)[UNIT]) {
+  if (c < cols) *reinterpret_cast<float4*>(row + c) = make_float4(v[0], v[1], v[2], v[3]);
+  if (c + 4 < cols) *reinterpret_cast<float4*>(row + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+template <typename H>
+__device__ __forceinline__ void store_unit(H* row, int64_t c, int64_t cols, const float (&v)[UNIT]) {
+  if (c < cols)
+    *reinterpret_cast<uint4*>(row + c) = make_uint4(float_to_pair(v[0], v[1], H()), float_to_pair(v[2], v[3], H()),
+                                                    float_to_pair(v[4], v[5], H()), float_to_pair(v[6], v[7], H()));
 }
 
-// Scale code of the block that this lane's unit and those of its three neighbours make up (all four lanes of the
-// quad take part).  The largest magnitude is found on the bit patterns, which order as the values do and put
-// infinities and NaNs on top.
+// Rows of any length and alignment are walked the other way round: the 32 lanes take 32 consecutive columns, so that every access
+// of a warp is one stretch of memory whatever its start, and a block is one such access.  v[i] is column c + 32 i.
+template <typename T, int N>
+__device__ __forceinline__ void load_stripes(const T* row, int64_t c, int64_t cols, float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = c + 32 * i < cols ? to_float<T>(row[c + 32 * i]) : 0.f;
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_stripes(T* row, int64_t c, int64_t cols, const float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) if (c + 32 * i < cols) row[c + 32 * i] = from_float<T>(v[i]);
+}
+
+// larger magnitude of the two, NaN if either is one
+__device__ __forceinline__ float max_magnitude(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  return r;
+}
+
+// Scale code of a block from the bits of its largest magnitude (a NaN or an infinity lies on top).
 template <int FORMAT>
-__device__ __forceinline__ uint32_t quad_scale_code(const float (&v)[UNIT]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < UNIT; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+__device__ __forceinline__ uint32_t scale_code(uint32_t m) {
   constexpr int EMAX = FORMAT == NES_MXFP4 ? 2 : 8;
   return m >= 0x7f800000u ? 255u : uint32_t(max(int(m >> 23) - EMAX, 0));
 }
 
-// 2^-e for a scale code below 255 (at most 253: a normal number)
-__device__ __forceinline__ float inverse_scale(uint32_t code) { return __uint_as_float((254u - code) << 23); }
+// 2^-e for a scale code below 255 (at most 253: a normal number); 0 for 255
+__device__ __forceinline__ float inverse_scale(uint32_t code) { return __uint_as_float(code == 255u ? 0u : (254u - code) << 23); }
 
 // 2^(code - 127), NaN for 255
 __device__ __forceinline__ float scale_value(uint32_t code) {
@@ -141,28 +141,70 @@ __device__ __forceinline__ uint32_t pack_e2m1x8(const float (&v)[UNIT]) {
       : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return r;
 }
-
-__device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
-  uint16_t lo, hi;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(lo) : "f"(a), "f"(b));
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(hi) : "f"(c), "f"(d));
-  return uint32_t(lo) | (uint32_t(hi) << 16);
+// byte of two e2m1 codes, a in the low half
+__device__ __forceinline__ uint32_t pack_e2m1x2(float a, float b) {
+  uint32_t r;
+  asm("{\n.reg .b8 b0, z;\nmov.b16 {b0, z}, 0;\ncvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\nmov.b32 %0, {b0, z, z, z};\n}\n" : "=r"(r) : "f"(a), "f"(b));
+  return r;
 }
 
-// Quantises this lane's unit of the block and stores its codes (4 or 8 bytes) and, from the block's first lane, the
-// scale.  unit: index within the padded row.  Every lane of the warp calls it; `store` is false for lanes without a unit.
+__device__ __forceinline__ uint32_t pack_e4m3x2(float a, float b) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) { return pack_e4m3x2(a, b) | (pack_e4m3x2(c, d) << 16); }
+
+// Quantises this lane's unit of a block that four neighbouring lanes hold (all lanes of the warp call it) and stores its codes
+// and, from the block's first lane, the scale.  unit: index within the padded row; `store` is false for lanes without one.
 template <int FORMAT>
 __device__ __forceinline__ void quantize_unit(float (&v)[UNIT], uint8_t* codes_row, uint8_t* scales_row, int64_t unit, bool store) {
-  const uint32_t code = quad_scale_code<FORMAT>(v);
-  const float inv = inverse_scale(code == 255u ? 127u : code);
+  float top = 0.f;
 #pragma unroll
-  for (int i = 0; i < UNIT; ++i) v[i] = code == 255u ? 0.f : v[i] * inv;
+  for (int i = 0; i < UNIT; ++i) top = max_magnitude(top, v[i]);
+  uint32_t m = __float_as_uint(top) & 0x7fffffffu;
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  const uint32_t code = scale_code<FORMAT>(m);
+  const float inv = inverse_scale(code);
+#pragma unroll
+  for (int i = 0; i < UNIT; ++i) v[i] *= inv;
   if (!store) return;
-  if (FORMAT == NES_MXFP4)
-    reinterpret_cast<uint32_t*>(codes_row)[unit] = pack_e2m1x8(v);
-  else
-    reinterpret_cast<uint2*>(codes_row)[unit] = make_uint2(pack_e4m3x4(v[0], v[1], v[2], v[3]), pack_e4m3x4(v[4], v[5], v[6], v[7]));
+  if (FORMAT == NES_MXFP4) {
+    const uint32_t q = pack_e2m1x8(v);
+    reinterpret_cast<uint32_t*>(codes_row)[unit] = code == 255u ? 0u : q;
+  } else {
+    const uint32_t lo = pack_e4m3x4(v[0], v[1], v[2], v[3]), hi = pack_e4m3x4(v[4], v[5], v[6], v[7]);
+    reinterpret_cast<uint2*>(codes_row)[unit] = make_uint2(code == 255u ? 0u : lo, code == 255u ? 0u : hi);
+  }
   if ((unit & 3) == 0) scales_row[unit >> 2] = uint8_t(code);
+}
+
+// The same for N blocks of 32 columns, one lane per column: blocks block0 ... block0 + N - 1 of the row, of which those below
+// `blocks` (the padded row's) are stored.  N is even.
+template <int FORMAT, int N>
+__device__ __forceinline__ void quantize_stripes(float (&v)[N], uint8_t* codes_row, uint8_t* scales_row, int64_t block0, int64_t blocks, int lane) {
+  uint32_t mine = 0;                                             // lane i keeps the scale of block i
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const uint32_t code = scale_code<FORMAT>(__reduce_max_sync(0xffffffffu, __float_as_uint(v[i]) & 0x7fffffffu));
+    v[i] = code == 255u ? 0.f : v[i] * inverse_scale(code);
+    if (lane == i) mine = code;
+  }
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {
+    if (FORMAT == NES_MXFP4) {
+      // two blocks at once: even lanes store the first one's bytes, odd lanes the second one's
+      const uint32_t b = pack_e2m1x2(v[i], v[i + 1]), o = __shfl_xor_sync(0xffffffffu, b, 1);
+      const int64_t block = block0 + i + (lane & 1);
+      if (block < blocks) codes_row[block * 16 + (lane >> 1)] = uint8_t(lane & 1 ? (o >> 4) | (b & 0xf0u) : (b & 15u) | (o << 4));
+    } else {
+      const uint32_t two = pack_e4m3x2(v[i], v[i + 1]);
+      if (block0 + i < blocks) codes_row[(block0 + i) * 32 + lane] = uint8_t(two);
+      if (block0 + i + 1 < blocks) codes_row[(block0 + i + 1) * 32 + lane] = uint8_t(two >> 8);
+    }
+  }
+  if (lane < N && block0 + lane < blocks) scales_row[block0 + lane] = uint8_t(mine);
 }
 
 // e4m3 bytes of four e2m1 codes (the low 16 bits of c): a byte look-up in the eight magnitudes, then the signs
@@ -179,16 +221,14 @@ __device__ __forceinline__ float2 e4m3x2_to_float(uint32_t two) {
   return pair_to_float(h2, __half());
 }
 
-// The eight element values of a unit of codes, before the scale.
+// The eight elements of a unit as e4m3 bytes, and their values before the scale.
 template <int FORMAT>
-__device__ __forceinline__ void unit_elements(const uint8_t* codes_row, int64_t unit, float (&v)[UNIT]) {
-  uint2 q;
-  if (FORMAT == NES_MXFP4) {
-    const uint32_t c = __ldg(reinterpret_cast<const uint32_t*>(codes_row) + unit);
-    q = make_uint2(e2m1x4_to_e4m3(c), e2m1x4_to_e4m3(c >> 16));
-  } else {
-    q = __ldg(reinterpret_cast<const uint2*>(codes_row) + unit);
-  }
+__device__ __forceinline__ uint2 load_codes(const uint8_t* codes_row, int64_t unit) {
+  if (FORMAT == NES_MXFP8) return __ldg(reinterpret_cast<const uint2*>(codes_row) + unit);
+  const uint32_t c = __ldg(reinterpret_cast<const uint32_t*>(codes_row) + unit);
+  return make_uint2(e2m1x4_to_e4m3(c), e2m1x4_to_e4m3(c >> 16));
+}
+__device__ __forceinline__ void unit_elements(const uint2& q, float (&v)[UNIT]) {
   const uint32_t half[4] = {q.x, q.x >> 16, q.y, q.y >> 16};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {

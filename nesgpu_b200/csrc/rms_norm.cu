@@ -4,9 +4,10 @@
 //   y = h * rsqrt(mean(h^2) + eps) * (gain + s(r) * noise[d])     row = r * members + d
 //
 // One pass: a row stays in registers between the sum of squares and the scaling, so x and the residual are read once
-// and h and y written once.  A group of THREADS threads owns a row (a warp for short rows, a block for longer ones)
-// and holds UNITS units of eight columns per thread; rows longer than that take the looping kernel, which reads x and
-// the residual a second time.
+// and h and y written once.  THREADS threads own a row (a warp for short rows, a block for longer ones) and hold UNITS
+// units of eight columns each; rows longer than that take the looping kernel, which reads x and the residual a second
+// time.  A unit is eight consecutive columns, or (STRIPES: rows that are not whole 16-byte pieces) one column in each of
+// eight consecutive blocks of 32, a lane per column, so that any row start is read and written in whole lines.
 #include <type_traits>
 #include "microscale.cuh"
 
@@ -25,7 +26,6 @@ struct NormArgs {
   int antithetic;
   float eps;
   double inv_cols;
-  bool vec, vec_gain;
 };
 
 // 1 / sqrt(v) as hi + lo: one Newton step on the hardware's approximation.  A reciprocal root that is zero or
@@ -41,64 +41,84 @@ __device__ __forceinline__ float2 rsqrt_pair(double v) {
 // value exactly on a border does not occur except for a zero.  Otherwise the result is rounded to nearest.
 template <bool SHARP>
 __device__ __forceinline__ float scaled(float h, float2 r, float g) {
-  const float t = h * r.x, te = fmaf(h, r.y, fmaf(h, r.x, -t));
-  const float p = t * g, c = fmaf(te, g, fmaf(t, g, -p));
+  const float s = r.x * g, se = fmaf(r.y, g, fmaf(r.x, g, -s));
+  const float p = h * s, c = fmaf(h, se, fmaf(h, s, -p));
   if (SHARP) return __uint_as_float(__float_as_uint(__fadd_rz(p, c)) | 1u);
-  return fabsf(p) < 3.0e38f && fabsf(t) < 3.0e38f ? p + c : p;       // infinities have no error terms
+  return fabsf(p) < 3.0e38f && fabsf(s) < 3.0e38f ? p + c : p;       // infinities have no error terms
 }
 
-__device__ __forceinline__ void load_gain(const NormArgs& a, int64_t row, int64_t c, float (&g)[UNIT]) {
-  if (a.gain) {
-    load_unit(a.gain, c, a.cols, a.vec_gain, g);
-  } else {
-#pragma unroll
-    for (int i = 0; i < UNIT; ++i) g[i] = 1.f;
-  }
-  if (a.noise) {
-    const int64_t d = row % a.members;
-    const float s = anti_sign(row / a.members, a.rows / a.members, a.antithetic);
-    float n[UNIT];
-    load_unit(a.noise + d * a.cols, c, a.cols, a.vec_gain, n);
-#pragma unroll
-    for (int i = 0; i < UNIT; ++i) g[i] = fmaf(s, n[i], g[i]);
-  }
+// Where a thread's unit u lies: its first column, and how the rest of the unit follows it.
+template <bool STRIPES, int THREADS>
+__device__ __forceinline__ int64_t unit_column(int t, int64_t u) {
+  if (STRIPES) return ((t >> 5) + u * (THREADS / 32)) * (32 * UNIT) + (t & 31);
+  return (t + u * THREADS) * UNIT;
+}
+template <bool STRIPES, typename T>
+__device__ __forceinline__ void get(const T* row, int64_t c, int64_t cols, float (&v)[UNIT]) {
+  if (STRIPES) load_stripes(row, c, cols, v); else load_unit(row, c, cols, v);
+}
+template <bool STRIPES, typename T>
+__device__ __forceinline__ void put(T* row, int64_t c, int64_t cols, const float (&v)[UNIT]) {
+  if (STRIPES) store_stripes(row, c, cols, v); else store_unit(row, c, cols, v);
 }
 
-template <typename T>
+// A row's member noise and its sign.
+struct RowNoise { const float* p; float sign; };
+__device__ __forceinline__ RowNoise row_noise(const NormArgs& a, int64_t row) {
+  if (!a.noise) return RowNoise{nullptr, 0.f};
+  const int64_t r = row / a.members, d = row - r * a.members;
+  return RowNoise{a.noise + d * a.cols, anti_sign(r, a.rows / a.members, a.antithetic)};
+}
+
+template <typename T, bool STRIPES>
 __device__ __forceinline__ void load_h(const NormArgs& a, int64_t row, int64_t c, float (&v)[UNIT]) {
-  load_unit(static_cast<const T*>(a.x) + row * a.cols, c, a.cols, a.vec, v);
+  get<STRIPES>(static_cast<const T*>(a.x) + row * a.cols, c, a.cols, v);
   if (a.residual) {
     float q[UNIT];
-    load_unit(static_cast<const T*>(a.residual) + row * a.cols, c, a.cols, a.vec, q);
+    get<STRIPES>(static_cast<const T*>(a.residual) + row * a.cols, c, a.cols, q);
 #pragma unroll
     for (int i = 0; i < UNIT; ++i) v[i] += q[i];
   }
 }
 
-// y of one unit; every lane of the warp calls it for a quantised output
-template <typename T, int OUT>
-__device__ __forceinline__ void emit(const NormArgs& a, int64_t row, int64_t unit, int64_t units, const float (&h)[UNIT], float2 r) {
-  float y[UNIT];
-  const bool on = unit < units;
-  if (on) {
-    float g[UNIT];
-    load_gain(a, row, unit * UNIT, g);
-#pragma unroll
-    for (int i = 0; i < UNIT; ++i) y[i] = scaled<OUT != 0>(h[i], r, g[i]);
+// y of the unit at column c; all lanes of a warp call it
+template <typename T, int OUT, bool STRIPES>
+__device__ __forceinline__ void emit(const NormArgs& a, const RowNoise& noise, int64_t row, int64_t c, const float (&h)[UNIT], float2 r) {
+  float g[UNIT], y[UNIT];
+  if (a.gain) {
+    get<STRIPES>(a.gain, c, a.cols, g);
   } else {
 #pragma unroll
-    for (int i = 0; i < UNIT; ++i) y[i] = 0.f;
+    for (int i = 0; i < UNIT; ++i) g[i] = 1.f;
   }
+  if (noise.p) {
+    float n[UNIT];
+    get<STRIPES>(noise.p, c, a.cols, n);
+#pragma unroll
+    for (int i = 0; i < UNIT; ++i) g[i] = fmaf(noise.sign, n[i], g[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < UNIT; ++i) y[i] = scaled<OUT != 0>(h[i], r, g[i]);
   if (OUT == 0) {
-    if (on) store_unit(static_cast<T*>(a.y) + row * a.cols, unit * UNIT, a.cols, a.vec, y);
-  } else {
-    if (on && (unit + 1) * UNIT > a.cols) {      // pad columns are zero whatever the row's scale (0 * inf is not)
-#pragma unroll
-      for (int i = 0; i < UNIT; ++i) if (unit * UNIT + i >= a.cols) y[i] = 0.f;
-    }
-    quantize_unit<OUT == 0 ? NES_MXFP8 : OUT>(y, static_cast<uint8_t*>(a.y) + row * code_pitch(a.cols, OUT),
-                                              a.scales + row * scale_pitch(a.cols), unit, on);
+    put<STRIPES>(static_cast<T*>(a.y) + row * a.cols, c, a.cols, y);
+    return;
   }
+  // columns of the padding are zero whatever the row's scale (0 * inf is not)
+  constexpr int FORMAT = OUT == 0 ? NES_MXFP8 : OUT, APART = STRIPES ? 32 : 1;
+  if (c + (UNIT - 1) * APART >= a.cols) {
+#pragma unroll
+    for (int i = 0; i < UNIT; ++i) if (c + i * APART >= a.cols) y[i] = 0.f;
+  }
+  uint8_t* codes = static_cast<uint8_t*>(a.y) + row * code_pitch(a.cols, FORMAT);
+  uint8_t* scales = a.scales + row * scale_pitch(a.cols);
+  if (STRIPES) quantize_stripes<FORMAT>(y, codes, scales, c / BLOCK, padded(a.cols) / BLOCK, int(c) & 31);
+  else quantize_unit<FORMAT>(y, codes, scales, c / UNIT, c < padded(a.cols));
+}
+
+template <int N>
+__device__ __forceinline__ double tree_sum(const double* p) {
+  if constexpr (N == 1) return p[0];
+  else return tree_sum<N / 2>(p) + tree_sum<N / 2>(p + N / 2);
 }
 
 // Sum over the THREADS threads that share a row (all of a block unless THREADS == 32), the same in every thread.  The
@@ -112,94 +132,89 @@ __device__ __forceinline__ double row_sum(float mine) {
     __shared__ double part[THREADS / 32];
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
     __syncthreads();
-    s = part[0];
-#pragma unroll
-    for (int i = 1; i < THREADS / 32; ++i) s += part[i];
+    s = tree_sum<THREADS / 32>(part);
   }
   return s;
 }
 
-template <typename T, int OUT, int THREADS, int UNITS>
+__device__ __forceinline__ float square_sum(const float (&v)[UNIT]) {
+  float q = 0.f;
+#pragma unroll
+  for (int i = 0; i < UNIT; ++i) q = fmaf(v[i], v[i], q);
+  return q;
+}
+
+template <typename T, int OUT, int THREADS, int UNITS, bool STRIPES>
 __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) rms_norm_kernel(const NormArgs a) {
   constexpr int ROWS = THREADS == 32 ? 4 : 1;
   const int64_t row = int64_t(blockIdx.x) * ROWS + (ROWS > 1 ? threadIdx.x / THREADS : 0);
   if (row >= a.rows) return;
   const int t = threadIdx.x % THREADS;
-  const int64_t units = OUT == 0 ? (a.cols + UNIT - 1) / UNIT : padded(a.cols) / UNIT;
   float v[UNITS][UNIT];
 #pragma unroll
-  for (int u = 0; u < UNITS; ++u) {
-    const int64_t c = int64_t(t + u * THREADS) * UNIT;
-    if (c < a.cols) {
-      load_h<T>(a, row, c, v[u]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < UNIT; ++i) v[u][i] = 0.f;
-    }
-  }
+  for (int u = 0; u < UNITS; ++u) load_h<T, STRIPES>(a, row, unit_column<STRIPES, THREADS>(t, u), v[u]);
+  const RowNoise noise = row_noise(a, row);
   float s = 0.f;
 #pragma unroll
-  for (int u = 0; u < UNITS; ++u) {
-    float q = 0.f;
+  for (int u = 0; u < UNITS; ++u) s += square_sum(v[u]);
+  if (a.h) {
 #pragma unroll
-    for (int i = 0; i < UNIT; ++i) q = fmaf(v[u][i], v[u][i], q);
-    s += q;
-    const int64_t c = int64_t(t + u * THREADS) * UNIT;
-    if (a.h && c < a.cols) store_unit(static_cast<T*>(a.h) + row * a.cols, c, a.cols, a.vec, v[u]);
+    for (int u = 0; u < UNITS; ++u) put<STRIPES>(static_cast<T*>(a.h) + row * a.cols, unit_column<STRIPES, THREADS>(t, u), a.cols, v[u]);
   }
   const float2 r = rsqrt_pair(row_sum<THREADS>(s) * a.inv_cols + double(a.eps));
 #pragma unroll
-  for (int u = 0; u < UNITS; ++u) emit<T, OUT>(a, row, t + u * THREADS, units, v[u], r);
+  for (int u = 0; u < UNITS; ++u) emit<T, OUT, STRIPES>(a, noise, row, unit_column<STRIPES, THREADS>(t, u), v[u], r);
 }
 
 // Rows of any length: the sum of squares in one loop over the row, the outputs in a second one.
-template <typename T, int OUT, int THREADS>
+template <typename T, int OUT, int THREADS, bool STRIPES>
 __global__ void __launch_bounds__(THREADS) rms_norm_long_kernel(const NormArgs a) {
   const int64_t row = blockIdx.x;
-  const int64_t units = OUT == 0 ? (a.cols + UNIT - 1) / UNIT : padded(a.cols) / UNIT;
+  const int64_t units = (padded(a.cols) + THREADS * UNIT - 1) / (THREADS * UNIT);
+  const RowNoise noise = row_noise(a, row);
   float s = 0.f;
-  for (int64_t c = int64_t(threadIdx.x) * UNIT; c < a.cols; c += THREADS * UNIT) {
+  for (int64_t u = 0; u < units; ++u) {
     float v[UNIT];
-    load_h<T>(a, row, c, v);
-    float q = 0.f;
-#pragma unroll
-    for (int i = 0; i < UNIT; ++i) q = fmaf(v[i], v[i], q);
-    s += q;
-    if (a.h) store_unit(static_cast<T*>(a.h) + row * a.cols, c, a.cols, a.vec, v);
+    const int64_t c = unit_column<STRIPES, THREADS>(threadIdx.x, u);
+    load_h<T, STRIPES>(a, row, c, v);
+    s += square_sum(v);
+    if (a.h) put<STRIPES>(static_cast<T*>(a.h) + row * a.cols, c, a.cols, v);
   }
   const float2 r = rsqrt_pair(row_sum<THREADS>(s) * a.inv_cols + double(a.eps));
-  for (int64_t u0 = 0; u0 < units; u0 += THREADS) {
-    const int64_t unit = u0 + threadIdx.x;
+  for (int64_t u = 0; u < units; ++u) {
     float v[UNIT];
-    if (unit * UNIT < a.cols) {
-      load_h<T>(a, row, unit * UNIT, v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < UNIT; ++i) v[i] = 0.f;
-    }
-    emit<T, OUT>(a, row, unit, units, v, r);
+    const int64_t c = unit_column<STRIPES, THREADS>(threadIdx.x, u);
+    load_h<T, STRIPES>(a, row, c, v);
+    emit<T, OUT, STRIPES>(a, noise, row, c, v, r);
   }
 }
 
-template <typename T, int OUT>
+template <typename T, int OUT, bool STRIPES>
 static void launch_norm(const NormArgs& a, cudaStream_t st) {
   const unsigned rows = unsigned(a.rows);
-  const int64_t units = padded(a.cols) / UNIT;
-  if (units <= 32) rms_norm_kernel<T, OUT, 32, 1><<<(rows + 3) / 4, 128, 0, st>>>(a);
-  else if (units <= 64) rms_norm_kernel<T, OUT, 32, 2><<<(rows + 3) / 4, 128, 0, st>>>(a);
-  else if (units <= 128) rms_norm_kernel<T, OUT, 32, 4><<<(rows + 3) / 4, 128, 0, st>>>(a);
-  else if (units <= 256) rms_norm_kernel<T, OUT, 128, 2><<<rows, 128, 0, st>>>(a);
-  else if (units <= 512) rms_norm_kernel<T, OUT, 128, 4><<<rows, 128, 0, st>>>(a);
-  else if (units <= 1024) rms_norm_kernel<T, OUT, 256, 4><<<rows, 256, 0, st>>>(a);
-  else if (units <= 2048) rms_norm_kernel<T, OUT, 512, 4><<<rows, 512, 0, st>>>(a);
-  else rms_norm_long_kernel<T, OUT, 512><<<rows, 512, 0, st>>>(a);
+  const int64_t cols = padded(a.cols);
+  if (cols <= 256) rms_norm_kernel<T, OUT, 32, 1, STRIPES><<<(rows + 3) / 4, 128, 0, st>>>(a);
+  else if (cols <= 512) rms_norm_kernel<T, OUT, 32, 2, STRIPES><<<(rows + 3) / 4, 128, 0, st>>>(a);
+  else if (cols <= 1024) rms_norm_kernel<T, OUT, 32, 4, STRIPES><<<(rows + 3) / 4, 128, 0, st>>>(a);
+  else if (cols <= 2048) rms_norm_kernel<T, OUT, 128, 2, STRIPES><<<rows, 128, 0, st>>>(a);
+  else if (cols <= 4096) rms_norm_kernel<T, OUT, 128, 4, STRIPES><<<rows, 128, 0, st>>>(a);
+  else if (cols <= 8192) rms_norm_kernel<T, OUT, 256, 4, STRIPES><<<rows, 256, 0, st>>>(a);
+  else if (cols <= 16384) rms_norm_kernel<T, OUT, 512, 4, STRIPES><<<rows, 512, 0, st>>>(a);
+  else rms_norm_long_kernel<T, OUT, 512, STRIPES><<<rows, 512, 0, st>>>(a);
+}
+
+template <typename T, int OUT>
+static void launch_norm_rows(const NormArgs& a, bool whole, cudaStream_t st) {
+  if (whole) launch_norm<T, OUT, false>(a, st); else launch_norm<T, OUT, true>(a, st);
 }
 
 template <typename T>
 static void launch_norm_out(const NormArgs& a, int format, cudaStream_t st) {
-  if (format == 0) launch_norm<T, 0>(a, st);
-  else if (format == NES_MXFP4) launch_norm<T, NES_MXFP4>(a, st);
-  else launch_norm<T, NES_MXFP8>(a, st);
+  const bool whole = (a.cols * sizeof(T)) % 16 == 0 && aligned16(a.x) && aligned16(a.residual) && aligned16(a.h) && aligned16(a.gain) &&
+                     aligned16(a.noise) && aligned16(a.y);
+  if (format == 0) launch_norm_rows<T, 0>(a, whole, st);
+  else if (format == NES_MXFP4) launch_norm_rows<T, NES_MXFP4>(a, whole, st);
+  else launch_norm_rows<T, NES_MXFP8>(a, whole, st);
 }
 
 }  // namespace mx
@@ -219,13 +234,10 @@ extern "C" int nes_rms_norm_fwd(const void* x, const void* residual, void* resid
   NES_REQUIRE(!noise || rows % members == 0, NES_ERR_BAD_ARG, "rms_norm_fwd: rows must be a multiple of members");
   NES_REQUIRE(rows <= INT32_MAX, NES_ERR_UNSUPPORTED, "rms_norm_fwd: too many rows");
   NES_REQUIRE(format == 0 || aligned16(y), NES_ERR_BAD_ARG, "rms_norm_fwd: codes must be 16-byte aligned");
-  const bool vec_rows = (cols * dtype_bytes(dtype)) % 16 == 0;
   NormArgs a;
   a.x = x; a.residual = residual; a.h = residual_out; a.gain = gain; a.noise = noise; a.y = y; a.scales = y_scales;
   a.rows = rows; a.cols = cols; a.members = members > 0 ? members : 1; a.antithetic = antithetic;
   a.eps = eps; a.inv_cols = 1.0 / double(cols);
-  a.vec = vec_rows && aligned16(x) && (!residual || (aligned16(residual) && aligned16(residual_out))) && (format != 0 || aligned16(y));
-  a.vec_gain = cols % 4 == 0 && (!gain || aligned16(gain)) && (!noise || aligned16(noise));
   cudaStream_t st = as_stream(stream);
   if (dtype == NES_F32) launch_norm_out<float>(a, format, st);
   else if (dtype == NES_BF16) launch_norm_out<__nv_bfloat16>(a, format, st);
