@@ -18,6 +18,7 @@ namespace mx {
 
 constexpr int BLOCK = 32;
 constexpr int GROUP = 128;         // row padding in elements
+constexpr int64_t LARGEST_EXTENT = 0x3fffffff;    // of rows and of columns: both are kept in 32 bits, offsets in 64
 constexpr int UNIT = 8;            // elements a thread handles at once; 4 neighbouring lanes make a block
 
 __host__ __device__ constexpr int64_t padded(int64_t cols) { return (cols + GROUP - 1) / GROUP * GROUP; }
@@ -38,7 +39,7 @@ template <> __device__ __forceinline__ float from_float<float>(float v) { return
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
-// Two fp32 values from one 32-bit word of two 16-bit ones.
+// Two fp32 values from one 32-bit word of two 16-bit ones, and back (rounded to nearest even).
 __device__ __forceinline__ float2 pair_to_float(uint32_t w, __nv_bfloat16) {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
@@ -60,55 +61,171 @@ __device__ __forceinline__ uint32_t float_to_pair(float a, float b, __half) {
   return w;
 }
 
-// Eight consecutive elements starting at column c of a row whose start is 16-byte aligned and whose length is a multiple
-// of 16 bytes; zeros from column `cols` on (with fp32 rows a unit may lie half inside).
-__device__ __forceinline__ void load_unit(const float* row, int64_t c, int64_t cols, float (&v)[UNIT]) {
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
-  if (c < cols) a = __ldg(reinterpret_cast<const float4*>(row + c));
-  if (c + 4 < cols) b = __ldg(reinterpret_cast<const float4*>(row + c) + 1);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-  v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+// ------------------------------------------------------------------- a unit of a row in memory: UNIT elements of T
+//
+// ALIGNED: the tensor starts on 16 bytes and its rows are whole 16-byte pieces.  Otherwise a row may start anywhere: a unit
+// is cut out of the aligned 16-byte words around it (the second of which is the neighbouring lane's first, so it comes from
+// the L1 cache), and put back by shifting it against the neighbouring lane's unit into aligned words; element accesses
+// remain at the ends of a run of lanes only.
+
+template <typename T> struct Raw { uint32_t w[UNIT * sizeof(T) / 4]; };
+struct Span { const uint8_t *begin, *end; };                      // of a whole tensor
+
+// the aligned 16-byte word at `at`, bytes outside the tensor read as zero without being touched
+template <typename T>
+__device__ __forceinline__ uint4 load_word(const Span& s, const uint8_t* at) {
+  if (at >= s.begin && at + 16 <= s.end) return __ldg(reinterpret_cast<const uint4*>(at));
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int i = 0; i < int(16 / sizeof(T)); ++i) {
+    const T* e = reinterpret_cast<const T*>(at) + i;
+    if (reinterpret_cast<const uint8_t*>(e) < s.begin || reinterpret_cast<const uint8_t*>(e) >= s.end) continue;
+    if (sizeof(T) == 4) w[i & 3] = *reinterpret_cast<const uint32_t*>(e);
+    else w[i / 2] |= uint32_t(*reinterpret_cast<const uint16_t*>(e)) << (16 * (i & 1));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Columns c ... c + 7 of a row, zeros from column `cols` on.
+template <bool ALIGNED, typename T>
+__device__ __forceinline__ Raw<T> load_raw(const T* row, int c, int cols, const Span& span) {
+  constexpr int NW = UNIT * sizeof(T) / 4;
+  Raw<T> r;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) r.w[i] = 0u;
+  if (c >= cols) return r;
+  const uint8_t* at = reinterpret_cast<const uint8_t*>(row + c);
+  if (ALIGNED) {
+#pragma unroll
+    for (int i = 0; i < NW; i += 4) {
+      if (i && c + 4 >= cols) break;                              // an fp32 unit may lie half inside
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(at) + i / 4);
+      r.w[i] = v.x; r.w[i + 1] = v.y; r.w[i + 2] = v.z; r.w[i + 3] = v.w;
+    }
+    return r;
+  }
+  const uint32_t shift = uint32_t(reinterpret_cast<uintptr_t>(at)) & 15u;
+  uint32_t e[NW + 4];
+#pragma unroll
+  for (int i = 0; i < NW + 4; i += 4) {
+    const uint4 v = (i < NW || shift) ? load_word<T>(span, at - shift + 4 * i) : make_uint4(0u, 0u, 0u, 0u);
+    e[i] = v.x; e[i + 1] = v.y; e[i + 2] = v.z; e[i + 3] = v.w;
+  }
+  const bool two = shift & 8u, one = shift & 4u;
+#pragma unroll
+  for (int i = 0; i < NW + 2; ++i) e[i] = two ? e[i + 2] : e[i];
+#pragma unroll
+  for (int i = 0; i < NW + 1; ++i) e[i] = one ? e[i + 1] : e[i];
+#pragma unroll
+  for (int i = 0; i < NW; ++i) r.w[i] = sizeof(T) == 4 ? e[i] : __funnelshift_r(e[i], e[i + 1], (shift & 2u) * 8u);
+  if (c + UNIT > cols) {                                          // the row ends inside: what follows is another row's
+#pragma unroll
+    for (int i = 0; i < UNIT; ++i) {
+      if (c + i < cols) continue;
+      if (sizeof(T) == 4) r.w[i & (NW - 1)] = 0u;
+      else r.w[i / 2] &= i & 1 ? 0x0000ffffu : 0u;
+    }
+  }
+  return r;
+}
+
+__device__ __forceinline__ void raw_values(const Raw<float>& r, float (&v)[UNIT]) {
+#pragma unroll
+  for (int i = 0; i < UNIT; ++i) v[i] = __uint_as_float(r.w[i]);
 }
 template <typename H>
-__device__ __forceinline__ void load_unit(const H* row, int64_t c, int64_t cols, float (&v)[UNIT]) {
-  uint4 a = make_uint4(0u, 0u, 0u, 0u);
-  if (c < cols) a = __ldg(reinterpret_cast<const uint4*>(row + c));
-  const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+__device__ __forceinline__ void raw_values(const Raw<H>& r, float (&v)[UNIT]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 p = pair_to_float(w[i], H());
+  for (int i = 0; i < UNIT / 2; ++i) {
+    const float2 p = pair_to_float(r.w[i], H());
     v[2 * i] = p.x;
     v[2 * i + 1] = p.y;
   }
 }
-__device__ __forceinline__ void store_unit(float* row, int64_t c, int64_t cols, const float (&v)[UNIT]) {
-  if (c < cols) *reinterpret_cast<float4*>(row + c) = make_float4(v[0], v[1], v[2], v[3]);
-  if (c + 4 < cols) *reinterpret_cast<float4*>(row + c + 4) = make_float4(v[4], v[5], v[6], v[7]);
+__device__ __forceinline__ Raw<float> values_raw(const float (&v)[UNIT], float) {
+  Raw<float> r;
+#pragma unroll
+  for (int i = 0; i < UNIT; ++i) r.w[i] = __float_as_uint(v[i]);
+  return r;
 }
 template <typename H>
-__device__ __forceinline__ void store_unit(H* row, int64_t c, int64_t cols, const float (&v)[UNIT]) {
-  if (c < cols)
-    *reinterpret_cast<uint4*>(row + c) = make_uint4(float_to_pair(v[0], v[1], H()), float_to_pair(v[2], v[3], H()),
-                                                    float_to_pair(v[4], v[5], H()), float_to_pair(v[6], v[7], H()));
+__device__ __forceinline__ Raw<H> values_raw(const float (&v)[UNIT], H) {
+  Raw<H> r;
+#pragma unroll
+  for (int i = 0; i < UNIT / 2; ++i) r.w[i] = float_to_pair(v[2 * i], v[2 * i + 1], H());
+  return r;
 }
 
-// Rows of any length and alignment are walked the other way round: the 32 lanes take 32 consecutive columns, so that every access
-// of a warp is one stretch of memory whatever its start, and a block is one such access.  v[i] is column c + 32 i.
-template <typename T, int N>
-__device__ __forceinline__ void load_stripes(const T* row, int64_t c, int64_t cols, float (&v)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = c + 32 * i < cols ? to_float<T>(row[c + 32 * i]) : 0.f;
-}
-template <typename T, int N>
-__device__ __forceinline__ void store_stripes(T* row, int64_t c, int64_t cols, const float (&v)[N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) if (c + 32 * i < cols) row[c + 32 * i] = from_float<T>(v[i]);
+template <typename T>
+__device__ __forceinline__ void store_element(T* row, int c, const Raw<T>& r, int i) {
+  constexpr int PER = 4 / sizeof(T);
+  const uint32_t w = r.w[i / PER] >> (32 / PER * (i % PER) & 31);
+  if (sizeof(T) == 4) reinterpret_cast<uint32_t*>(row)[c + i] = w;
+  else if (sizeof(T) == 2) reinterpret_cast<uint16_t*>(row)[c + i] = uint16_t(w);
+  else reinterpret_cast<uint8_t*>(row)[c + i] = uint8_t(w);
 }
 
-// larger magnitude of the two, NaN if either is one
-__device__ __forceinline__ float max_magnitude(float a, float b) {
+// Stores columns c ... c + 7 as far as they lie below `cols` (for a lane without a unit, c >= cols).  All lanes of the warp
+// call it; runs of WIDTH lanes hold neighbouring units of one row.  T is a type of 4, 2 or 1 bytes.
+template <bool ALIGNED, int WIDTH, typename T>
+__device__ __forceinline__ void store_raw(T* row, int c, int cols, const Raw<T>& r) {
+  constexpr int NW = UNIT * sizeof(T) / 4, FRAME = NW >= 4 ? 16 : 4 * NW;      // bytes of an aligned store
+  uint8_t* at = reinterpret_cast<uint8_t*>(row + c);
+  if (ALIGNED) {
+    if (c >= cols) return;
+    if (NW == 2) {
+      *reinterpret_cast<uint2*>(at) = make_uint2(r.w[0], r.w[1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NW; i += 4) {
+        if (i && c + 4 >= cols) break;
+        reinterpret_cast<uint4*>(at)[i / 4] = make_uint4(r.w[i], r.w[i + 1], r.w[i + 2], r.w[i + 3]);
+      }
+    }
+    return;
+  }
+  constexpr int FW = FRAME / 4;                                   // words of a frame
+  const uint32_t shift = uint32_t(reinterpret_cast<uintptr_t>(at)) & (FRAME - 1);
+  const int lane = threadIdx.x & (WIDTH - 1);
+  const bool full = c + UNIT <= cols;
+  const unsigned fulls = __ballot_sync(0xffffffffu, full) >> ((threadIdx.x & 31) & ~(WIDTH - 1));
+  const bool before = lane > 0 && (fulls >> (lane - 1) & 1u), after = lane < WIDTH - 1 && (fulls >> (lane + 1) & 1u);
+  // e: the last frame of the lane before, then this lane's words; a frame to store begins `shift` bytes ahead of the unit
+  uint32_t e[FW + NW];
+#pragma unroll
+  for (int i = 0; i < FW; ++i) e[i] = __shfl_up_sync(0xffffffffu, r.w[NW - FW + i], 1, WIDTH);
+#pragma unroll
+  for (int i = 0; i < NW; ++i) e[FW + i] = r.w[i];
+  if (FW == 4) {
+#pragma unroll
+    for (int i = FW + NW - 1; i >= 2; --i) e[i] = shift & 8u ? e[i - 2] : e[i];
+  }
+#pragma unroll
+  for (int i = FW + NW - 1; i >= 1; --i) e[i] = shift & 4u ? e[i - 1] : e[i];
+  uint32_t out[NW];
+#pragma unroll
+  for (int i = 0; i < NW; ++i) out[i] = sizeof(T) == 4 ? e[FW + i] : __funnelshift_l(e[FW + i - 1], e[FW + i], (shift & 3u) * 8u);
+  const bool first = full && (before || shift == 0);              // this lane stores its first frame as a whole
+  if (NW == 2) {
+    if (first) *reinterpret_cast<uint2*>(at - shift) = make_uint2(out[0], out[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < NW; i += 4)
+      if (i ? full : first) reinterpret_cast<uint4*>(at - shift)[i / 4] = make_uint4(out[i], out[i + 1], out[i + 2], out[i + 3]);
+  }
+  // elements ahead of this lane's first whole frame, and those that the next lane's first frame does not take along
+  const int head = int((FRAME - shift) / sizeof(T)), tail = UNIT - int(shift / sizeof(T));
+#pragma unroll
+  for (int i = 0; i < UNIT; ++i) {
+    const bool mine = full ? (!first && i < head) || (!after && i >= tail) : c + i < cols;
+    if (mine) store_element(row, c, r, i);
+  }
+}
+
+// largest magnitude of the three, NaN if one is
+__device__ __forceinline__ float max_magnitude(float a, float b, float c) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(fabsf(b)));
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
@@ -141,13 +258,6 @@ __device__ __forceinline__ uint32_t pack_e2m1x8(const float (&v)[UNIT]) {
       : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
   return r;
 }
-// byte of two e2m1 codes, a in the low half
-__device__ __forceinline__ uint32_t pack_e2m1x2(float a, float b) {
-  uint32_t r;
-  asm("{\n.reg .b8 b0, z;\nmov.b16 {b0, z}, 0;\ncvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\nmov.b32 %0, {b0, z, z, z};\n}\n" : "=r"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 __device__ __forceinline__ uint32_t pack_e4m3x2(float a, float b) {
   uint16_t r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(a), "f"(b));
@@ -156,12 +266,11 @@ __device__ __forceinline__ uint32_t pack_e4m3x2(float a, float b) {
 __device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) { return pack_e4m3x2(a, b) | (pack_e4m3x2(c, d) << 16); }
 
 // Quantises this lane's unit of a block that four neighbouring lanes hold (all lanes of the warp call it) and stores its codes
-// and, from the block's first lane, the scale.  unit: index within the padded row; `store` is false for lanes without one.
-template <int FORMAT>
-__device__ __forceinline__ void quantize_unit(float (&v)[UNIT], uint8_t* codes_row, uint8_t* scales_row, int64_t unit, bool store) {
-  float top = 0.f;
-#pragma unroll
-  for (int i = 0; i < UNIT; ++i) top = max_magnitude(top, v[i]);
+// and, from the block's first lane, the scale.  unit: index within the row, or within the whole tensor with its first
+// code and scale (rows are padded to whole groups); `store` is false for lanes without one.
+template <int FORMAT, typename I>
+__device__ __forceinline__ void quantize_unit(float (&v)[UNIT], uint8_t* codes_row, uint8_t* scales_row, I unit, bool store) {
+  const float top = max_magnitude(max_magnitude(v[0], v[1], v[2]), max_magnitude(v[3], v[4], v[5]), max_magnitude(v[6], v[7], v[7]));
   uint32_t m = __float_as_uint(top) & 0x7fffffffu;
   m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
   m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
@@ -178,33 +287,6 @@ __device__ __forceinline__ void quantize_unit(float (&v)[UNIT], uint8_t* codes_r
     reinterpret_cast<uint2*>(codes_row)[unit] = make_uint2(code == 255u ? 0u : lo, code == 255u ? 0u : hi);
   }
   if ((unit & 3) == 0) scales_row[unit >> 2] = uint8_t(code);
-}
-
-// The same for N blocks of 32 columns, one lane per column: blocks block0 ... block0 + N - 1 of the row, of which those below
-// `blocks` (the padded row's) are stored.  N is even.
-template <int FORMAT, int N>
-__device__ __forceinline__ void quantize_stripes(float (&v)[N], uint8_t* codes_row, uint8_t* scales_row, int64_t block0, int64_t blocks, int lane) {
-  uint32_t mine = 0;                                             // lane i keeps the scale of block i
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const uint32_t code = scale_code<FORMAT>(__reduce_max_sync(0xffffffffu, __float_as_uint(v[i]) & 0x7fffffffu));
-    v[i] = code == 255u ? 0.f : v[i] * inverse_scale(code);
-    if (lane == i) mine = code;
-  }
-#pragma unroll
-  for (int i = 0; i < N; i += 2) {
-    if (FORMAT == NES_MXFP4) {
-      // two blocks at once: even lanes store the first one's bytes, odd lanes the second one's
-      const uint32_t b = pack_e2m1x2(v[i], v[i + 1]), o = __shfl_xor_sync(0xffffffffu, b, 1);
-      const int64_t block = block0 + i + (lane & 1);
-      if (block < blocks) codes_row[block * 16 + (lane >> 1)] = uint8_t(lane & 1 ? (o >> 4) | (b & 0xf0u) : (b & 15u) | (o << 4));
-    } else {
-      const uint32_t two = pack_e4m3x2(v[i], v[i + 1]);
-      if (block0 + i < blocks) codes_row[(block0 + i) * 32 + lane] = uint8_t(two);
-      if (block0 + i + 1 < blocks) codes_row[(block0 + i + 1) * 32 + lane] = uint8_t(two >> 8);
-    }
-  }
-  if (lane < N && block0 + lane < blocks) scales_row[block0 + lane] = uint8_t(mine);
 }
 
 // e4m3 bytes of four e2m1 codes (the low 16 bits of c): a byte look-up in the eight magnitudes, then the signs

@@ -6,8 +6,7 @@
 // One pass: a row stays in registers between the sum of squares and the scaling, so x and the residual are read once
 // and h and y written once.  THREADS threads own a row (a warp for short rows, a block for longer ones) and hold UNITS
 // units of eight columns each; rows longer than that take the looping kernel, which reads x and the residual a second
-// time.  A unit is eight consecutive columns, or (STRIPES: rows that are not whole 16-byte pieces) one column in each of
-// eight consecutive blocks of 32, a lane per column, so that any row start is read and written in whole lines.
+// time.
 #include <type_traits>
 #include "microscale.cuh"
 
@@ -36,83 +35,91 @@ __device__ __forceinline__ float2 rsqrt_pair(double v) {
   return make_float2(r, 0.5f * r * float(1.0 - v * (double(r) * double(r))));
 }
 
-// h * (r.x + r.y) * g, the products' rounding errors carried along.  SHARP leaves the fp32 result rounded to odd (cut
-// off, lowest bit set), so that a rounding to fewer bits afterwards decides as it would on the unrounded value; a
-// value exactly on a border does not occur except for a zero.  Otherwise the result is rounded to nearest.
+// h * (r.x + r.y) * g with the products' rounding errors carried along: s + se is the row's scale times the gain to 48 bits.
+// SHARP leaves the fp32 result rounded to odd (cut off, lowest bit set), so that a rounding to fewer bits afterwards
+// decides as it would on the unrounded value; a value exactly on a border does not occur except for a zero.  Otherwise
+// the result is rounded to nearest.
 template <bool SHARP>
 __device__ __forceinline__ float scaled(float h, float2 r, float g) {
   const float s = r.x * g, se = fmaf(r.y, g, fmaf(r.x, g, -s));
-  const float p = h * s, c = fmaf(h, se, fmaf(h, s, -p));
-  if (SHARP) return __uint_as_float(__float_as_uint(__fadd_rz(p, c)) | 1u);
-  return fabsf(p) < 3.0e38f && fabsf(s) < 3.0e38f ? p + c : p;       // infinities have no error terms
+  if (SHARP) return __uint_as_float(__float_as_uint(__fmaf_rz(h, s, h * se)) | 1u);
+  return fmaf(h, s, h * se);
 }
 
-// Where a thread's unit u lies: its first column, and how the rest of the unit follows it.
-template <bool STRIPES, int THREADS>
-__device__ __forceinline__ int64_t unit_column(int t, int64_t u) {
-  if (STRIPES) return ((t >> 5) + u * (THREADS / 32)) * (32 * UNIT) + (t & 31);
-  return (t + u * THREADS) * UNIT;
-}
-template <bool STRIPES, typename T>
-__device__ __forceinline__ void get(const T* row, int64_t c, int64_t cols, float (&v)[UNIT]) {
-  if (STRIPES) load_stripes(row, c, cols, v); else load_unit(row, c, cols, v);
-}
-template <bool STRIPES, typename T>
-__device__ __forceinline__ void put(T* row, int64_t c, int64_t cols, const float (&v)[UNIT]) {
-  if (STRIPES) store_stripes(row, c, cols, v); else store_unit(row, c, cols, v);
+// A row's places in memory.
+template <typename T>
+struct Row {
+  const T *x, *residual;
+  T* h;
+  const float* noise;
+  float sign;
+  __device__ Row(const NormArgs& a, int64_t row) {
+    const int64_t at = row * a.cols;
+    x = static_cast<const T*>(a.x) + at;
+    residual = a.residual ? static_cast<const T*>(a.residual) + at : nullptr;
+    h = a.h ? static_cast<T*>(a.h) + at : nullptr;
+    noise = nullptr;
+    sign = 0.f;
+    if (a.noise) {
+      const int64_t r = row / a.members;
+      noise = a.noise + (row - r * a.members) * a.cols;
+      sign = anti_sign(r, a.rows / a.members, a.antithetic);
+    }
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ Span span_of(const NormArgs& a, const void* p) {
+  const T* b = static_cast<const T*>(p);
+  return Span{reinterpret_cast<const uint8_t*>(b), reinterpret_cast<const uint8_t*>(b + a.rows * a.cols)};
 }
 
-// A row's member noise and its sign.
-struct RowNoise { const float* p; float sign; };
-__device__ __forceinline__ RowNoise row_noise(const NormArgs& a, int64_t row) {
-  if (!a.noise) return RowNoise{nullptr, 0.f};
-  const int64_t r = row / a.members, d = row - r * a.members;
-  return RowNoise{a.noise + d * a.cols, anti_sign(r, a.rows / a.members, a.antithetic)};
-}
-
-template <typename T, bool STRIPES>
-__device__ __forceinline__ void load_h(const NormArgs& a, int64_t row, int64_t c, float (&v)[UNIT]) {
-  get<STRIPES>(static_cast<const T*>(a.x) + row * a.cols, c, a.cols, v);
-  if (a.residual) {
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void load_h(const NormArgs& a, const Row<T>& row, int c, float (&v)[UNIT]) {
+  const Raw<T> x = load_raw<ALIGNED>(row.x, c, int(a.cols), span_of<T>(a, a.x));
+  if (row.residual) {
+    const Raw<T> r = load_raw<ALIGNED>(row.residual, c, int(a.cols), span_of<T>(a, a.residual));
     float q[UNIT];
-    get<STRIPES>(static_cast<const T*>(a.residual) + row * a.cols, c, a.cols, q);
+    raw_values(x, v);
+    raw_values(r, q);
 #pragma unroll
     for (int i = 0; i < UNIT; ++i) v[i] += q[i];
+  } else {
+    raw_values(x, v);
   }
 }
 
 // y of the unit at column c; all lanes of a warp call it
-template <typename T, int OUT, bool STRIPES>
-__device__ __forceinline__ void emit(const NormArgs& a, const RowNoise& noise, int64_t row, int64_t c, const float (&h)[UNIT], float2 r) {
+template <typename T, int OUT, bool ALIGNED>
+__device__ __forceinline__ void emit(const NormArgs& a, const Row<T>& row, int64_t index, int c, const float (&h)[UNIT], float2 r) {
+  const int cols = int(a.cols);
   float g[UNIT], y[UNIT];
   if (a.gain) {
-    get<STRIPES>(a.gain, c, a.cols, g);
+    raw_values(load_raw<ALIGNED>(a.gain, c, cols, Span{reinterpret_cast<const uint8_t*>(a.gain), reinterpret_cast<const uint8_t*>(a.gain + cols)}), g);
   } else {
 #pragma unroll
     for (int i = 0; i < UNIT; ++i) g[i] = 1.f;
   }
-  if (noise.p) {
+  if (row.noise) {
     float n[UNIT];
-    get<STRIPES>(noise.p, c, a.cols, n);
+    raw_values(load_raw<ALIGNED>(row.noise, c, cols, Span{reinterpret_cast<const uint8_t*>(a.noise),
+                                                          reinterpret_cast<const uint8_t*>(a.noise + a.members * a.cols)}), n);
 #pragma unroll
-    for (int i = 0; i < UNIT; ++i) g[i] = fmaf(noise.sign, n[i], g[i]);
+    for (int i = 0; i < UNIT; ++i) g[i] = fmaf(row.sign, n[i], g[i]);
   }
 #pragma unroll
   for (int i = 0; i < UNIT; ++i) y[i] = scaled<OUT != 0>(h[i], r, g[i]);
   if (OUT == 0) {
-    put<STRIPES>(static_cast<T*>(a.y) + row * a.cols, c, a.cols, y);
+    store_raw<ALIGNED, 32>(static_cast<T*>(a.y) + index * a.cols, c, cols, values_raw(y, T()));
     return;
   }
-  // columns of the padding are zero whatever the row's scale (0 * inf is not)
-  constexpr int FORMAT = OUT == 0 ? NES_MXFP8 : OUT, APART = STRIPES ? 32 : 1;
-  if (c + (UNIT - 1) * APART >= a.cols) {
+  constexpr int FORMAT = OUT == 0 ? NES_MXFP8 : OUT;
+  if (c + UNIT > cols) {                          // columns of the padding are zero whatever the row's scale (0 * inf is not)
 #pragma unroll
-    for (int i = 0; i < UNIT; ++i) if (c + i * APART >= a.cols) y[i] = 0.f;
+    for (int i = 0; i < UNIT; ++i) if (c + i >= cols) y[i] = 0.f;
   }
-  uint8_t* codes = static_cast<uint8_t*>(a.y) + row * code_pitch(a.cols, FORMAT);
-  uint8_t* scales = a.scales + row * scale_pitch(a.cols);
-  if (STRIPES) quantize_stripes<FORMAT>(y, codes, scales, c / BLOCK, padded(a.cols) / BLOCK, int(c) & 31);
-  else quantize_unit<FORMAT>(y, codes, scales, c / UNIT, c < padded(a.cols));
+  quantize_unit<FORMAT>(y, static_cast<uint8_t*>(a.y) + index * code_pitch(cols, FORMAT), a.scales + index * scale_pitch(cols), c / UNIT,
+                        c < int(padded(cols)));
 }
 
 template <int N>
@@ -144,68 +151,68 @@ __device__ __forceinline__ float square_sum(const float (&v)[UNIT]) {
   return q;
 }
 
-template <typename T, int OUT, int THREADS, int UNITS, bool STRIPES>
+template <typename T, int OUT, int THREADS, int UNITS, bool ALIGNED>
 __global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) rms_norm_kernel(const NormArgs a) {
   constexpr int ROWS = THREADS == 32 ? 4 : 1;
-  const int64_t row = int64_t(blockIdx.x) * ROWS + (ROWS > 1 ? threadIdx.x / THREADS : 0);
-  if (row >= a.rows) return;
-  const int t = threadIdx.x % THREADS;
+  const int64_t index = int64_t(blockIdx.x) * ROWS + (ROWS > 1 ? threadIdx.x / THREADS : 0);
+  if (index >= a.rows) return;
+  const Row<T> row(a, index);
+  const int t = (threadIdx.x % THREADS) * UNIT;
   float v[UNITS][UNIT];
 #pragma unroll
-  for (int u = 0; u < UNITS; ++u) load_h<T, STRIPES>(a, row, unit_column<STRIPES, THREADS>(t, u), v[u]);
-  const RowNoise noise = row_noise(a, row);
+  for (int u = 0; u < UNITS; ++u) load_h<T, ALIGNED>(a, row, t + u * THREADS * UNIT, v[u]);
   float s = 0.f;
 #pragma unroll
   for (int u = 0; u < UNITS; ++u) s += square_sum(v[u]);
-  if (a.h) {
+  if (row.h) {
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) put<STRIPES>(static_cast<T*>(a.h) + row * a.cols, unit_column<STRIPES, THREADS>(t, u), a.cols, v[u]);
+    for (int u = 0; u < UNITS; ++u) store_raw<ALIGNED, 32>(row.h, t + u * THREADS * UNIT, int(a.cols), values_raw(v[u], T()));
   }
   const float2 r = rsqrt_pair(row_sum<THREADS>(s) * a.inv_cols + double(a.eps));
 #pragma unroll
-  for (int u = 0; u < UNITS; ++u) emit<T, OUT, STRIPES>(a, noise, row, unit_column<STRIPES, THREADS>(t, u), v[u], r);
+  for (int u = 0; u < UNITS; ++u) emit<T, OUT, ALIGNED>(a, row, index, t + u * THREADS * UNIT, v[u], r);
 }
 
 // Rows of any length: the sum of squares in one loop over the row, the outputs in a second one.
-template <typename T, int OUT, int THREADS, bool STRIPES>
+template <typename T, int OUT, int THREADS, bool ALIGNED>
 __global__ void __launch_bounds__(THREADS) rms_norm_long_kernel(const NormArgs a) {
-  const int64_t row = blockIdx.x;
-  const int64_t units = (padded(a.cols) + THREADS * UNIT - 1) / (THREADS * UNIT);
-  const RowNoise noise = row_noise(a, row);
+  const int64_t index = blockIdx.x;
+  const Row<T> row(a, index);
+  const int end = int(padded(a.cols));
   float s = 0.f;
-  for (int64_t u = 0; u < units; ++u) {
+  for (int c0 = 0; c0 < end; c0 += THREADS * UNIT) {
     float v[UNIT];
-    const int64_t c = unit_column<STRIPES, THREADS>(threadIdx.x, u);
-    load_h<T, STRIPES>(a, row, c, v);
+    const int c = c0 + threadIdx.x * UNIT;
+    load_h<T, ALIGNED>(a, row, c, v);
     s += square_sum(v);
-    if (a.h) put<STRIPES>(static_cast<T*>(a.h) + row * a.cols, c, a.cols, v);
+    if (row.h) store_raw<ALIGNED, 32>(row.h, c, int(a.cols), values_raw(v, T()));
   }
   const float2 r = rsqrt_pair(row_sum<THREADS>(s) * a.inv_cols + double(a.eps));
-  for (int64_t u = 0; u < units; ++u) {
+  for (int c0 = 0; c0 < end; c0 += THREADS * UNIT) {
     float v[UNIT];
-    const int64_t c = unit_column<STRIPES, THREADS>(threadIdx.x, u);
-    load_h<T, STRIPES>(a, row, c, v);
-    emit<T, OUT, STRIPES>(a, noise, row, c, v, r);
+    const int c = c0 + threadIdx.x * UNIT;
+    load_h<T, ALIGNED>(a, row, c, v);
+    emit<T, OUT, ALIGNED>(a, row, index, c, v, r);
   }
 }
 
-template <typename T, int OUT, bool STRIPES>
+template <typename T, int OUT, bool ALIGNED>
 static void launch_norm(const NormArgs& a, cudaStream_t st) {
   const unsigned rows = unsigned(a.rows);
   const int64_t cols = padded(a.cols);
-  if (cols <= 256) rms_norm_kernel<T, OUT, 32, 1, STRIPES><<<(rows + 3) / 4, 128, 0, st>>>(a);
-  else if (cols <= 512) rms_norm_kernel<T, OUT, 32, 2, STRIPES><<<(rows + 3) / 4, 128, 0, st>>>(a);
-  else if (cols <= 1024) rms_norm_kernel<T, OUT, 32, 4, STRIPES><<<(rows + 3) / 4, 128, 0, st>>>(a);
-  else if (cols <= 2048) rms_norm_kernel<T, OUT, 128, 2, STRIPES><<<rows, 128, 0, st>>>(a);
-  else if (cols <= 4096) rms_norm_kernel<T, OUT, 128, 4, STRIPES><<<rows, 128, 0, st>>>(a);
-  else if (cols <= 8192) rms_norm_kernel<T, OUT, 256, 4, STRIPES><<<rows, 256, 0, st>>>(a);
-  else if (cols <= 16384) rms_norm_kernel<T, OUT, 512, 4, STRIPES><<<rows, 512, 0, st>>>(a);
-  else rms_norm_long_kernel<T, OUT, 512, STRIPES><<<rows, 512, 0, st>>>(a);
+  if (cols <= 256) rms_norm_kernel<T, OUT, 32, 1, ALIGNED><<<(rows + 3) / 4, 128, 0, st>>>(a);
+  else if (cols <= 512) rms_norm_kernel<T, OUT, 32, 2, ALIGNED><<<(rows + 3) / 4, 128, 0, st>>>(a);
+  else if (cols <= 1024) rms_norm_kernel<T, OUT, 32, 4, ALIGNED><<<(rows + 3) / 4, 128, 0, st>>>(a);
+  else if (cols <= 2048) rms_norm_kernel<T, OUT, 128, 2, ALIGNED><<<rows, 128, 0, st>>>(a);
+  else if (cols <= 4096) rms_norm_kernel<T, OUT, 128, 4, ALIGNED><<<rows, 128, 0, st>>>(a);
+  else if (cols <= 8192) rms_norm_kernel<T, OUT, 256, 4, ALIGNED><<<rows, 256, 0, st>>>(a);
+  else if (cols <= 16384) rms_norm_kernel<T, OUT, 512, 4, ALIGNED><<<rows, 512, 0, st>>>(a);
+  else rms_norm_long_kernel<T, OUT, 512, ALIGNED><<<rows, 512, 0, st>>>(a);
 }
 
 template <typename T, int OUT>
 static void launch_norm_rows(const NormArgs& a, bool whole, cudaStream_t st) {
-  if (whole) launch_norm<T, OUT, false>(a, st); else launch_norm<T, OUT, true>(a, st);
+  if (whole) launch_norm<T, OUT, true>(a, st); else launch_norm<T, OUT, false>(a, st);
 }
 
 template <typename T>
@@ -232,7 +239,7 @@ extern "C" int nes_rms_norm_fwd(const void* x, const void* residual, void* resid
   NES_REQUIRE(x && y && (format == 0 || y_scales) && (!noise || members > 0) && (residual != nullptr) == (residual_out != nullptr),
               NES_ERR_BAD_ARG, "rms_norm_fwd: null pointer");
   NES_REQUIRE(!noise || rows % members == 0, NES_ERR_BAD_ARG, "rms_norm_fwd: rows must be a multiple of members");
-  NES_REQUIRE(rows <= INT32_MAX, NES_ERR_UNSUPPORTED, "rms_norm_fwd: too many rows");
+  NES_REQUIRE(rows <= LARGEST_EXTENT && cols <= LARGEST_EXTENT, NES_ERR_UNSUPPORTED, "rms_norm_fwd: too large");
   NES_REQUIRE(format == 0 || aligned16(y), NES_ERR_BAD_ARG, "rms_norm_fwd: codes must be 16-byte aligned");
   NormArgs a;
   a.x = x; a.residual = residual; a.h = residual_out; a.gain = gain; a.noise = noise; a.y = y; a.scales = y_scales;
