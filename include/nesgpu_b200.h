@@ -621,7 +621,8 @@ int nes_mx_linear_fwd(const void* x, const uint8_t* x_scales, int x_dtype, int x
  * x, residual, residual_out (rows, cols) of nes_dtype `dtype`; residual and residual_out are both NULL or both given,
  * residual_out receives h rounded to `dtype` and may not overlap x or residual.  gain (cols) and noise
  * (members, cols) are fp32, either may be NULL (gain 1, no noise).  format 0: y (rows, cols) of `dtype`;
- * otherwise y and y_scales receive the codes and scales of that microscaled format. */
+ * otherwise y and y_scales receive the codes and scales of that microscaled format.  All tensors but y_scales start
+ * on 16 bytes. */
 int nes_rms_norm_fwd(const void* x, const void* residual, void* residual_out, const float* gain, const float* noise,
                      void* y, uint8_t* y_scales, int64_t rows, int64_t cols, int64_t members, int antithetic,
                      int dtype, int format, float eps, nes_stream_t stream);

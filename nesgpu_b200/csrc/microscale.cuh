@@ -105,10 +105,12 @@ __device__ __forceinline__ Raw<T> load_raw(const T* row, int c, int cols, const 
     return r;
   }
   const uint32_t shift = uint32_t(reinterpret_cast<uintptr_t>(at)) & 15u;
+  const bool inside = at - 16 >= span.begin && at + 4 * NW + 16 <= span.end;
   uint32_t e[NW + 4];
 #pragma unroll
   for (int i = 0; i < NW + 4; i += 4) {
-    const uint4 v = (i < NW || shift) ? load_word<T>(span, at - shift + 4 * i) : make_uint4(0u, 0u, 0u, 0u);
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (i < NW || shift) v = inside ? __ldg(reinterpret_cast<const uint4*>(at - shift + 4 * i)) : load_word<T>(span, at - shift + 4 * i);
     e[i] = v.x; e[i + 1] = v.y; e[i + 2] = v.z; e[i + 3] = v.w;
   }
   const bool two = shift & 8u, one = shift & 4u;
@@ -289,11 +291,13 @@ __device__ __forceinline__ void quantize_unit(float (&v)[UNIT], uint8_t* codes_r
   if ((unit & 3) == 0) scales_row[unit >> 2] = uint8_t(code);
 }
 
-// e4m3 bytes of four e2m1 codes (the low 16 bits of c): a byte look-up in the eight magnitudes, then the signs
+// e4m3 bytes of four e2m1 codes (the low 16 bits of c): a byte look-up in the eight magnitudes, and one that fills a byte
+// with its top bit where a code's fourth bit is set (0xff, else 0x80), whose lowest bit is then the sign
 __device__ __forceinline__ uint32_t e2m1x4_to_e4m3(uint32_t c) {
   const uint32_t magnitude = __byte_perm(0x3c383000u, 0x4c484440u, c & 0x7777u);   // 0 .5 1 1.5 | 2 3 4 6
-  const uint32_t s = c & 0x8888u;
-  return magnitude | ((s << 4) & 0x80u) | ((s << 8) & 0x8000u) | ((s << 12) & 0x800000u) | ((s << 16) & 0x80000000u);
+  uint32_t filled;
+  asm("prmt.b32 %0, %1, %1, %2;" : "=r"(filled) : "r"(0x80808080u), "r"(c));
+  return magnitude | ((filled << 7) & 0x80808080u);
 }
 
 // value of one e4m3 byte (exact in fp16, hence in fp32)

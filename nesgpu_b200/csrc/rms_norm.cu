@@ -4,9 +4,14 @@
 //   y = h * rsqrt(mean(h^2) + eps) * (gain + s(r) * noise[d])     row = r * members + d
 //
 // One pass: a row stays in registers between the sum of squares and the scaling, so x and the residual are read once
-// and h and y written once.  THREADS threads own a row (a warp for short rows, a block for longer ones) and hold UNITS
-// units of eight columns each; rows longer than that take the looping kernel, which reads x and the residual a second
-// time.
+// and h and y written once.  WARPS warps own a row and hold UNITS units of eight columns per lane, a warp's units next to
+// one another; rows longer than that take the looping kernel, which reads x and the residual a second time.
+//
+// Rows that are not whole 16-byte pieces (SHIFTED): all plain tensors start on 16 bytes, so a row begins the same number of
+// elements s past such a boundary in each of them, and a unit is taken from column 8 i - s on: loads and stores stay whole
+// 16-byte words, and only a row's two ends are element accesses.  For a quantised output, whose blocks begin at
+// column 0, the values of h are then moved s places between neighbouring lanes.
+#include <algorithm>
 #include <type_traits>
 #include "microscale.cuh"
 
@@ -50,14 +55,17 @@ __device__ __forceinline__ float scaled(float h, float2 r, float g) {
 template <typename T>
 struct Row {
   const T *x, *residual;
-  T* h;
+  T *h, *y;
   const float* noise;
   float sign;
+  int shift;                                       // elements past a 16-byte boundary at which the row begins
   __device__ Row(const NormArgs& a, int64_t row) {
     const int64_t at = row * a.cols;
     x = static_cast<const T*>(a.x) + at;
     residual = a.residual ? static_cast<const T*>(a.residual) + at : nullptr;
     h = a.h ? static_cast<T*>(a.h) + at : nullptr;
+    y = static_cast<T*>(a.y) + at;
+    shift = int(at % int64_t(16 / sizeof(T)));
     noise = nullptr;
     sign = 0.f;
     if (a.noise) {
@@ -69,16 +77,67 @@ struct Row {
 };
 
 template <typename T>
-__device__ __forceinline__ Span span_of(const NormArgs& a, const void* p) {
-  const T* b = static_cast<const T*>(p);
-  return Span{reinterpret_cast<const uint8_t*>(b), reinterpret_cast<const uint8_t*>(b + a.rows * a.cols)};
+__device__ __forceinline__ Span span_of(const T* p, int64_t elements) {
+  return Span{reinterpret_cast<const uint8_t*>(p), reinterpret_cast<const uint8_t*>(p + elements)};
 }
 
-template <typename T, bool ALIGNED>
+// A unit from column c on that lies on a 16-byte boundary; c may be negative, columns outside the row read as zero.
+template <typename T>
+__device__ __forceinline__ Raw<T> load_boundary(const T* row, int c, int cols, const Span& span) {
+  constexpr int NW = UNIT * sizeof(T) / 4, PER = 4 / sizeof(T);
+  Raw<T> r;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) r.w[i] = 0u;
+  if (c >= 0 && c + UNIT <= cols) {
+#pragma unroll
+    for (int i = 0; i < NW; i += 4) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + c) + i / 4);
+      r.w[i] = v.x; r.w[i + 1] = v.y; r.w[i + 2] = v.z; r.w[i + 3] = v.w;
+    }
+  } else if (c < cols && c + UNIT > 0) {
+#pragma unroll
+    for (int i = 0; i < NW; i += 4) {
+      const uint4 v = load_word<T>(span, reinterpret_cast<const uint8_t*>(row + c) + 4 * i);
+      r.w[i] = v.x; r.w[i + 1] = v.y; r.w[i + 2] = v.z; r.w[i + 3] = v.w;
+    }
+#pragma unroll
+    for (int i = 0; i < UNIT; ++i)
+      if (c + i < 0 || c + i >= cols) r.w[i / PER] &= PER == 1 ? 0u : i & 1 ? 0x0000ffffu : 0xffff0000u;
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void store_boundary(T* row, int c, int cols, const Raw<T>& r) {
+  constexpr int NW = UNIT * sizeof(T) / 4;
+  if (c >= 0 && c + UNIT <= cols) {
+#pragma unroll
+    for (int i = 0; i < NW; i += 4) reinterpret_cast<uint4*>(row + c)[i / 4] = make_uint4(r.w[i], r.w[i + 1], r.w[i + 2], r.w[i + 3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < UNIT; ++i) if (c + i >= 0 && c + i < cols) store_element(row, c, r, i);
+  }
+}
+
+enum RowAccess { WHOLE, SHIFTED, ANY };          // ANY: the looping kernel's, units from column 8 i on wherever they lie
+
+template <RowAccess ACCESS, typename T>
+__device__ __forceinline__ Raw<T> load_at(const T* row, int c, int cols, const Span& span) {
+  if (ACCESS == SHIFTED) return load_boundary(row, c, cols, span);
+  return load_raw<ACCESS == WHOLE>(row, c, cols, span);
+}
+template <RowAccess ACCESS, typename T>
+__device__ __forceinline__ void store_at(T* row, int c, int cols, const Raw<T>& r) {
+  if (ACCESS == SHIFTED) store_boundary(row, c, cols, r);
+  else store_raw<ACCESS == WHOLE, 32>(row, c, cols, r);
+}
+
+template <typename T, RowAccess ACCESS>
 __device__ __forceinline__ void load_h(const NormArgs& a, const Row<T>& row, int c, float (&v)[UNIT]) {
-  const Raw<T> x = load_raw<ALIGNED>(row.x, c, int(a.cols), span_of<T>(a, a.x));
+  const int cols = int(a.cols);
+  const int64_t n = a.rows * a.cols;
+  const Raw<T> x = load_at<ACCESS>(row.x, c, cols, span_of(static_cast<const T*>(a.x), n));
   if (row.residual) {
-    const Raw<T> r = load_raw<ALIGNED>(row.residual, c, int(a.cols), span_of<T>(a, a.residual));
+    const Raw<T> r = load_at<ACCESS>(row.residual, c, cols, span_of(static_cast<const T*>(a.residual), n));
     float q[UNIT];
     raw_values(x, v);
     raw_values(r, q);
@@ -89,28 +148,29 @@ __device__ __forceinline__ void load_h(const NormArgs& a, const Row<T>& row, int
   }
 }
 
-// y of the unit at column c; all lanes of a warp call it
-template <typename T, int OUT, bool ALIGNED>
+// y of the unit at column c; all lanes of a warp call it.  A quantised output is stored from units of whole columns 8 i.
+template <typename T, int OUT, RowAccess ACCESS>
 __device__ __forceinline__ void emit(const NormArgs& a, const Row<T>& row, int64_t index, int c, const float (&h)[UNIT], float2 r) {
+  constexpr bool WHOLE_GAIN = ACCESS == WHOLE;
   const int cols = int(a.cols);
   float g[UNIT], y[UNIT];
   if (a.gain) {
-    raw_values(load_raw<ALIGNED>(a.gain, c, cols, Span{reinterpret_cast<const uint8_t*>(a.gain), reinterpret_cast<const uint8_t*>(a.gain + cols)}), g);
+    if (ACCESS == SHIFTED && OUT != 0) raw_values(load_boundary(a.gain, c, cols, span_of(a.gain, cols)), g);
+    else raw_values(load_raw<WHOLE_GAIN>(a.gain, c, cols, span_of(a.gain, cols)), g);
   } else {
 #pragma unroll
     for (int i = 0; i < UNIT; ++i) g[i] = 1.f;
   }
   if (row.noise) {
     float n[UNIT];
-    raw_values(load_raw<ALIGNED>(row.noise, c, cols, Span{reinterpret_cast<const uint8_t*>(a.noise),
-                                                          reinterpret_cast<const uint8_t*>(a.noise + a.members * a.cols)}), n);
+    raw_values(load_raw<WHOLE_GAIN>(row.noise, c, cols, span_of(a.noise, a.members * a.cols)), n);
 #pragma unroll
     for (int i = 0; i < UNIT; ++i) g[i] = fmaf(row.sign, n[i], g[i]);
   }
 #pragma unroll
   for (int i = 0; i < UNIT; ++i) y[i] = scaled<OUT != 0>(h[i], r, g[i]);
   if (OUT == 0) {
-    store_raw<ALIGNED, 32>(static_cast<T*>(a.y) + index * a.cols, c, cols, values_raw(y, T()));
+    store_at<ACCESS>(row.y, c, cols, values_raw(y, T()));
     return;
   }
   constexpr int FORMAT = OUT == 0 ? NES_MXFP8 : OUT;
@@ -122,24 +182,38 @@ __device__ __forceinline__ void emit(const NormArgs& a, const Row<T>& row, int64
                         c < int(padded(cols)));
 }
 
-template <int N>
-__device__ __forceinline__ double tree_sum(const double* p) {
-  if constexpr (N == 1) return p[0];
-  else return tree_sum<N / 2>(p) + tree_sum<N / 2>(p + N / 2);
+// h of columns 8 i ... from units that begin `shift` elements earlier: the end of the unit `from` and the start of the next
+// lane's, for lane 31 of the unit `next` of lane 0.
+__device__ __forceinline__ void unshift(const float (&from)[UNIT], const float (&next)[UNIT], int shift, float (&to)[UNIT]) {
+  const int lane = threadIdx.x & 31;
+  float e[2 * UNIT];
+#pragma unroll
+  for (int i = 0; i < UNIT; ++i) {
+    e[i] = from[i];
+    e[UNIT + i] = __shfl_sync(0xffffffffu, lane == 0 ? next[i] : from[i], (lane + 1) & 31);
+  }
+#pragma unroll
+  for (int b = 4; b; b >>= 1)
+#pragma unroll
+    for (int i = 0; i < 2 * UNIT - b; ++i) e[i] = shift & b ? e[i + b] : e[i];
+#pragma unroll
+  for (int i = 0; i < UNIT; ++i) to[i] = e[i];
 }
 
-// Sum over the THREADS threads that share a row (all of a block unless THREADS == 32), the same in every thread.  The
-// threads' partial sums are joined in 64 bits: the last few additions carry the whole row's rounding.
-template <int THREADS>
+// Sum over a row's threads (all of a block, or one warp), the same in every thread.  The threads' partial sums are joined in
+// 64 bits: the last few additions carry the whole row's rounding.
+template <bool BLOCK_ROW>
 __device__ __forceinline__ double row_sum(float mine) {
   double s = mine;
 #pragma unroll
   for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (THREADS > 32) {
-    __shared__ double part[THREADS / 32];
+  if (BLOCK_ROW) {
+    __shared__ double part[32];
+    const int warps = blockDim.x >> 5;
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
     __syncthreads();
-    s = tree_sum<THREADS / 32>(part);
+    s = part[0];
+    for (int i = 1; i < warps; ++i) s += part[i];
   }
   return s;
 }
@@ -151,63 +225,87 @@ __device__ __forceinline__ float square_sum(const float (&v)[UNIT]) {
   return q;
 }
 
-template <typename T, int OUT, int THREADS, int UNITS, bool ALIGNED>
-__global__ void __launch_bounds__(THREADS == 32 ? 128 : THREADS) rms_norm_kernel(const NormArgs a) {
-  constexpr int ROWS = THREADS == 32 ? 4 : 1;
-  const int64_t index = int64_t(blockIdx.x) * ROWS + (ROWS > 1 ? threadIdx.x / THREADS : 0);
+constexpr int MOST_WARPS = 17;                   // of a row: 16384 columns, and one unit more where rows are shifted
+constexpr int WARP_ROWS = 4;                     // rows of a block whose warps take one each
+
+template <typename T, int OUT, int UNITS, RowAccess ACCESS, bool BLOCK_ROW>
+__global__ void __launch_bounds__(BLOCK_ROW ? MOST_WARPS * 32 : WARP_ROWS * 32) rms_norm_kernel(const NormArgs a) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t index = BLOCK_ROW ? int64_t(blockIdx.x) : int64_t(blockIdx.x) * WARP_ROWS + warp;
   if (index >= a.rows) return;
   const Row<T> row(a, index);
-  const int t = (threadIdx.x % THREADS) * UNIT;
-  float v[UNITS][UNIT];
+  const int first = ((BLOCK_ROW ? warp * UNITS * 32 : 0) + lane) * UNIT, shift = ACCESS == SHIFTED ? row.shift : 0;
+  const int end = OUT != 0 ? int(padded(a.cols)) : int(a.cols) + shift;
+  float v[UNITS + 1][UNIT];
 #pragma unroll
-  for (int u = 0; u < UNITS; ++u) load_h<T, ALIGNED>(a, row, t + u * THREADS * UNIT, v[u]);
+  for (int u = 0; u < UNITS; ++u) load_h<T, ACCESS>(a, row, first - shift + u * 32 * UNIT, v[u]);
+  constexpr bool MOVE = ACCESS == SHIFTED && OUT != 0;
+  if (MOVE && lane == 0) load_h<T, ACCESS>(a, row, first - shift + UNITS * 32 * UNIT, v[UNITS]);     // the next warp's first unit
   float s = 0.f;
 #pragma unroll
   for (int u = 0; u < UNITS; ++u) s += square_sum(v[u]);
   if (row.h) {
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) store_raw<ALIGNED, 32>(row.h, t + u * THREADS * UNIT, int(a.cols), values_raw(v[u], T()));
+    for (int u = 0; u < UNITS; ++u) if (first - lane * UNIT + u * 32 * UNIT < int(a.cols) + shift) store_at<ACCESS>(row.h, first - shift + u * 32 * UNIT, int(a.cols), values_raw(v[u], T()));
   }
-  const float2 r = rsqrt_pair(row_sum<THREADS>(s) * a.inv_cols + double(a.eps));
+  const float2 r = rsqrt_pair(row_sum<BLOCK_ROW>(s) * a.inv_cols + double(a.eps));
 #pragma unroll
-  for (int u = 0; u < UNITS; ++u) emit<T, OUT, ALIGNED>(a, row, index, t + u * THREADS * UNIT, v[u], r);
+  for (int u = 0; u < UNITS; ++u) {
+    if (first - lane * UNIT + u * 32 * UNIT >= end) break;         // nothing of the row in this warp's unit u
+    if (MOVE) {
+      float h[UNIT];
+      unshift(v[u], v[u + 1], shift, h);
+      emit<T, OUT, ACCESS>(a, row, index, first + u * 32 * UNIT, h, r);
+    } else {
+      emit<T, OUT, ACCESS>(a, row, index, first - shift + u * 32 * UNIT, v[u], r);
+    }
+  }
 }
 
 // Rows of any length: the sum of squares in one loop over the row, the outputs in a second one.
-template <typename T, int OUT, int THREADS, bool ALIGNED>
-__global__ void __launch_bounds__(THREADS) rms_norm_long_kernel(const NormArgs a) {
+template <typename T, int OUT, RowAccess ACCESS>
+__global__ void __launch_bounds__(512) rms_norm_long_kernel(const NormArgs a) {
   const int64_t index = blockIdx.x;
   const Row<T> row(a, index);
-  const int end = int(padded(a.cols));
+  const int end = int(padded(a.cols)), step = blockDim.x * UNIT;
   float s = 0.f;
-  for (int c0 = 0; c0 < end; c0 += THREADS * UNIT) {
+  for (int c0 = 0; c0 < end; c0 += step) {
     float v[UNIT];
     const int c = c0 + threadIdx.x * UNIT;
-    load_h<T, ALIGNED>(a, row, c, v);
+    load_h<T, ACCESS>(a, row, c, v);
     s += square_sum(v);
-    if (row.h) store_raw<ALIGNED, 32>(row.h, c, int(a.cols), values_raw(v, T()));
+    if (row.h) store_at<ACCESS>(row.h, c, int(a.cols), values_raw(v, T()));
   }
-  const float2 r = rsqrt_pair(row_sum<THREADS>(s) * a.inv_cols + double(a.eps));
-  for (int c0 = 0; c0 < end; c0 += THREADS * UNIT) {
+  const float2 r = rsqrt_pair(row_sum<true>(s) * a.inv_cols + double(a.eps));
+  for (int c0 = 0; c0 < end; c0 += step) {
     float v[UNIT];
     const int c = c0 + threadIdx.x * UNIT;
-    load_h<T, ALIGNED>(a, row, c, v);
-    emit<T, OUT, ALIGNED>(a, row, index, c, v, r);
+    load_h<T, ACCESS>(a, row, c, v);
+    emit<T, OUT, ACCESS>(a, row, index, c, v, r);
   }
 }
 
+// Four units per lane keep the most loads in flight where there are rows enough for all SMs; a few rows are spread over more
+// warps instead (one row of 4096: 4.3 us with 4 warps, see the launch below for the figure with 16).
 template <typename T, int OUT, bool ALIGNED>
 static void launch_norm(const NormArgs& a, cudaStream_t st) {
+  constexpr RowAccess ACCESS = ALIGNED ? WHOLE : SHIFTED;
   const unsigned rows = unsigned(a.rows);
-  const int64_t cols = padded(a.cols);
-  if (cols <= 256) rms_norm_kernel<T, OUT, 32, 1, ALIGNED><<<(rows + 3) / 4, 128, 0, st>>>(a);
-  else if (cols <= 512) rms_norm_kernel<T, OUT, 32, 2, ALIGNED><<<(rows + 3) / 4, 128, 0, st>>>(a);
-  else if (cols <= 1024) rms_norm_kernel<T, OUT, 32, 4, ALIGNED><<<(rows + 3) / 4, 128, 0, st>>>(a);
-  else if (cols <= 2048) rms_norm_kernel<T, OUT, 128, 2, ALIGNED><<<rows, 128, 0, st>>>(a);
-  else if (cols <= 4096) rms_norm_kernel<T, OUT, 128, 4, ALIGNED><<<rows, 128, 0, st>>>(a);
-  else if (cols <= 8192) rms_norm_kernel<T, OUT, 256, 4, ALIGNED><<<rows, 256, 0, st>>>(a);
-  else if (cols <= 16384) rms_norm_kernel<T, OUT, 512, 4, ALIGNED><<<rows, 512, 0, st>>>(a);
-  else rms_norm_long_kernel<T, OUT, 512, ALIGNED><<<rows, 512, 0, st>>>(a);
+  const int64_t units = ALIGNED ? padded(a.cols) / UNIT : std::max<int64_t>(padded(a.cols) / UNIT, (a.cols + 2 * (UNIT - 1)) / UNIT);
+  const bool few = a.rows < 2 * sm_count();
+  if (units > MOST_WARPS * 32 * 4) {
+    rms_norm_long_kernel<T, OUT, ALIGNED ? WHOLE : ANY><<<rows, 512, 0, st>>>(a);
+  } else if (units <= 32) {
+    rms_norm_kernel<T, OUT, 1, ACCESS, false><<<(rows + WARP_ROWS - 1) / WARP_ROWS, WARP_ROWS * 32, 0, st>>>(a);
+  } else if (few && units <= MOST_WARPS * 32) {
+    rms_norm_kernel<T, OUT, 1, ACCESS, true><<<rows, unsigned(ceil_div<int64_t>(units, 32)) * 32, 0, st>>>(a);
+  } else if (units <= 64) {
+    rms_norm_kernel<T, OUT, 2, ACCESS, false><<<(rows + WARP_ROWS - 1) / WARP_ROWS, WARP_ROWS * 32, 0, st>>>(a);
+  } else if (units <= 128) {
+    rms_norm_kernel<T, OUT, 4, ACCESS, false><<<(rows + WARP_ROWS - 1) / WARP_ROWS, WARP_ROWS * 32, 0, st>>>(a);
+  } else {
+    rms_norm_kernel<T, OUT, 4, ACCESS, true><<<rows, unsigned(ceil_div<int64_t>(units, 128)) * 32, 0, st>>>(a);
+  }
 }
 
 template <typename T, int OUT>
@@ -217,8 +315,7 @@ static void launch_norm_rows(const NormArgs& a, bool whole, cudaStream_t st) {
 
 template <typename T>
 static void launch_norm_out(const NormArgs& a, int format, cudaStream_t st) {
-  const bool whole = (a.cols * sizeof(T)) % 16 == 0 && aligned16(a.x) && aligned16(a.residual) && aligned16(a.h) && aligned16(a.gain) &&
-                     aligned16(a.noise) && aligned16(a.y);
+  const bool whole = (a.cols * sizeof(T)) % 16 == 0;
   if (format == 0) launch_norm_rows<T, 0>(a, whole, st);
   else if (format == NES_MXFP4) launch_norm_rows<T, NES_MXFP4>(a, whole, st);
   else launch_norm_rows<T, NES_MXFP8>(a, whole, st);
@@ -240,7 +337,8 @@ extern "C" int nes_rms_norm_fwd(const void* x, const void* residual, void* resid
               NES_ERR_BAD_ARG, "rms_norm_fwd: null pointer");
   NES_REQUIRE(!noise || rows % members == 0, NES_ERR_BAD_ARG, "rms_norm_fwd: rows must be a multiple of members");
   NES_REQUIRE(rows <= LARGEST_EXTENT && cols <= LARGEST_EXTENT, NES_ERR_UNSUPPORTED, "rms_norm_fwd: too large");
-  NES_REQUIRE(format == 0 || aligned16(y), NES_ERR_BAD_ARG, "rms_norm_fwd: codes must be 16-byte aligned");
+  NES_REQUIRE(aligned16(x) && aligned16(residual) && aligned16(residual_out) && aligned16(gain) && aligned16(noise) && aligned16(y),
+              NES_ERR_BAD_ARG, "rms_norm_fwd: tensors must be 16-byte aligned");
   NormArgs a;
   a.x = x; a.residual = residual; a.h = residual_out; a.gain = gain; a.noise = noise; a.y = y; a.scales = y_scales;
   a.rows = rows; a.cols = cols; a.members = members > 0 ? members : 1; a.antithetic = antithetic;

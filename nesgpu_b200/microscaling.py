@@ -133,6 +133,11 @@ def _empty(x, rows, cols, format):
         rows, cols, format)
 
 
+def _aligned(t):
+    """``t`` at an address that is a multiple of 16 bytes (a copy if it starts inside an allocation)."""
+    return t if t is None or t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _rows(t, name):
     """A contiguous CUDA tensor of a supported type with at least one column, and its number of rows."""
     t = C.require_cuda(t, name)
@@ -237,6 +242,7 @@ def rms_norm(input, weight=None, eps=1e-6, residual=None, noise=None, antithetic
     else:
         y = torch.empty_like(x)
         data, scales = y.data_ptr(), None
+    x, residual, weight, noise = _aligned(x), _aligned(residual), _aligned(weight), _aligned(noise)
     _launch("nes_rms_norm_fwd", device, x.data_ptr(), C.ptr(residual), C.ptr(h), C.ptr(weight), C.ptr(noise), data,
             scales, rows, cols, members, 1 if antithetic else 0, _DTYPES[x.dtype], kind, eps)
     return y if residual is None else (y, h)

@@ -150,7 +150,9 @@ def _check_norm(y, want, form, dtype):
 @pytest.mark.parametrize("rows,cols,members,with_residual,antithetic", [
     (1, 1, 0, False, False), (1, 33, 0, True, False), (6, 200, 3, True, True), (5, 256, 0, False, False), (9, 257, 9, False, True),
     (4, 512, 0, True, False), (12, 1000, 4, True, True), (3, 1024, 0, True, False), (2, 2048, 1, False, False), (1, 4096, 0, True, False),
-    (3, 4097, 0, True, False), (2, 8192, 2, True, False), (2, 16384, 0, True, False), (3, 16389, 0, True, False), (2, 40000, 2, True, True)])
+    (3, 4097, 0, True, False), (2, 8192, 2, True, False), (2, 16384, 0, True, False), (3, 16389, 0, True, False), (2, 40000, 2, True, True),
+    (9, 16383, 0, True, False), (3, 17400, 0, True, False), (4, 17411, 2, False, False), (700, 515, 7, True, True), (601, 1023, 0, True, False),
+    (600, 1009, 0, True, False), (500, 250, 5, True, False), (420, 4099, 3, True, True), (300, 4350, 0, True, False), (640, 127, 0, True, False)])
 def test_rms_norm(rows, cols, members, with_residual, antithetic, dtype, form):
     ms = _ms()
     x = _inputs(rows, cols, dtype, rows + cols)
@@ -181,6 +183,10 @@ def test_rms_norm_defaults_and_shapes():
     want, _ = O.rms_norm(_f64(strided), None, float(np.float32(1e-6)))
     _check_norm(ms.rms_norm(strided), want, None, "fp32")
     assert ms.rms_norm(torch.empty(0, 8, device="cuda")).shape == (0, 8)
+    flat = _inputs(1, 8 * 128 + 1, "bf16", 7).view(-1)
+    off = flat[1:].view(8, 128)                       # rows start 2 bytes past a 16-byte boundary
+    want, _ = O.rms_norm(_f64(off), _f64(flat[1:129].float()), float(np.float32(1e-6)))
+    _check_norm(ms.rms_norm(off, flat.float()[1:129]), want, None, "bf16")
 
 
 @pytest.mark.parametrize("form", [None, "mxfp8", "mxfp4"])
