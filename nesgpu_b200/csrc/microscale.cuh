@@ -267,27 +267,34 @@ __device__ __forceinline__ uint32_t pack_e4m3x2(float a, float b) {
 }
 __device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) { return pack_e4m3x2(a, b) | (pack_e4m3x2(c, d) << 16); }
 
-// Quantises this lane's unit of a block that four neighbouring lanes hold (all lanes of the warp call it) and stores its codes
-// and, from the block's first lane, the scale.  unit: index within the row, or within the whole tensor with its first
-// code and scale (rows are padded to whole groups); `store` is false for lanes without one.
-template <int FORMAT, typename I>
-__device__ __forceinline__ void quantize_unit(float (&v)[UNIT], uint8_t* codes_row, uint8_t* scales_row, I unit, bool store) {
+// Codes (4 or, in x and y, 8 bytes) and scale of this lane's unit of a block that four neighbouring lanes hold; all lanes of the
+// warp call it.
+template <int FORMAT>
+__device__ __forceinline__ uint2 encode_unit(float (&v)[UNIT], uint32_t& code) {
   const float top = max_magnitude(max_magnitude(v[0], v[1], v[2]), max_magnitude(v[3], v[4], v[5]), max_magnitude(v[6], v[7], v[7]));
   uint32_t m = __float_as_uint(top) & 0x7fffffffu;
   m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
   m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-  const uint32_t code = scale_code<FORMAT>(m);
+  code = scale_code<FORMAT>(m);
   const float inv = inverse_scale(code);
 #pragma unroll
   for (int i = 0; i < UNIT; ++i) v[i] *= inv;
+  uint2 q;
+  if (FORMAT == NES_MXFP4) q = make_uint2(pack_e2m1x8(v), 0u);
+  else q = make_uint2(pack_e4m3x4(v[0], v[1], v[2], v[3]), pack_e4m3x4(v[4], v[5], v[6], v[7]));
+  if (code == 255u) q = make_uint2(0u, 0u);
+  return q;
+}
+
+// The same, stored: codes and, from the block's first lane, the scale.  unit: index within the row, or within the whole tensor
+// with its first code and scale (rows are padded to whole groups); `store` is false for lanes without one.
+template <int FORMAT, typename I>
+__device__ __forceinline__ void quantize_unit(float (&v)[UNIT], uint8_t* codes_row, uint8_t* scales_row, I unit, bool store) {
+  uint32_t code;
+  const uint2 q = encode_unit<FORMAT>(v, code);
   if (!store) return;
-  if (FORMAT == NES_MXFP4) {
-    const uint32_t q = pack_e2m1x8(v);
-    reinterpret_cast<uint32_t*>(codes_row)[unit] = code == 255u ? 0u : q;
-  } else {
-    const uint32_t lo = pack_e4m3x4(v[0], v[1], v[2], v[3]), hi = pack_e4m3x4(v[4], v[5], v[6], v[7]);
-    reinterpret_cast<uint2*>(codes_row)[unit] = make_uint2(code == 255u ? 0u : lo, code == 255u ? 0u : hi);
-  }
+  if (FORMAT == NES_MXFP4) reinterpret_cast<uint32_t*>(codes_row)[unit] = q.x;
+  else reinterpret_cast<uint2*>(codes_row)[unit] = q;
   if ((unit & 3) == 0) scales_row[unit >> 2] = uint8_t(code);
 }
 

@@ -12,6 +12,8 @@
 //     column per 32 rows and 128 elements, repeated in each quarter of the lanes.  Four warps load them for STEP = 512
 //     elements of K at a time, 16 bytes per row and thread, transpose them on the way into shared memory, and tcgen05.cp
 //     brings them over in the order of the products.
+//   * Plain activations are quantised into scratch first; a few tokens are quantised by the product itself, every CTA
+//     its own part of K straight into the operand's place in shared memory.
 //   * Few output tiles: a cluster of up to eight CTAs splits K and adds its partial tiles in a fixed order through
 //     distributed shared memory.
 #include <type_traits>
@@ -34,24 +36,33 @@ struct Product {
   const uint8_t *x_scales, *w_scales;
   const float* bias;
   void* y;
-  int M, N, groups;                          // tokens, features, 128-element groups of K
+  int M, N, K, groups;                       // tokens, features, columns and their 128-element groups
   int y_dtype, vec_scales;
+  const void* x;                             // plain activations of a product that quantises them itself
+  int whole_rows;                            // their rows are whole, aligned 16-byte pieces
 };
 struct ProductMaps { CUtensorMap w, x; };
 
-template <int TOKENS>
+constexpr int RAW_STEPS = 8;                 // steps of K whose quantised activations a CTA keeps
+
+// RAW: the activations of all the CTA's stages lie behind the stages, which hold weights only; so do their scales
+template <int TOKENS, bool RAW, int STAGES_PER_STEP>
 struct Layout {
   static constexpr int W_BYTES = FEATURES * ROW_BYTES;
   static constexpr int X_BYTES = TOKENS * ROW_BYTES;
-  static constexpr int STAGE = W_BYTES + X_BYTES;
+  static constexpr int STAGE = W_BYTES + (RAW ? 0 : X_BYTES);
   static constexpr int STAGES = TOKENS >= 128 ? 6 : 8;
   static constexpr int X_COLS = 4;                                         // scale columns of x per 128 elements
   static constexpr int SCALE_COLS = CHUNKS * (4 + X_COLS);                 // one buffer
   static constexpr int SCALE_BASE = TOKENS < 32 ? 32 : TOKENS;
   static constexpr int USED_COLS = SCALE_BASE + 2 * SCALE_COLS;
   static constexpr int TMEM_COLS = USED_COLS <= 128 ? 128 : USED_COLS <= 256 ? 256 : 512;
-  static constexpr int SCALES = 2 * CHUNKS * SCALE_TILE;                   // a buffer in shared memory: w, then x
-  static constexpr size_t SMEM = 1024 + size_t(STAGES) * STAGE + 2 * SCALES + (2 * STAGES + 5) * sizeof(uint64_t) + 16;
+  static constexpr int STEP_SCALES = CHUNKS * SCALE_TILE;                  // of one operand
+  static constexpr int SCALES = (RAW ? 1 : 2) * STEP_SCALES;               // a buffer in shared memory: w, then x
+  static constexpr int RAW_X = RAW ? RAW_STEPS * STAGES_PER_STEP * X_BYTES : 0;
+  static constexpr int RAW_SCALES = RAW ? RAW_STEPS * STEP_SCALES : 0;
+  static constexpr size_t SMEM = 1024 + size_t(STAGES) * STAGE + RAW_X + RAW_SCALES + 2 * SCALES + (2 * STAGES + 6) * sizeof(uint64_t) + 16;
+  static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
 // Instruction descriptor with block scales: element formats at bits 7 and 10 (kind::mxf4: 1 = e2m1; kind::mxf8f6f4: 0 = e4m3,
@@ -246,25 +257,68 @@ __device__ __forceinline__ void join_tiles(const Product& p, uint32_t part, int 
   }
 }
 
-template <int XF, int WF, int TOKENS>
+// Quantises columns c0 ... c0 + width - 1 of all (at most 16) tokens with 128 threads: codes into the 128-byte-swizzled rows of
+// consecutive stages at `tiles`, scales into the tiles of consecutive steps at `scales`.  What no token fills is zero.
+template <typename T, int XF>
+__device__ __forceinline__ void quantize_tokens(const Product& p, int c0, int width, unsigned char* tiles, unsigned char* scales, int t) {
+  constexpr int TILE = 16 * ROW_BYTES, UNIT_BYTES = XF == NES_MXFP4 ? 4 : 8, AT_ONCE = 4;
+  const int row_units = width / UNIT, units = p.M * row_units;
+  const T* x = static_cast<const T*>(p.x);
+  const Span span = {reinterpret_cast<const uint8_t*>(x), reinterpret_cast<const uint8_t*>(x + int64_t(p.M) * p.K)};
+  for (int i = t; i < width / STEP * (CHUNKS * SCALE_TILE / 16); i += 128) reinterpret_cast<uint4*>(scales)[i] = make_uint4(0u, 0u, 0u, 0u);
+  for (int i = t; i < row_units * UNIT_BYTES; i += 128)                                       // = 16 rows in 16-byte pieces
+    if (i / (ROW_BYTES / 16) % 16 >= p.M) reinterpret_cast<uint4*>(tiles)[i] = make_uint4(0u, 0u, 0u, 0u);
+  asm volatile("bar.sync 1, 128;" ::: "memory");                                              // before scales are written
+  for (int u0 = t; u0 - (t & 31) < units; u0 += 128 * AT_ONCE) {
+    Raw<T> raw[AT_ONCE];
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const int u = u0 + 128 * i, row = u / row_units, c = c0 + (u - row * row_units) * UNIT;
+      if (p.whole_rows) raw[i] = load_raw<true>(x + int64_t(row) * p.K, u < units ? c : p.K, p.K, span);
+      else raw[i] = load_raw<false>(x + int64_t(row) * p.K, u < units ? c : p.K, p.K, span);
+    }
+#pragma unroll
+    for (int i = 0; i < AT_ONCE; ++i) {
+      const int u = u0 + 128 * i;
+      if (u - (t & 31) >= units) break;                                                       // whole warps: 64 units divide a row
+      const int row = u / row_units, at = u - row * row_units;
+      float v[UNIT];
+      raw_values(raw[i], v);
+      uint32_t code;
+      const uint2 q = encode_unit<XF>(v, code);
+      const int byte = at * UNIT_BYTES, stage = byte / ROW_BYTES, in_row = byte % ROW_BYTES;
+      unsigned char* to = tiles + stage * TILE + row * ROW_BYTES + (((in_row >> 4) ^ (row & 7)) << 4) + (in_row & 15);
+      if (XF == NES_MXFP4) *reinterpret_cast<uint32_t*>(to) = q.x;
+      else *reinterpret_cast<uint2*>(to) = q;
+      if ((at & 3) == 0) scales[(at / (GROUP / UNIT)) * SCALE_TILE + row * 16 + ((at >> 2) & 3)] = uint8_t(code);
+    }
+  }
+}
+
+// X: void for activations that are quantised already, else the type of plain ones
+template <int XF, int WF, int TOKENS, typename X>
 __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_constant__ ProductMaps maps, const Product p, int splits) {
-  using L = Layout<TOKENS>;
+  constexpr bool RAW = !std::is_same<X, void>::value;
+  constexpr int STAGE_GROUPS = XF == NES_MXFP4 ? 2 : 1;                  // 128-element groups per stage
+  constexpr int STAGES_PER_STEP = CHUNKS / STAGE_GROUPS;
+  using L = Layout<TOKENS, RAW, STAGES_PER_STEP>;
   extern __shared__ unsigned char dyn_raw[];
   const unsigned int timeouts_at_start = timeouts_so_far();
   const uint32_t raw = smem_u32(dyn_raw);
   unsigned char* tiles = dyn_raw + (((raw + 1023u) & ~1023u) - raw);
-  unsigned char* scale_tiles = tiles + size_t(L::STAGES) * L::STAGE;
+  unsigned char* raw_tiles = tiles + size_t(L::STAGES) * L::STAGE;
+  unsigned char* raw_scales = raw_tiles + L::RAW_X;
+  unsigned char* scale_tiles = raw_scales + L::RAW_SCALES;
   uint64_t* full = reinterpret_cast<uint64_t*>(scale_tiles + 2 * L::SCALES);
   uint64_t* empty = full + L::STAGES;
   uint64_t* sf_full = empty + L::STAGES;
   uint64_t* sf_empty = sf_full + 2;
   uint64_t* accum = sf_empty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(accum + 1);
+  uint64_t* raw_full = accum + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(raw_full + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = blockIdx.x % splits, n0 = (blockIdx.x / splits) * FEATURES, m0 = blockIdx.y * TOKENS;
-  constexpr int STAGE_GROUPS = XF == NES_MXFP4 ? 2 : 1;                  // 128-element groups per stage
-  constexpr int STAGES_PER_STEP = CHUNKS / STAGE_GROUPS;
   const int all_steps = (p.groups + CHUNKS - 1) / CHUNKS;
   const int step0 = int(int64_t(all_steps) * rank / splits), step1 = int(int64_t(all_steps) * (rank + 1) / splits);
   const int kt0 = step0 * STAGES_PER_STEP;
@@ -274,6 +328,7 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
     for (int s = 0; s < L::STAGES; ++s) { mbar_init(&full[s], 1); mbar_init(&empty[s], 1); }
     for (int s = 0; s < 2; ++s) { mbar_init(&sf_full[s], 4); mbar_init(&sf_empty[s], 1); }
     mbar_init(accum, 1);
+    mbar_init(raw_full, 4);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) tmem_alloc(tmem_slot, L::TMEM_COLS);
@@ -286,7 +341,7 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
   if (warp == 0) {
     if (lane == 0) {
       // a spreading copy counts the bytes it reads, half of those it fills
-      constexpr uint32_t TX = L::X_BYTES + (XF == NES_MXFP8 && WF == NES_MXFP4 ? L::W_BYTES / 2 : L::W_BYTES);
+      constexpr uint32_t TX = (RAW ? 0 : L::X_BYTES) + (XF == NES_MXFP8 && WF == NES_MXFP4 ? L::W_BYTES / 2 : L::W_BYTES);
       int s = 0;
       uint32_t ph = 0;
       for (int kt = kt0; kt < kt1; ++kt) {
@@ -296,7 +351,7 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
         // first coordinate: bytes of codes, or elements of a copy that spreads 4-bit codes
         const int c = kt * ROW_BYTES;
         tma_load_2d(st, &maps.w, &full[s], c, n0);
-        tma_load_2d(st + L::W_BYTES, &maps.x, &full[s], c, m0);
+        if (!RAW) tma_load_2d(st + L::W_BYTES, &maps.x, &full[s], c, m0);
         if (++s == L::STAGES) { s = 0; ph ^= 1u; }
       }
     }
@@ -304,10 +359,11 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
   } else if (warp == 1) {
     constexpr uint32_t idesc = idesc_scaled<XF, WF>(FEATURES, TOKENS);
     const uint64_t desc0 = smem_desc_sw128(smem_u32(tiles));
-    const uint64_t sdesc0 = scale_desc(smem_u32(scale_tiles));
+    const uint64_t sdesc0 = scale_desc(smem_u32(scale_tiles)), xdesc0 = smem_desc_sw128(smem_u32(raw_tiles));
     int s = 0;
     uint32_t ph = 0, sf_ph = 0, accumulate = 0;
     int kt = kt0;
+    if (RAW) ok = warp_mbar_wait(raw_full, 0, 2);
     for (int step = step0; step < step1 && ok; ++step) {
       const int b = (step - step0) & 1;
       ok = warp_mbar_wait(&sf_full[b], sf_ph, 2);
@@ -317,7 +373,7 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
       const uint32_t sfa = tmem + L::SCALE_BASE + b * L::SCALE_COLS, sfb = sfa + CHUNKS * 4;
       const uint64_t sdesc = sdesc0 + uint64_t((b * L::SCALES) >> 4);
       warp_copy_scales<1, 4>(sfa, sdesc);
-      warp_copy_scales<1, L::X_COLS>(sfb, sdesc + uint64_t((CHUNKS * SCALE_TILE) >> 4));
+      warp_copy_scales<1, L::X_COLS>(sfb, RAW ? scale_desc(smem_u32(raw_scales) + (step - step0) * L::STEP_SCALES) : sdesc + uint64_t(L::STEP_SCALES >> 4));
       warp_mma_commit(&sf_empty[b]);
 #pragma unroll
       for (int i = 0; i < STAGES_PER_STEP; ++i, ++kt) {
@@ -325,7 +381,8 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
         ok = warp_mbar_wait(&full[s], ph, 2);
         if (!ok) break;
         tc_fence_after();
-        const uint64_t a = desc0 + uint64_t(uint32_t(s) * uint32_t(L::STAGE >> 4)), x = a + (L::W_BYTES >> 4);
+        const uint64_t a = desc0 + uint64_t(uint32_t(s) * uint32_t(L::STAGE >> 4));
+        const uint64_t x = RAW ? xdesc0 + uint64_t(uint32_t(kt - kt0) * uint32_t(L::X_BYTES >> 4)) : a + (L::W_BYTES >> 4);
         const int j = i * STAGE_GROUPS;
         if (STAGE_GROUPS == 1 || kt * 2 + 1 < p.groups)
           warp_mma_stage<XF, 1>(tmem, a, x, idesc, sfa + 4 * j, sfb + L::X_COLS * j, sfa + 4 * (j + STAGE_GROUPS - 1),
@@ -346,20 +403,25 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
     auto load = [&](int step, uint4& wo, uint4& xo) {
       if (step >= step1) return;
       wo = load_scale_words(p.w_scales, n0 + row, p.N, step * CHUNKS, p.groups, p.vec_scales);
-      xo = load_scale_words(p.x_scales, row < TOKENS ? m0 + row : p.M, p.M, step * CHUNKS, p.groups, p.vec_scales);
+      if (!RAW) xo = load_scale_words(p.x_scales, row < TOKENS ? m0 + row : p.M, p.M, step * CHUNKS, p.groups, p.vec_scales);
     };
+    if (RAW) {
+      quantize_tokens<typename std::conditional<RAW, X, float>::type, XF>(p, step0 * STEP, (step1 - step0) * STEP, raw_tiles, raw_scales, t);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(raw_full);
+    }
 #pragma unroll
     for (int u = 0; u < 4; ++u) load(step0 + u, wv[u], xv[u]);
     for (int step = step0; step < step1 && ok; step += 4) {
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        if (step + u >= step1) break;
+        if (step + u >= step1 || !ok) break;
         const int b = u & 1;
         ok = warp_mbar_wait(&sf_empty[b], u < 2 ? 1u : 0u, 4);
         if (!ok) break;
         unsigned char* to = scale_tiles + b * L::SCALES;
         put_scale_words(to, t, wv[u]);
-        put_scale_words(to + CHUNKS * SCALE_TILE, t, xv[u]);
+        if (!RAW) put_scale_words(to + L::STEP_SCALES, t, xv[u]);
         __syncwarp();
         if (lane == 0) mbar_arrive(&sf_full[b]);
         load(step + u + 4, wv[u], xv[u]);
@@ -782,18 +844,19 @@ static int allow_smem(size_t bytes) {
   return NES_OK;
 }
 
-template <int XF, int WF, int TOKENS>
+template <int XF, int WF, int TOKENS, typename X = void>
 static int launch_product(const Product& p, const void* x, const void* w, cudaStream_t st) {
-  using L = Layout<TOKENS>;
+  using L = Layout<TOKENS, !std::is_same<X, void>::value, XF == NES_MXFP4 ? 2 : 4>;
   ProductMaps maps;
   int rc = code_map(&maps.w, w, p.N, p.groups, WF == NES_MXFP4, WF == NES_MXFP4 && XF == NES_MXFP8, FEATURES);
   if (rc != NES_OK) return rc;
-  if ((rc = code_map(&maps.x, x, p.M, p.groups, XF == NES_MXFP4, false, TOKENS)) != NES_OK) return rc;
+  maps.x = maps.w;
+  if (std::is_same<X, void>::value && (rc = code_map(&maps.x, x, p.M, p.groups, XF == NES_MXFP4, false, TOKENS)) != NES_OK) return rc;
   const int64_t ftiles = ceil_div<int64_t>(p.N, FEATURES), ttiles = ceil_div<int64_t>(p.M, TOKENS);
   const int steps = ceil_div(p.groups, CHUNKS);
   const int splits = choose_splits(ftiles * ttiles, steps);
   NES_REQUIRE(ttiles <= 65535 && ftiles * splits <= INT32_MAX, NES_ERR_UNSUPPORTED, "mx_linear_fwd: too large");
-  if ((rc = allow_smem<mx_product_kernel<XF, WF, TOKENS>>(L::SMEM)) != NES_OK) return rc;
+  if ((rc = allow_smem<mx_product_kernel<XF, WF, TOKENS, X>>(L::SMEM)) != NES_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(ftiles * splits), unsigned(ttiles));
   cfg.blockDim = dim3(THREADS_TC);
@@ -805,7 +868,7 @@ static int launch_product(const Product& p, const void* x, const void* w, cudaSt
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, mx_product_kernel<XF, WF, TOKENS>, maps, p, splits);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, mx_product_kernel<XF, WF, TOKENS, X>, maps, p, splits);
   if (e != cudaSuccess) return fail(NES_ERR_LAUNCH, "mx_linear_fwd: %s", cudaGetErrorString(e));
   return check_launch("mx_linear_fwd");
 }
@@ -837,6 +900,23 @@ static int launch_pair(const Product& p, const void* x, const void* w, cudaStrea
   const int64_t pairs = tiles < sm_count() / 2 ? tiles : sm_count() / 2;
   mx_pair_kernel<XF, WF><<<unsigned(pairs * 2), THREADS_PAIR, L::SMEM, st>>>(maps, p, int(ftiles), int(ttiles), tma_out);
   return check_launch("mx_linear_fwd");
+}
+
+// Whether the product quantises its plain activations itself: few tokens, and a part of K per CTA that fits its shared memory.
+// Every feature tile's CTAs do so before their first product, at about 0.23 us per 8 elements of a thread (of 128); a
+// launch of its own costs the device 1.8 us and the host 4 us (1 token of 4096x4096: 7.9 us, else 8.6; 16 tokens: 11.3 and 9.0).
+static bool quantises_itself(int64_t M, int64_t N, int64_t K) {
+  if (M > 16) return false;
+  const int steps = int(ceil_div<int64_t>(K, STEP));
+  const int64_t mine = ceil_div<int64_t>(steps, choose_splits(ceil_div<int64_t>(N, FEATURES), steps));
+  return mine <= RAW_STEPS && M * mine * STEP <= 16 * 128 * UNIT;
+}
+
+template <int XF, int WF>
+static int launch_raw(const Product& p, int x_dtype, const void* w, cudaStream_t st) {
+  if (x_dtype == NES_F32) return launch_product<XF, WF, 16, float>(p, nullptr, w, st);
+  if (x_dtype == NES_BF16) return launch_product<XF, WF, 16, __nv_bfloat16>(p, nullptr, w, st);
+  return launch_product<XF, WF, 16, __half>(p, nullptr, w, st);
 }
 
 template <int XF, int WF>
@@ -871,7 +951,7 @@ using namespace nes;
 using namespace nes::mx;
 
 extern "C" int64_t nes_mx_linear_fwd_scratch_bytes(int64_t M, int64_t N, int64_t K, int x_format) {
-  if (M <= 0 || N <= 0 || K <= 0 || !known_format(x_format)) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || !known_format(x_format) || quantises_itself(M, N, K)) return 0;
   return align256(M * code_pitch(K, x_format)) + align256(M * scale_pitch(K));
 }
 
@@ -886,7 +966,19 @@ extern "C" int nes_mx_linear_fwd(const void* x, const uint8_t* x_scales, int x_d
   NES_REQUIRE(x && w_codes && w_scales && y, NES_ERR_BAD_ARG, "mx_linear_fwd: null pointer");
   NES_REQUIRE(aligned32(w_codes) && (!x_scales || aligned32(x)), NES_ERR_BAD_ARG, "mx_linear_fwd: codes must be 32-byte aligned");
   NES_REQUIRE(M <= INT32_MAX / 2 && N <= INT32_MAX / 2 && K <= INT32_MAX / 2, NES_ERR_UNSUPPORTED, "mx_linear_fwd: too large");
+  NES_REQUIRE((reinterpret_cast<uintptr_t>(x_scales) & 3u) == 0 && (reinterpret_cast<uintptr_t>(w_scales) & 3u) == 0, NES_ERR_BAD_ARG,
+              "mx_linear_fwd: scales must be 4-byte aligned");
   cudaStream_t st = as_stream(stream);
+  Product p;
+  p.x_scales = x_scales; p.w_scales = w_scales; p.bias = bias; p.y = y; p.x = x; p.whole_rows = 0;
+  p.M = int(M); p.N = int(N); p.K = int(K); p.groups = int(padded(K) / GROUP); p.y_dtype = y_dtype;
+  p.vec_scales = p.groups % CHUNKS == 0 && aligned16(x_scales) && aligned16(w_scales);
+  if (!x_scales && quantises_itself(M, N, K)) {
+    p.whole_rows = aligned16(x) && (K * dtype_bytes(x_dtype)) % 16 == 0;
+    if (x_format == NES_MXFP4) return launch_raw<NES_MXFP4, NES_MXFP4>(p, x_dtype, w_codes, st);
+    if (w_format == NES_MXFP4) return launch_raw<NES_MXFP8, NES_MXFP4>(p, x_dtype, w_codes, st);
+    return launch_raw<NES_MXFP8, NES_MXFP8>(p, x_dtype, w_codes, st);
+  }
   if (!x_scales) {
     const int64_t need = nes_mx_linear_fwd_scratch_bytes(M, N, K, x_format);
     NES_REQUIRE(scratch && scratch_bytes >= need && aligned32(scratch), NES_ERR_SCRATCH,
@@ -896,14 +988,8 @@ extern "C" int nes_mx_linear_fwd(const void* x, const uint8_t* x_scales, int x_d
     const int rc = nes_mx_quantize(x, x_dtype, codes, scales, M, K, x_format, stream);
     if (rc != NES_OK) return rc;
     x = codes;
-    x_scales = scales;
+    p.x_scales = scales;
   }
-  Product p;
-  p.x_scales = x_scales; p.w_scales = w_scales; p.bias = bias; p.y = y;
-  p.M = int(M); p.N = int(N); p.groups = int(padded(K) / GROUP); p.y_dtype = y_dtype;
-  NES_REQUIRE((reinterpret_cast<uintptr_t>(x_scales) & 3u) == 0 && (reinterpret_cast<uintptr_t>(w_scales) & 3u) == 0, NES_ERR_BAD_ARG,
-              "mx_linear_fwd: scales must be 4-byte aligned");
-  p.vec_scales = p.groups % CHUNKS == 0 && aligned16(x_scales) && aligned16(w_scales);
   if (x_format == NES_MXFP4) return launch_tokens<NES_MXFP4, NES_MXFP4>(p, x, w_codes, st);
   if (w_format == NES_MXFP4) return launch_tokens<NES_MXFP8, NES_MXFP4>(p, x, w_codes, st);
   return launch_tokens<NES_MXFP8, NES_MXFP8>(p, x, w_codes, st);
