@@ -39,12 +39,16 @@ def _pitches(cols, format):
     return groups * (64 if format == "mxfp4" else 128), groups * 4
 
 
+_current_device, _raw_stream = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
+
+
 def _launch(name, device, *args):
     """Calls an entry point on ``device`` and the stream that is current there."""
-    if device.index == torch.cuda.current_device():
-        return C.call(name, *args, C.stream())
+    index = device.index
+    if index == _current_device():
+        return C.call(name, *args, _raw_stream(index))
     with torch.cuda.device(device):
-        return C.call(name, *args, C.stream())
+        return C.call(name, *args, _raw_stream(index))
 
 
 def _same_device(device, name, t):
@@ -60,7 +64,7 @@ class MicroscaledTensor:
     contiguous CUDA tensors whose padding is zero.  ``shape`` gives the leading dimensions if there are several (their
     product is ``rows``).  The object refers to the tensors it is given."""
 
-    __slots__ = ("codes", "scales", "shape", "rows", "cols", "format")
+    __slots__ = ("codes", "scales", "rows", "cols", "format", "_lead")
 
     def __init__(self, codes, scales, cols, format="mxfp4", shape=None):
         _format(format)
@@ -82,13 +86,11 @@ class MicroscaledTensor:
         lead = (rows,) if shape is None else tuple(int(s) for s in shape)
         if math.prod(lead) != rows:
             raise RuntimeError("leading dimensions %s do not match %d rows" % (lead, rows))
-        self._set(codes, scales, lead, rows, cols, format)
+        self.codes, self.scales, self.rows, self.cols, self.format, self._lead = codes, scales, rows, cols, format, lead
 
-    def _set(self, codes, scales, lead, rows, cols, format):
-        self.codes, self.scales = codes, scales
-        self.shape = torch.Size((*lead, cols))
-        self.rows, self.cols, self.format = rows, cols, format
-        return self
+    @property
+    def shape(self):
+        return torch.Size((*self._lead, self.cols))
 
     @property
     def device(self):
@@ -101,7 +103,7 @@ class MicroscaledTensor:
         """The first ``width`` columns of a row-major byte matrix, with this tensor's leading dimensions."""
         if t.shape[1] != width:
             t = t.narrow(1, 0, width)
-        return t if len(self.shape) == 2 else t.unflatten(0, self.shape[:-1])
+        return t if len(self._lead) == 1 else t.unflatten(0, self._lead)
 
     def block_scales(self):
         """``(..., ceil(cols / 32))`` scales as ``torch.float8_e8m0fnu`` (a view)."""
@@ -112,8 +114,9 @@ class MicroscaledTensor:
         unpacked for ``"mxfp4"`` (every e2m1 value is an e4m3 value)."""
         if self.format == "mxfp8":
             return self._view(self.codes, self.cols).view(torch.float8_e4m3fn)
-        out = self.codes.new_empty(self.shape, dtype=torch.float8_e4m3fn)
-        _launch("nes_mx_elements", self.codes.device, self.codes.data_ptr(), out.data_ptr(), self.rows, self.cols)
+        codes = self.codes
+        out = codes.new_empty((*self._lead, self.cols), dtype=torch.float8_e4m3fn)
+        _launch("nes_mx_elements", codes.device, codes.data_ptr(), out.data_ptr(), self.rows, self.cols)
         return out
 
     def dequantize(self, dtype=torch.float32):
@@ -128,9 +131,11 @@ class MicroscaledTensor:
 def _empty(x, rows, cols, format):
     """Uninitialised blocks for ``rows`` rows, with the leading dimensions and on the device of ``x``."""
     pitch, spitch = _pitches(cols, format)
-    return MicroscaledTensor.__new__(MicroscaledTensor)._set(
-        x.new_empty((rows, pitch), dtype=torch.uint8), x.new_empty((rows, spitch), dtype=torch.uint8), x.shape[:-1],
-        rows, cols, format)
+    q = MicroscaledTensor.__new__(MicroscaledTensor)
+    q.codes = x.new_empty((rows, pitch), dtype=torch.uint8)
+    q.scales = x.new_empty((rows, spitch), dtype=torch.uint8)
+    q.rows, q.cols, q.format, q._lead = rows, cols, format, x.shape[:-1]
+    return q
 
 
 def _aligned(t):
@@ -165,22 +170,22 @@ def linear(input, weight, bias=None, activations="mxfp8", dtype=None, out=None):
     Products are accumulated in fp32 and rounded once to ``dtype`` (default: the type of a plain input, float32 for a
     microscaled one).  8-bit activations take weights of either format, 4-bit activations 4-bit weights.  ``out``
     receives the result if given (contiguous, of the result's type and number of elements)."""
-    if not isinstance(weight, MicroscaledTensor) or len(weight.shape) != 2:
+    if not isinstance(weight, MicroscaledTensor) or len(weight._lead) != 1:
         raise RuntimeError("weight must be a MicroscaledTensor of (out_features, in_features)")
-    out_features, in_features = weight.shape
+    out_features, in_features = weight.rows, weight.cols
     x_scales, x_kind = None, 0
     if isinstance(input, MicroscaledTensor):
         x, rows, activations, default = input.codes, input.rows, input.format, torch.float32
-        x_scales = input.scales.data_ptr()
+        x_scales, lead, cols = input.scales.data_ptr(), input._lead, input.cols
     else:
         x, rows = _rows(input, "input")
-        x_kind, default = _DTYPES[x.dtype], x.dtype
+        x_kind, default, lead, cols = _DTYPES[x.dtype], x.dtype, x.shape[:-1], x.shape[-1]
     if dtype is None:
         dtype = default if out is None else out.dtype
     x_format, y_kind = _format(activations, "activations"), _dtype(dtype, "the result")
     device = x.device
-    if input.shape[-1] != in_features:
-        raise RuntimeError("expected last dimension %d, got %d" % (in_features, input.shape[-1]))
+    if cols != in_features:
+        raise RuntimeError("expected last dimension %d, got %d" % (in_features, cols))
     _same_device(device, "weight", weight.codes)
     if bias is not None:
         bias = C.require_cuda(bias, "bias", torch.float32)
@@ -189,7 +194,7 @@ def linear(input, weight, bias=None, activations="mxfp8", dtype=None, out=None):
         _same_device(device, "bias", bias)
     y = out
     if out is None:
-        y = x.new_empty((*input.shape[:-1], out_features), dtype=dtype)
+        y = x.new_empty((*lead, out_features), dtype=dtype)
     elif out.device != device or out.dtype != dtype or not out.is_contiguous() or out.numel() != rows * out_features:
         raise RuntimeError("out must be a contiguous %s tensor of %d elements on %s" % (dtype, rows * out_features, device))
     buf, nbytes = None, 0
