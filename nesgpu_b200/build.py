@@ -1,4 +1,5 @@
-"""Builds ``nesgpu_b200/lib/libnesgpu_b200.so`` (sm_100a only) from ``nesgpu_b200/csrc/*.cu``.
+"""Builds ``nesgpu_b200/lib/libnesgpu_b200.so`` (sm_100a only) from ``nesgpu_b200/csrc/*.cu`` and the extension module
+``nesgpu_b200/_host.so`` (host code that allocates through PyTorch and calls the library) from ``csrc/*_host.cpp``.
 
 Usage: ``python -m nesgpu_b200.build [--force] [--verbose]``.  nvcc cross-compiles without a
 GPU; the shared library is kept in-tree next to the package.
@@ -7,11 +8,13 @@ import concurrent.futures
 import os
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libnesgpu_b200.so")
+HOST_PATH = os.path.join(PKG, "_host.so")
 OBJ_DIR = os.path.join(PKG, "build")
 INCLUDE = os.path.join(os.path.dirname(PKG), "include")
 
@@ -44,15 +47,44 @@ def _compile(src, verbose):
     return obj, res.stderr
 
 
+def _torch_dir():
+    import torch
+    return os.path.dirname(torch.__file__)
+
+
+def _compile_host():
+    """Object of the extension module: PyTorch's headers, no CUDA code."""
+    src, obj = os.path.join(CSRC, "microscaling_host.cpp"), os.path.join(OBJ_DIR, "microscaling_host.o")
+    torch_include = os.path.join(_torch_dir(), "include")
+    include = [torch_include, os.path.join(torch_include, "torch", "csrc", "api", "include"),
+               sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-c", src, "-o", obj] + ["-I" + d for d in include]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError("g++ failed for %s:\n%s\n%s" % (src, res.stdout, res.stderr))
+    return obj
+
+
+def _link_host(obj):
+    cmd = ["g++", "-shared", "-o", HOST_PATH, obj, "-L" + LIB_DIR, "-lnesgpu_b200", "-Wl,-rpath,$ORIGIN/lib",
+           "-L" + os.path.join(_torch_dir(), "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError("link failed:\n%s\n%s" % (res.stdout, res.stderr))
+
+
 def build(force=False, verbose=False):
-    """Compile every CUDA source for sm_100a and link the shared library.  Returns its path."""
+    """Compile every CUDA source for sm_100a and link the shared library and the extension module.  Returns the
+    library's path."""
     os.makedirs(LIB_DIR, exist_ok=True)
     os.makedirs(OBJ_DIR, exist_ok=True)
-    if not force and os.path.exists(LIB_PATH) and os.path.getmtime(LIB_PATH) >= _deps_mtime():
+    if not force and all(os.path.exists(p) and os.path.getmtime(p) >= _deps_mtime() for p in (LIB_PATH, HOST_PATH)):
         return LIB_PATH
     srcs = sources()
-    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as pool:
+    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as pool:
+        host = pool.submit(_compile_host)
         results = list(pool.map(lambda s: _compile(s, verbose), srcs))
+        host_obj = host.result()
     if verbose:
         for _, log in results:
             sys.stderr.write(log)
@@ -61,6 +93,7 @@ def build(force=False, verbose=False):
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError("link failed:\n%s\n%s" % (res.stdout, res.stderr))
+    _link_host(host_obj)
     return LIB_PATH
 
 

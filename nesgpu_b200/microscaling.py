@@ -14,11 +14,16 @@ import math
 import torch
 from torch import nn
 
-from . import _cabi as C
+from . import _cabi as C         # loads the library that the extension module is linked with
+
+try:
+    from . import _host
+except ImportError as e:
+    raise RuntimeError("nesgpu_b200: the extension module _host cannot be loaded (%s). Build it with `python -m "
+                       "nesgpu_b200.build`; there is no fallback path." % e) from e
 
 BLOCK = 32
 FORMATS = {"mxfp4": 4, "mxfp8": 8}
-_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 def _format(name, what="format"):
@@ -27,33 +32,10 @@ def _format(name, what="format"):
     return FORMATS[name]
 
 
-def _dtype(dtype, what):
-    if dtype not in _DTYPES:
-        raise NotImplementedError("nesgpu_b200: %s must have dtype float32, bfloat16 or float16, got %s" % (what, dtype))
-    return _DTYPES[dtype]
-
-
 def _pitches(cols, format):
     """Bytes of codes and of scales per row: rows are padded to whole groups of 128 elements."""
     groups = -(-cols // 128)
     return groups * (64 if format == "mxfp4" else 128), groups * 4
-
-
-_current_device, _raw_stream = torch.cuda.current_device, torch._C._cuda_getCurrentRawStream
-
-
-def _launch(name, device, *args):
-    """Calls an entry point on ``device`` and the stream that is current there."""
-    index = device.index
-    if index == _current_device():
-        return C.call(name, *args, _raw_stream(index))
-    with torch.cuda.device(device):
-        return C.call(name, *args, _raw_stream(index))
-
-
-def _same_device(device, name, t):
-    if t is not None and t.device != device:
-        raise RuntimeError("nesgpu_b200: %s is on %s, expected %s" % (name, t.device, device))
 
 
 class MicroscaledTensor:
@@ -73,7 +55,8 @@ class MicroscaledTensor:
             raise RuntimeError("a microscaled tensor needs at least one column")
         codes = C.require_cuda(codes, "codes", torch.uint8)
         scales = C.require_cuda(scales, "scales", torch.uint8)
-        _same_device(codes.device, "scales", scales)
+        if scales.device != codes.device:
+            raise RuntimeError("nesgpu_b200: scales is on %s, expected %s" % (scales.device, codes.device))
         pitch, spitch = _pitches(cols, format)
         rows = codes.shape[0] if codes.dim() else 0
         if codes.shape != (rows, pitch) or scales.shape != (rows, spitch):
@@ -99,68 +82,31 @@ class MicroscaledTensor:
     def __repr__(self):
         return "MicroscaledTensor(shape=%s, format=%s, device=%s)" % (tuple(self.shape), self.format, self.device)
 
-    def _view(self, t, width):
-        """The first ``width`` columns of a row-major byte matrix, with this tensor's leading dimensions."""
-        if t.shape[1] != width:
-            t = t.narrow(1, 0, width)
-        return t if len(self._lead) == 1 else t.unflatten(0, self._lead)
-
     def block_scales(self):
         """``(..., ceil(cols / 32))`` scales as ``torch.float8_e8m0fnu`` (a view)."""
-        return self._view(self.scales, -(-self.cols // BLOCK)).view(torch.float8_e8m0fnu)
+        return _host.block_scales(self.scales, self.cols, self._lead)
 
     def elements(self):
         """``(..., cols)`` element values before the scale, as ``torch.float8_e4m3fn``: a view for ``"mxfp8"``,
         unpacked for ``"mxfp4"`` (every e2m1 value is an e4m3 value)."""
-        if self.format == "mxfp8":
-            return self._view(self.codes, self.cols).view(torch.float8_e4m3fn)
-        codes = self.codes
-        out = codes.new_empty((*self._lead, self.cols), dtype=torch.float8_e4m3fn)
-        _launch("nes_mx_elements", codes.device, codes.data_ptr(), out.data_ptr(), self.rows, self.cols)
-        return out
+        return _host.elements(self.codes, self.cols, self._lead, FORMATS[self.format])
 
     def dequantize(self, dtype=torch.float32):
         """The values ``element * scale`` (exact in fp32; rounded to nearest even in bfloat16 and float16)."""
-        kind = _dtype(dtype, "the result")
-        out = self.codes.new_empty(self.shape, dtype=dtype)
-        _launch("nes_mx_dequantize", self.codes.device, self.codes.data_ptr(), self.scales.data_ptr(), out.data_ptr(), kind,
-                self.rows, self.cols, FORMATS[self.format])
-        return out
+        return _host.dequantize(self.codes, self.scales, self.cols, self._lead, FORMATS[self.format], dtype)
 
 
-def _empty(x, rows, cols, format):
-    """Uninitialised blocks for ``rows`` rows, with the leading dimensions and on the device of ``x``."""
-    pitch, spitch = _pitches(cols, format)
+def _made(blocks, format):
+    """The tensor of blocks that a call has just written."""
     q = MicroscaledTensor.__new__(MicroscaledTensor)
-    q.codes = x.new_empty((rows, pitch), dtype=torch.uint8)
-    q.scales = x.new_empty((rows, spitch), dtype=torch.uint8)
-    q.rows, q.cols, q.format, q._lead = rows, cols, format, x.shape[:-1]
+    q.codes, q.scales, q.rows, q.cols, q._lead = blocks
+    q.format = format
     return q
-
-
-def _aligned(t):
-    """``t`` at an address that is a multiple of 16 bytes (a copy if it starts inside an allocation)."""
-    return t if t is None or t.data_ptr() % 16 == 0 else t.clone()
-
-
-def _rows(t, name):
-    """A contiguous CUDA tensor of a supported type with at least one column, and its number of rows."""
-    t = C.require_cuda(t, name)
-    _dtype(t.dtype, name)
-    if t.dim() == 0 or t.shape[-1] == 0:
-        raise RuntimeError("%s needs at least one column, got shape %s" % (name, tuple(t.shape)))
-    return t, t.numel() // t.shape[-1]
 
 
 def quantize(input, format="mxfp4"):
     """``(..., cols)`` float32 / bfloat16 / float16 -> :class:`MicroscaledTensor`."""
-    kind = _format(format)
-    x, rows = _rows(input, "input")
-    cols = x.shape[-1]
-    q = _empty(x, rows, cols, format)
-    _launch("nes_mx_quantize", x.device, x.data_ptr(), _DTYPES[x.dtype], q.codes.data_ptr(), q.scales.data_ptr(), rows,
-            cols, kind)
-    return q
+    return _made(_host.quantize(input, _format(format)), format)
 
 
 def linear(input, weight, bias=None, activations="mxfp8", dtype=None, out=None):
@@ -172,40 +118,11 @@ def linear(input, weight, bias=None, activations="mxfp8", dtype=None, out=None):
     receives the result if given (contiguous, of the result's type and number of elements)."""
     if not isinstance(weight, MicroscaledTensor) or len(weight._lead) != 1:
         raise RuntimeError("weight must be a MicroscaledTensor of (out_features, in_features)")
-    out_features, in_features = weight.rows, weight.cols
-    x_scales, x_kind = None, 0
     if isinstance(input, MicroscaledTensor):
-        x, rows, activations, default = input.codes, input.rows, input.format, torch.float32
-        x_scales, lead, cols = input.scales.data_ptr(), input._lead, input.cols
-    else:
-        x, rows = _rows(input, "input")
-        x_kind, default, lead, cols = _DTYPES[x.dtype], x.dtype, x.shape[:-1], x.shape[-1]
-    if dtype is None:
-        dtype = default if out is None else out.dtype
-    x_format, y_kind = _format(activations, "activations"), _dtype(dtype, "the result")
-    device = x.device
-    if cols != in_features:
-        raise RuntimeError("expected last dimension %d, got %d" % (in_features, cols))
-    _same_device(device, "weight", weight.codes)
-    if bias is not None:
-        bias = C.require_cuda(bias, "bias", torch.float32)
-        if bias.shape != (out_features,):
-            raise RuntimeError("bias must have shape (%d,), got %s" % (out_features, tuple(bias.shape)))
-        _same_device(device, "bias", bias)
-    y = out
-    if out is None:
-        y = x.new_empty((*lead, out_features), dtype=dtype)
-    elif out.device != device or out.dtype != dtype or not out.is_contiguous() or out.numel() != rows * out_features:
-        raise RuntimeError("out must be a contiguous %s tensor of %d elements on %s" % (dtype, rows * out_features, device))
-    buf, nbytes = None, 0
-    if x_scales is None:
-        nbytes = C.call("nes_mx_linear_fwd_scratch_bytes", rows, out_features, in_features, x_format)
-        if nbytes:      # a buffer of this call's own: calls captured into different graphs share nothing
-            buf = x.new_empty(nbytes, dtype=torch.uint8)
-    _launch("nes_mx_linear_fwd", device, x.data_ptr(), x_scales, x_kind, x_format, weight.codes.data_ptr(),
-            weight.scales.data_ptr(), FORMATS[weight.format], C.ptr(bias), y.data_ptr(), y_kind, rows, out_features,
-            in_features, C.ptr(buf), nbytes)
-    return y
+        return _host.linear(input.codes, input.scales, input._lead, input.cols, FORMATS[input.format], weight.codes,
+                            weight.scales, weight.cols, FORMATS[weight.format], bias, dtype, out)
+    return _host.linear(input, None, None, 0, _format(activations, "activations"), weight.codes, weight.scales,
+                        weight.cols, FORMATS[weight.format], bias, dtype, out)
 
 
 def rms_norm(input, weight=None, eps=1e-6, residual=None, noise=None, antithetic=False, output=None):
@@ -216,41 +133,10 @@ def rms_norm(input, weight=None, eps=1e-6, residual=None, noise=None, antithetic
     ``(members, cols)`` float32 adds ``noise[d]`` to the gain of the rows ``r * members + d`` (its negative for the
     second half of the repeats with ``antithetic``).  ``output`` is None for a ``y`` of the input's type, or
     ``"mxfp8"`` / ``"mxfp4"`` for a :class:`MicroscaledTensor`."""
-    x, rows = _rows(input, "input")
-    cols, device = x.shape[-1], x.device
-    kind = 0 if output is None or output == x.dtype else _format(output, "output")
-    if not eps >= 0:
-        raise RuntimeError("eps must not be negative, got %r" % (eps,))
-    h, members = None, 0
-    if residual is not None:
-        if not isinstance(residual, torch.Tensor) or residual.shape != x.shape:
-            raise RuntimeError("residual must have the input's shape %s" % (tuple(x.shape),))
-        residual = C.require_cuda(residual, "residual", x.dtype)
-        _same_device(device, "residual", residual)
-        h = torch.empty_like(x)
-    if weight is not None:
-        weight = C.require_cuda(weight, "weight", torch.float32)
-        if weight.shape != (cols,):
-            raise RuntimeError("weight must have shape (%d,), got %s" % (cols, tuple(weight.shape)))
-        _same_device(device, "weight", weight)
-    if noise is not None:
-        noise = C.require_cuda(noise, "noise", torch.float32)
-        members = noise.shape[0] if noise.dim() else 0
-        if not members or noise.shape != (members, cols):
-            raise RuntimeError("noise must have shape (members, %d), got %s" % (cols, tuple(noise.shape)))
-        if rows % members:
-            raise RuntimeError("batch size %d is not a multiple of directions %d" % (rows, members))
-        _same_device(device, "noise", noise)
-    if kind:
-        y = _empty(x, rows, cols, output)
-        data, scales = y.codes.data_ptr(), y.scales.data_ptr()
-    else:
-        y = torch.empty_like(x)
-        data, scales = y.data_ptr(), None
-    x, residual, weight, noise = _aligned(x), _aligned(residual), _aligned(weight), _aligned(noise)
-    _launch("nes_rms_norm_fwd", device, x.data_ptr(), C.ptr(residual), C.ptr(h), C.ptr(weight), C.ptr(noise), data,
-            scales, rows, cols, members, 1 if antithetic else 0, _DTYPES[x.dtype], kind, eps)
-    return y if residual is None else (y, h)
+    if output is None or output == getattr(input, "dtype", None):
+        return _host.rms_norm(input, weight, eps, residual, noise, antithetic, 0)
+    got = _host.rms_norm(input, weight, eps, residual, noise, antithetic, _format(output, "output"))
+    return _made(got, output) if residual is None else (_made(got[0], output), got[1])
 
 
 class MicroscaledLinear(nn.Module):
@@ -285,7 +171,8 @@ class MicroscaledLinear(nn.Module):
         return MicroscaledTensor(self.weight_codes, self.weight_scales, self.in_features, self.format)
 
     def forward(self, input, dtype=None):
-        return linear(input, self.weight, self.bias, self.activations, dtype)
+        bias = self.bias if self.bias is None or self.bias.dtype == torch.float32 else self.bias.float()
+        return linear(input, self.weight, bias, self.activations, dtype)
 
     def extra_repr(self):
         return "in_features=%d, out_features=%d, bias=%s, format=%s, activations=%s" % (

@@ -104,6 +104,9 @@ def test_quantize_leading_dimensions_strides_and_alignment():
     flat = _inputs(1, 8 * 128 + 1, "fp16", 7).view(-1)
     off = flat[1:].view(8, 128)                       # rows start 2 bytes past a 16-byte boundary
     _check_quantized(ms.quantize(off, "mxfp4"), _f64(off), "mxfp4")
+    row = ms.quantize(x[5], "mxfp8")                  # no leading dimension at all
+    assert tuple(row.shape) == (96,) and tuple(row.elements().shape) == (96,) and tuple(row.block_scales().shape) == (3,)
+    _check_quantized(row, _f64(x[5:6]), "mxfp8")
     empty = ms.quantize(torch.empty(0, 64, device="cuda"))
     assert tuple(empty.dequantize().shape) == (0, 64) and tuple(empty.elements().shape) == (0, 64)
     assert tuple(empty.block_scales().shape) == (0, 2)
@@ -177,6 +180,7 @@ def test_rms_norm_defaults_and_shapes():
     assert tuple(y.shape) == (2, 3, 4, 48) and y.dtype == torch.bfloat16
     want, _ = O.rms_norm(_f64(x), None, float(np.float32(1e-6)))
     _check_norm(y.view(24, 48), want, None, "bf16")
+    assert torch.equal(ms.rms_norm(x[3]), ms.rms_norm(x)[3])
     y, h = ms.rms_norm(x.view(4, 6, 48), residual=x.view(4, 6, 48), output="mxfp8")
     assert tuple(y.shape) == (4, 6, 48) and tuple(h.shape) == (4, 6, 48)
     strided = _inputs(10, 100, "fp32", 4)[:, 3:60]
@@ -283,6 +287,7 @@ def test_linear_types_shapes_and_out():
     x = _inputs(12, 64, "fp16", 1)
     codes, scales = O.quantize(_f64(x), "mxfp8")
     x64 = O.values(codes, scales, "mxfp8")
+    assert torch.equal(ms.linear(x[3], w), ms.linear(x[3:4], w)[0]) and ms.linear(ms.quantize(x[3]), w).shape == (48,)
     y = ms.linear(x.view(3, 4, 64), w)
     assert tuple(y.shape) == (3, 4, 48) and y.dtype == torch.float16
     _check_linear(y.view(12, 48), x64, w64, None, torch.float16)
@@ -304,6 +309,12 @@ def test_rows_do_not_depend_on_their_neighbours():
     assert (buf[300] == 3).all()
     again = ms.linear(x, w, activations="mxfp4")
     assert torch.equal(buf[:300], again)
+    w, _ = _weight(ms, 4104, 512, "mxfp4", 0)                # and through boxes that are cut off at the edges
+    x = _inputs(1100, 512, "bf16", 1)
+    for dtype in (torch.bfloat16, torch.float32):
+        buf = torch.full((1101, 4104), 3.0, device="cuda", dtype=dtype)
+        ms.linear(x, w, out=buf[:1100])
+        assert (buf[1100] == 3).all() and torch.equal(buf[:1100], ms.linear(x, w, dtype=dtype))
 
 
 # ---------------------------------------------------------------------------------------------------- refusals
@@ -340,3 +351,11 @@ def test_refusals():
         ms.rms_norm(x, eps=-1.0)
     with pytest.raises(RuntimeError, match="CUDA"):
         ms.linear(x, q, torch.zeros(4))
+    with pytest.raises(RuntimeError, match="weight must"):
+        ms.rms_norm(x, torch.ones(32, device="cuda"))
+    with pytest.raises(NotImplementedError, match="bfloat16"):
+        ms.rms_norm(x, torch.ones(64, device="cuda").bfloat16())
+    with pytest.raises(NotImplementedError, match="int32"):
+        ms.linear(x, q, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ms.linear([1.0], q)
