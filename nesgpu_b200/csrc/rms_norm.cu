@@ -118,17 +118,71 @@ __device__ __forceinline__ void store_boundary(T* row, int c, int cols, const Ra
   }
 }
 
-enum RowAccess { WHOLE, SHIFTED, ANY };          // ANY: the looping kernel's, units from column 8 i on wherever they lie
+// SPLIT: a unit is two runs of four columns, 128 apart, so that a warp's 16-byte accesses lie next to one another (fp32 rows in
+// units of eight consecutive columns reach every 32-byte sector twice, half of it each time, and so do their gains).
+enum RowAccess { WHOLE, SPLIT, SHIFTED, ANY };   // ANY: the looping kernel's, units from column 8 i on wherever they lie
+
+constexpr int HALF_APART = 128;
+__device__ __forceinline__ Raw<float> load_split(const float* row, int c, int cols) {
+  Raw<float> r;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (c + h * HALF_APART < cols) v = __ldg(reinterpret_cast<const uint4*>(row + c + h * HALF_APART));
+    r.w[4 * h] = v.x; r.w[4 * h + 1] = v.y; r.w[4 * h + 2] = v.z; r.w[4 * h + 3] = v.w;
+  }
+  return r;
+}
+__device__ __forceinline__ void store_split(float* row, int c, int cols, const Raw<float>& r) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    if (c + h * HALF_APART < cols) *reinterpret_cast<uint4*>(row + c + h * HALF_APART) = make_uint4(r.w[4 * h], r.w[4 * h + 1], r.w[4 * h + 2], r.w[4 * h + 3]);
+}
+// Quantises a split unit: its halves belong to two blocks, each held by eight neighbouring lanes; columns of the padding are zero.
+template <int FORMAT>
+__device__ __forceinline__ void quantize_split(float (&v)[UNIT], uint8_t* codes_row, uint8_t* scales_row, int c, int cols) {
+  const int end = int(padded(cols));
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int at = c + h * HALF_APART;
+    float* q = v + 4 * h;
+    if (at >= cols) q[0] = q[1] = q[2] = q[3] = 0.f;             // fp32 rows end on a multiple of four columns here
+    uint32_t m = __float_as_uint(max_magnitude(max_magnitude(q[0], q[1], q[2]), q[3], q[3])) & 0x7fffffffu;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const uint32_t code = scale_code<FORMAT>(m);
+    const float inv = inverse_scale(code);
+    if (at >= end) continue;
+    if (FORMAT == NES_MXFP4) {
+      const float e[UNIT] = {q[0] * inv, q[1] * inv, q[2] * inv, q[3] * inv, 0.f, 0.f, 0.f, 0.f};
+      *reinterpret_cast<uint16_t*>(codes_row + at / 2) = uint16_t(code == 255u ? 0u : pack_e2m1x8(e));
+    } else {
+      const uint32_t e = pack_e4m3x4(q[0] * inv, q[1] * inv, q[2] * inv, q[3] * inv);
+      *reinterpret_cast<uint32_t*>(codes_row + at) = code == 255u ? 0u : e;
+    }
+    if (at % BLOCK == 0) scales_row[at / BLOCK] = uint8_t(code);
+  }
+}
 
 template <RowAccess ACCESS, typename T>
 __device__ __forceinline__ Raw<T> load_at(const T* row, int c, int cols, const Span& span) {
-  if (ACCESS == SHIFTED) return load_boundary(row, c, cols, span);
-  return load_raw<ACCESS == WHOLE>(row, c, cols, span);
+  if constexpr (ACCESS == SPLIT) return load_split(row, c, cols);
+  else if constexpr (ACCESS == SHIFTED) return load_boundary(row, c, cols, span);
+  else return load_raw<ACCESS == WHOLE>(row, c, cols, span);
 }
 template <RowAccess ACCESS, typename T>
 __device__ __forceinline__ void store_at(T* row, int c, int cols, const Raw<T>& r) {
-  if (ACCESS == SHIFTED) store_boundary(row, c, cols, r);
+  if constexpr (ACCESS == SPLIT) store_split(row, c, cols, r);
+  else if constexpr (ACCESS == SHIFTED) store_boundary(row, c, cols, r);
   else store_raw<ACCESS == WHOLE, 32>(row, c, cols, r);
+}
+// gains and noise of a unit's columns, fp32 whatever the rows' type; a quantised output's shifted units have been moved by then
+template <RowAccess ACCESS, bool MOVED>
+__device__ __forceinline__ void load_gain(const float* row, int c, int cols, const Span& span, bool aligned_row, float (&g)[UNIT]) {
+  if constexpr (ACCESS == SPLIT) raw_values(load_split(row, c, cols), g);
+  else if constexpr (ACCESS == WHOLE) raw_values(load_raw<true>(row, c, cols, span), g);
+  else if (MOVED && aligned_row) raw_values(load_boundary(row, c, cols, span), g);
+  else raw_values(load_raw<false>(row, c, cols, span), g);
 }
 
 template <typename T, RowAccess ACCESS>
@@ -151,19 +205,18 @@ __device__ __forceinline__ void load_h(const NormArgs& a, const Row<T>& row, int
 // y of the unit at column c; all lanes of a warp call it.  A quantised output is stored from units of whole columns 8 i.
 template <typename T, int OUT, RowAccess ACCESS>
 __device__ __forceinline__ void emit(const NormArgs& a, const Row<T>& row, int64_t index, int c, const float (&h)[UNIT], float2 r) {
-  constexpr bool WHOLE_GAIN = ACCESS == WHOLE;
+  constexpr bool MOVED = ACCESS == SHIFTED && OUT != 0;
   const int cols = int(a.cols);
   float g[UNIT], y[UNIT];
   if (a.gain) {
-    if (ACCESS == SHIFTED && OUT != 0) raw_values(load_boundary(a.gain, c, cols, span_of(a.gain, cols)), g);
-    else raw_values(load_raw<WHOLE_GAIN>(a.gain, c, cols, span_of(a.gain, cols)), g);
+    load_gain<ACCESS, MOVED>(a.gain, c, cols, span_of(a.gain, cols), true, g);
   } else {
 #pragma unroll
     for (int i = 0; i < UNIT; ++i) g[i] = 1.f;
   }
   if (row.noise) {
     float n[UNIT];
-    raw_values(load_raw<WHOLE_GAIN>(row.noise, c, cols, span_of(a.noise, a.members * a.cols)), n);
+    load_gain<ACCESS, MOVED>(row.noise, c, cols, span_of(a.noise, a.members * a.cols), false, n);
 #pragma unroll
     for (int i = 0; i < UNIT; ++i) g[i] = fmaf(row.sign, n[i], g[i]);
   }
@@ -174,12 +227,17 @@ __device__ __forceinline__ void emit(const NormArgs& a, const Row<T>& row, int64
     return;
   }
   constexpr int FORMAT = OUT == 0 ? NES_MXFP8 : OUT;
+  uint8_t* codes = static_cast<uint8_t*>(a.y) + index * code_pitch(cols, FORMAT);
+  uint8_t* scales = a.scales + index * scale_pitch(cols);
+  if (ACCESS == SPLIT) {
+    quantize_split<FORMAT>(y, codes, scales, c, cols);
+    return;
+  }
   if (c + UNIT > cols) {                          // columns of the padding are zero whatever the row's scale (0 * inf is not)
 #pragma unroll
     for (int i = 0; i < UNIT; ++i) if (c + i >= cols) y[i] = 0.f;
   }
-  quantize_unit<FORMAT>(y, static_cast<uint8_t*>(a.y) + index * code_pitch(cols, FORMAT), a.scales + index * scale_pitch(cols), c / UNIT,
-                        c < int(padded(cols)));
+  quantize_unit<FORMAT>(y, codes, scales, c / UNIT, c < int(padded(cols)));
 }
 
 // h of columns 8 i ... from units that begin `shift` elements earlier: the end of the unit `from` and the start of the next
@@ -234,7 +292,8 @@ __global__ void __launch_bounds__(BLOCK_ROW ? MOST_WARPS * 32 : WARP_ROWS * 32) 
   const int64_t index = BLOCK_ROW ? int64_t(blockIdx.x) : int64_t(blockIdx.x) * WARP_ROWS + warp;
   if (index >= a.rows) return;
   const Row<T> row(a, index);
-  const int first = ((BLOCK_ROW ? warp * UNITS * 32 : 0) + lane) * UNIT, shift = ACCESS == SHIFTED ? row.shift : 0;
+  const int base = BLOCK_ROW ? warp * UNITS * 32 * UNIT : 0, first = base + lane * (ACCESS == SPLIT ? 4 : UNIT);
+  const int shift = ACCESS == SHIFTED ? row.shift : 0;
   const int end = OUT != 0 ? int(padded(a.cols)) : int(a.cols) + shift;
   float v[UNITS + 1][UNIT];
 #pragma unroll
@@ -246,12 +305,12 @@ __global__ void __launch_bounds__(BLOCK_ROW ? MOST_WARPS * 32 : WARP_ROWS * 32) 
   for (int u = 0; u < UNITS; ++u) s += square_sum(v[u]);
   if (row.h) {
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) if (first - lane * UNIT + u * 32 * UNIT < int(a.cols) + shift) store_at<ACCESS>(row.h, first - shift + u * 32 * UNIT, int(a.cols), values_raw(v[u], T()));
+    for (int u = 0; u < UNITS; ++u) if (base + u * 32 * UNIT < int(a.cols) + shift) store_at<ACCESS>(row.h, first - shift + u * 32 * UNIT, int(a.cols), values_raw(v[u], T()));
   }
   const float2 r = rsqrt_pair(row_sum<BLOCK_ROW>(s) * a.inv_cols + double(a.eps));
 #pragma unroll
   for (int u = 0; u < UNITS; ++u) {
-    if (first - lane * UNIT + u * 32 * UNIT >= end) break;         // nothing of the row in this warp's unit u
+    if (base + u * 32 * UNIT >= end) break;         // nothing of the row in this warp's unit u
     if (MOVE) {
       float h[UNIT];
       unshift(v[u], v[u + 1], shift, h);
@@ -289,9 +348,9 @@ __global__ void __launch_bounds__(512) rms_norm_long_kernel(const NormArgs a) {
 // warps instead (one row of 4096: 4.3 us with 4 warps, see the launch below for the figure with 16).
 template <typename T, int OUT, bool ALIGNED>
 static void launch_norm(const NormArgs& a, cudaStream_t st) {
-  constexpr RowAccess ACCESS = ALIGNED ? WHOLE : SHIFTED;
+  constexpr RowAccess ACCESS = !ALIGNED ? SHIFTED : sizeof(T) == 4 ? SPLIT : WHOLE;
   const unsigned rows = unsigned(a.rows);
-  const int64_t units = ALIGNED ? padded(a.cols) / UNIT : std::max<int64_t>(padded(a.cols) / UNIT, (a.cols + 2 * (UNIT - 1)) / UNIT);
+  const int64_t units = ALIGNED ? ceil_div<int64_t>(a.cols, 32 * UNIT) * 32 : std::max<int64_t>(padded(a.cols) / UNIT, (a.cols + 2 * (UNIT - 1)) / UNIT);
   const bool few = a.rows < 2 * sm_count();
   if (units > MOST_WARPS * 32 * 4) {
     rms_norm_long_kernel<T, OUT, ALIGNED ? WHOLE : ANY><<<rows, 512, 0, st>>>(a);
@@ -303,6 +362,8 @@ static void launch_norm(const NormArgs& a, cudaStream_t st) {
     rms_norm_kernel<T, OUT, 2, ACCESS, false><<<(rows + WARP_ROWS - 1) / WARP_ROWS, WARP_ROWS * 32, 0, st>>>(a);
   } else if (units <= 128) {
     rms_norm_kernel<T, OUT, 4, ACCESS, false><<<(rows + WARP_ROWS - 1) / WARP_ROWS, WARP_ROWS * 32, 0, st>>>(a);
+  } else if (sizeof(T) == 2 && ALIGNED && units <= 1024) {
+    rms_norm_kernel<T, OUT, 2, ACCESS, true><<<rows, unsigned(ceil_div<int64_t>(units, 64)) * 32, 0, st>>>(a);
   } else {
     rms_norm_kernel<T, OUT, 4, ACCESS, true><<<rows, unsigned(ceil_div<int64_t>(units, 128)) * 32, 0, st>>>(a);
   }
