@@ -4,6 +4,7 @@
 // consecutive elements and a block is the four neighbouring lanes of a quad, so the block maximum costs two shuffles and
 // no shared memory; IN_FLIGHT units are loaded before the first is worked on, since one 16-byte load per thread does not
 // cover the memory's latency.  With 16-bit inputs the kernels are near the ALU pipe's rate as well as the memory's.
+#include <algorithm>
 #include <type_traits>
 #include "microscale.cuh"
 
@@ -31,6 +32,33 @@ struct Place {
     if (group >= w.groups) { group -= w.groups; ++row; }
   }
 };
+
+// Rows of whole groups have no padding: the plain matrix is one row of groups.
+template <typename T, int FORMAT>
+__global__ void __launch_bounds__(THREADS) quantize_groups_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+                                                                  int64_t total, int64_t step) {
+  const int lane16 = threadIdx.x & 15;
+  int64_t index = (int64_t(blockIdx.x) * THREADS + threadIdx.x) >> 4;
+  for (; index + (IN_FLIGHT - 1) * step < (total & ~int64_t(1)); index += IN_FLIGHT * step) {        // both half-warps, all units
+    Raw<T> raw[IN_FLIGHT];
+    const T* at = x + (index * GROUP + lane16 * UNIT);
+#pragma unroll
+    for (int u = 0; u < IN_FLIGHT; ++u) raw[u] = load_raw<true>(at + u * step * GROUP, 0, NO_END, Span());
+    const int64_t unit = index * (GROUP / UNIT) + lane16;
+#pragma unroll
+    for (int u = 0; u < IN_FLIGHT; ++u) {
+      float v[UNIT];
+      raw_values(raw[u], v);
+      quantize_unit<FORMAT>(v, codes, scales, unit + u * step * (GROUP / UNIT), true);
+    }
+  }
+  while (__any_sync(0xffffffffu, index < total)) {
+    float v[UNIT];
+    raw_values(load_raw<true>(x + index * GROUP, index < total ? lane16 * UNIT : GROUP, GROUP, Span()), v);
+    quantize_unit<FORMAT>(v, codes, scales, index * (GROUP / UNIT) + lane16, index < total);
+    index += step;
+  }
+}
 
 template <typename T, int FORMAT, bool ALIGNED>
 __global__ void __launch_bounds__(THREADS) quantize_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
@@ -87,6 +115,20 @@ __global__ void __launch_bounds__(THREADS) dequantize_kernel(const uint8_t* __re
   }
 }
 
+// e2m1 codes -> e4m3 bytes of the same values, where there is no padding: 16 codes of 8 bytes at a time
+__global__ void __launch_bounds__(THREADS) elements_groups_kernel(const uint2* __restrict__ codes, uint4* __restrict__ y, int64_t total) {
+  const int64_t step = int64_t(gridDim.x) * THREADS;
+  for (int64_t i = int64_t(blockIdx.x) * THREADS + threadIdx.x; i < total; i += IN_FLIGHT * step) {
+    uint2 q[IN_FLIGHT];
+#pragma unroll
+    for (int u = 0; u < IN_FLIGHT; ++u) if (i + u * step < total) q[u] = __ldg(codes + i + u * step);
+#pragma unroll
+    for (int u = 0; u < IN_FLIGHT; ++u)
+      if (i + u * step < total)
+        y[i + u * step] = make_uint4(e2m1x4_to_e4m3(q[u].x), e2m1x4_to_e4m3(q[u].x >> 16), e2m1x4_to_e4m3(q[u].y), e2m1x4_to_e4m3(q[u].y >> 16));
+  }
+}
+
 // e2m1 codes -> e4m3 bytes of the same values, without the padding
 template <bool ALIGNED>
 __global__ void __launch_bounds__(THREADS) elements_kernel(const uint8_t* __restrict__ codes, uint8_t* __restrict__ y, int cols, Walk w) {
@@ -127,7 +169,8 @@ static void launch_quantize(const void* x, void* codes, uint8_t* scales, int64_t
   const T* in = static_cast<const T*>(x);
   const Span span = {static_cast<const uint8_t*>(x), reinterpret_cast<const uint8_t*>(in + rows * cols)};
   uint8_t* out = static_cast<uint8_t*>(codes);
-  if (aligned16(x) && (cols * sizeof(T)) % 16 == 0) quantize_kernel<T, FORMAT, true><<<grid, THREADS, 0, st>>>(in, out, scales, int(cols), span, w);
+  if (aligned16(x) && cols % GROUP == 0) quantize_groups_kernel<T, FORMAT><<<grid, THREADS, 0, st>>>(in, out, scales, w.total, w.step);
+  else if (aligned16(x) && (cols * sizeof(T)) % 16 == 0) quantize_kernel<T, FORMAT, true><<<grid, THREADS, 0, st>>>(in, out, scales, int(cols), span, w);
   else quantize_kernel<T, FORMAT, false><<<grid, THREADS, 0, st>>>(in, out, scales, int(cols), span, w);
 }
 
@@ -188,7 +231,11 @@ extern "C" int nes_mx_elements(const void* codes, uint8_t* y, int64_t rows, int6
   unsigned grid;
   const Walk w = plan(rows, cols, &grid);
   const uint8_t* in = static_cast<const uint8_t*>(codes);
-  if ((reinterpret_cast<uintptr_t>(y) & 7u) == 0 && cols % UNIT == 0) elements_kernel<true><<<grid, THREADS, 0, as_stream(stream)>>>(in, y, int(cols), w);
+  if (aligned16(y) && cols % GROUP == 0) {
+    const int64_t total = rows * cols / 16;
+    const int64_t blocks = std::min<int64_t>(ceil_div<int64_t>(total, THREADS), int64_t(sm_count()) * 8);
+    elements_groups_kernel<<<unsigned(blocks), THREADS, 0, as_stream(stream)>>>(static_cast<const uint2*>(codes), reinterpret_cast<uint4*>(y), total);
+  } else if ((reinterpret_cast<uintptr_t>(y) & 7u) == 0 && cols % UNIT == 0) elements_kernel<true><<<grid, THREADS, 0, as_stream(stream)>>>(in, y, int(cols), w);
   else elements_kernel<false><<<grid, THREADS, 0, as_stream(stream)>>>(in, y, int(cols), w);
   return check_launch("mx_elements");
 }

@@ -68,6 +68,11 @@ __device__ __forceinline__ uint32_t float_to_pair(float a, float b, __half) {
 // the L1 cache), and put back by shifting it against the neighbouring lane's unit into aligned words; element accesses
 // remain at the ends of a run of lanes only.
 
+// NO_END in the place of `cols`: the caller knows that the unit lies inside the row.
+
+constexpr int NO_END = 0x7fffffff;
+__device__ __forceinline__ bool inside(int c, int cols) { return cols == NO_END || c < cols; }
+
 template <typename T> struct Raw { uint32_t w[UNIT * sizeof(T) / 4]; };
 struct Span { const uint8_t *begin, *end; };                      // of a whole tensor
 
@@ -93,24 +98,24 @@ __device__ __forceinline__ Raw<T> load_raw(const T* row, int c, int cols, const 
   Raw<T> r;
 #pragma unroll
   for (int i = 0; i < NW; ++i) r.w[i] = 0u;
-  if (c >= cols) return r;
+  if (!inside(c, cols)) return r;
   const uint8_t* at = reinterpret_cast<const uint8_t*>(row + c);
   if (ALIGNED) {
 #pragma unroll
     for (int i = 0; i < NW; i += 4) {
-      if (i && c + 4 >= cols) break;                              // an fp32 unit may lie half inside
+      if (i && !inside(c + 4, cols)) break;                       // an fp32 unit may lie half inside
       const uint4 v = __ldg(reinterpret_cast<const uint4*>(at) + i / 4);
       r.w[i] = v.x; r.w[i + 1] = v.y; r.w[i + 2] = v.z; r.w[i + 3] = v.w;
     }
     return r;
   }
   const uint32_t shift = uint32_t(reinterpret_cast<uintptr_t>(at)) & 15u;
-  const bool inside = at - 16 >= span.begin && at + 4 * NW + 16 <= span.end;
+  const bool interior = at - 16 >= span.begin && at + 4 * NW + 16 <= span.end;
   uint32_t e[NW + 4];
 #pragma unroll
   for (int i = 0; i < NW + 4; i += 4) {
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (i < NW || shift) v = inside ? __ldg(reinterpret_cast<const uint4*>(at - shift + 4 * i)) : load_word<T>(span, at - shift + 4 * i);
+    if (i < NW || shift) v = interior ? __ldg(reinterpret_cast<const uint4*>(at - shift + 4 * i)) : load_word<T>(span, at - shift + 4 * i);
     e[i] = v.x; e[i + 1] = v.y; e[i + 2] = v.z; e[i + 3] = v.w;
   }
   const bool two = shift & 8u, one = shift & 4u;
@@ -174,13 +179,13 @@ __device__ __forceinline__ void store_raw(T* row, int c, int cols, const Raw<T>&
   constexpr int NW = UNIT * sizeof(T) / 4, FRAME = NW >= 4 ? 16 : 4 * NW;      // bytes of an aligned store
   uint8_t* at = reinterpret_cast<uint8_t*>(row + c);
   if (ALIGNED) {
-    if (c >= cols) return;
+    if (!inside(c, cols)) return;
     if (NW == 2) {
       *reinterpret_cast<uint2*>(at) = make_uint2(r.w[0], r.w[1]);
     } else {
 #pragma unroll
       for (int i = 0; i < NW; i += 4) {
-        if (i && c + 4 >= cols) break;
+        if (i && !inside(c + 4, cols)) break;
         reinterpret_cast<uint4*>(at)[i / 4] = make_uint4(r.w[i], r.w[i + 1], r.w[i + 2], r.w[i + 3]);
       }
     }

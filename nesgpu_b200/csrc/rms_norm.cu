@@ -120,7 +120,11 @@ __device__ __forceinline__ void store_boundary(T* row, int c, int cols, const Ra
 
 // SPLIT: a unit is two runs of four columns, 128 apart, so that a warp's 16-byte accesses lie next to one another (fp32 rows in
 // units of eight consecutive columns reach every 32-byte sector twice, half of it each time, and so do their gains).
-enum RowAccess { WHOLE, SPLIT, SHIFTED, ANY };   // ANY: the looping kernel's, units from column 8 i on wherever they lie
+// FULL, SPLIT_FULL: WHOLE and SPLIT where every unit of the block lies inside the row, without checks and zeros for what does not.
+// ANY: the looping kernel's, units from column 8 i on wherever they lie.
+enum RowAccess { WHOLE, FULL, SPLIT, SPLIT_FULL, SHIFTED, ANY };
+__host__ __device__ constexpr bool is_split(RowAccess a) { return a == SPLIT || a == SPLIT_FULL; }
+__host__ __device__ constexpr bool is_full(RowAccess a) { return a == FULL || a == SPLIT_FULL; }
 
 constexpr int HALF_APART = 128;
 __device__ __forceinline__ Raw<float> load_split(const float* row, int c, int cols) {
@@ -128,7 +132,7 @@ __device__ __forceinline__ Raw<float> load_split(const float* row, int c, int co
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (c + h * HALF_APART < cols) v = __ldg(reinterpret_cast<const uint4*>(row + c + h * HALF_APART));
+    if (inside(c + h * HALF_APART, cols)) v = __ldg(reinterpret_cast<const uint4*>(row + c + h * HALF_APART));
     r.w[4 * h] = v.x; r.w[4 * h + 1] = v.y; r.w[4 * h + 2] = v.z; r.w[4 * h + 3] = v.w;
   }
   return r;
@@ -136,23 +140,23 @@ __device__ __forceinline__ Raw<float> load_split(const float* row, int c, int co
 __device__ __forceinline__ void store_split(float* row, int c, int cols, const Raw<float>& r) {
 #pragma unroll
   for (int h = 0; h < 2; ++h)
-    if (c + h * HALF_APART < cols) *reinterpret_cast<uint4*>(row + c + h * HALF_APART) = make_uint4(r.w[4 * h], r.w[4 * h + 1], r.w[4 * h + 2], r.w[4 * h + 3]);
+    if (inside(c + h * HALF_APART, cols)) *reinterpret_cast<uint4*>(row + c + h * HALF_APART) = make_uint4(r.w[4 * h], r.w[4 * h + 1], r.w[4 * h + 2], r.w[4 * h + 3]);
 }
 // Quantises a split unit: its halves belong to two blocks, each held by eight neighbouring lanes; columns of the padding are zero.
-template <int FORMAT>
+template <int FORMAT, bool ALL>
 __device__ __forceinline__ void quantize_split(float (&v)[UNIT], uint8_t* codes_row, uint8_t* scales_row, int c, int cols) {
   const int end = int(padded(cols));
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int at = c + h * HALF_APART;
     float* q = v + 4 * h;
-    if (at >= cols) q[0] = q[1] = q[2] = q[3] = 0.f;             // fp32 rows end on a multiple of four columns here
+    if (!ALL && at >= cols) q[0] = q[1] = q[2] = q[3] = 0.f;             // fp32 rows end on a multiple of four columns here
     uint32_t m = __float_as_uint(max_magnitude(max_magnitude(q[0], q[1], q[2]), q[3], q[3])) & 0x7fffffffu;
 #pragma unroll
     for (int o = 1; o < 8; o <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
     const uint32_t code = scale_code<FORMAT>(m);
     const float inv = inverse_scale(code);
-    if (at >= end) continue;
+    if (!ALL && at >= end) continue;
     if (FORMAT == NES_MXFP4) {
       const float e[UNIT] = {q[0] * inv, q[1] * inv, q[2] * inv, q[3] * inv, 0.f, 0.f, 0.f, 0.f};
       *reinterpret_cast<uint16_t*>(codes_row + at / 2) = uint16_t(code == 255u ? 0u : pack_e2m1x8(e));
@@ -166,21 +170,21 @@ __device__ __forceinline__ void quantize_split(float (&v)[UNIT], uint8_t* codes_
 
 template <RowAccess ACCESS, typename T>
 __device__ __forceinline__ Raw<T> load_at(const T* row, int c, int cols, const Span& span) {
-  if constexpr (ACCESS == SPLIT) return load_split(row, c, cols);
+  if constexpr (is_split(ACCESS)) return load_split(row, c, ACCESS == SPLIT_FULL ? NO_END : cols);
   else if constexpr (ACCESS == SHIFTED) return load_boundary(row, c, cols, span);
-  else return load_raw<ACCESS == WHOLE>(row, c, cols, span);
+  else return load_raw<ACCESS != ANY>(row, c, ACCESS == FULL ? NO_END : cols, span);
 }
 template <RowAccess ACCESS, typename T>
 __device__ __forceinline__ void store_at(T* row, int c, int cols, const Raw<T>& r) {
-  if constexpr (ACCESS == SPLIT) store_split(row, c, cols, r);
+  if constexpr (is_split(ACCESS)) store_split(row, c, ACCESS == SPLIT_FULL ? NO_END : cols, r);
   else if constexpr (ACCESS == SHIFTED) store_boundary(row, c, cols, r);
-  else store_raw<ACCESS == WHOLE, 32>(row, c, cols, r);
+  else store_raw<ACCESS != ANY, 32>(row, c, ACCESS == FULL ? NO_END : cols, r);
 }
 // gains and noise of a unit's columns, fp32 whatever the rows' type; a quantised output's shifted units have been moved by then
 template <RowAccess ACCESS, bool MOVED>
 __device__ __forceinline__ void load_gain(const float* row, int c, int cols, const Span& span, bool aligned_row, float (&g)[UNIT]) {
-  if constexpr (ACCESS == SPLIT) raw_values(load_split(row, c, cols), g);
-  else if constexpr (ACCESS == WHOLE) raw_values(load_raw<true>(row, c, cols, span), g);
+  if constexpr (is_split(ACCESS)) raw_values(load_split(row, c, ACCESS == SPLIT_FULL ? NO_END : cols), g);
+  else if constexpr (ACCESS == WHOLE || ACCESS == FULL) raw_values(load_raw<true>(row, c, ACCESS == FULL ? NO_END : cols, span), g);
   else if (MOVED && aligned_row) raw_values(load_boundary(row, c, cols, span), g);
   else raw_values(load_raw<false>(row, c, cols, span), g);
 }
@@ -229,15 +233,15 @@ __device__ __forceinline__ void emit(const NormArgs& a, const Row<T>& row, int64
   constexpr int FORMAT = OUT == 0 ? NES_MXFP8 : OUT;
   uint8_t* codes = static_cast<uint8_t*>(a.y) + index * code_pitch(cols, FORMAT);
   uint8_t* scales = a.scales + index * scale_pitch(cols);
-  if (ACCESS == SPLIT) {
-    quantize_split<FORMAT>(y, codes, scales, c, cols);
+  if (is_split(ACCESS)) {
+    quantize_split<FORMAT, ACCESS == SPLIT_FULL>(y, codes, scales, c, cols);
     return;
   }
-  if (c + UNIT > cols) {                          // columns of the padding are zero whatever the row's scale (0 * inf is not)
+  if (ACCESS != FULL && c + UNIT > cols) {                          // columns of the padding are zero whatever the row's scale (0 * inf is not)
 #pragma unroll
     for (int i = 0; i < UNIT; ++i) if (c + i >= cols) y[i] = 0.f;
   }
-  quantize_unit<FORMAT>(y, codes, scales, c / UNIT, c < int(padded(cols)));
+  quantize_unit<FORMAT>(y, codes, scales, c / UNIT, ACCESS == FULL || c < int(padded(cols)));
 }
 
 // h of columns 8 i ... from units that begin `shift` elements earlier: the end of the unit `from` and the start of the next
@@ -292,7 +296,7 @@ __global__ void __launch_bounds__(BLOCK_ROW ? MOST_WARPS * 32 : WARP_ROWS * 32) 
   const int64_t index = BLOCK_ROW ? int64_t(blockIdx.x) : int64_t(blockIdx.x) * WARP_ROWS + warp;
   if (index >= a.rows) return;
   const Row<T> row(a, index);
-  const int base = BLOCK_ROW ? warp * UNITS * 32 * UNIT : 0, first = base + lane * (ACCESS == SPLIT ? 4 : UNIT);
+  const int base = BLOCK_ROW ? warp * UNITS * 32 * UNIT : 0, first = base + lane * (is_split(ACCESS) ? 4 : UNIT);
   const int shift = ACCESS == SHIFTED ? row.shift : 0;
   const int end = OUT != 0 ? int(padded(a.cols)) : int(a.cols) + shift;
   float v[UNITS + 1][UNIT];
@@ -305,12 +309,12 @@ __global__ void __launch_bounds__(BLOCK_ROW ? MOST_WARPS * 32 : WARP_ROWS * 32) 
   for (int u = 0; u < UNITS; ++u) s += square_sum(v[u]);
   if (row.h) {
 #pragma unroll
-    for (int u = 0; u < UNITS; ++u) if (base + u * 32 * UNIT < int(a.cols) + shift) store_at<ACCESS>(row.h, first - shift + u * 32 * UNIT, int(a.cols), values_raw(v[u], T()));
+    for (int u = 0; u < UNITS; ++u) if (is_full(ACCESS) || base + u * 32 * UNIT < int(a.cols) + shift) store_at<ACCESS>(row.h, first - shift + u * 32 * UNIT, int(a.cols), values_raw(v[u], T()));
   }
   const float2 r = rsqrt_pair(row_sum<BLOCK_ROW>(s) * a.inv_cols + double(a.eps));
 #pragma unroll
   for (int u = 0; u < UNITS; ++u) {
-    if (base + u * 32 * UNIT >= end) break;         // nothing of the row in this warp's unit u
+    if (!is_full(ACCESS) && base + u * 32 * UNIT >= end) break;         // nothing of the row in this warp's unit u
     if (MOVE) {
       float h[UNIT];
       unshift(v[u], v[u + 1], shift, h);
@@ -345,28 +349,29 @@ __global__ void __launch_bounds__(512) rms_norm_long_kernel(const NormArgs a) {
 }
 
 // Four units per lane keep the most loads in flight where there are rows enough for all SMs; a few rows are spread over more
-// warps instead (one row of 4096: 4.3 us with 4 warps, see the launch below for the figure with 16).
+// warps instead (one row of 4096 bf16: 4.3 us with 4 warps, 3.3 us with 16).
+template <typename T, int OUT, int UNITS, bool ALIGNED, bool BLOCK_ROW>
+static void launch_rows(const NormArgs& a, int64_t units, cudaStream_t st) {
+  constexpr int OF_WARP = UNITS * 32;              // units that a warp holds
+  constexpr RowAccess GUARDED = !ALIGNED ? SHIFTED : sizeof(T) == 4 ? SPLIT : WHOLE, PLAIN = sizeof(T) == 4 ? SPLIT_FULL : FULL;
+  const unsigned grid = unsigned(BLOCK_ROW ? a.rows : ceil_div<int64_t>(a.rows, WARP_ROWS));
+  const unsigned threads = unsigned(BLOCK_ROW ? ceil_div<int64_t>(units, OF_WARP) : WARP_ROWS) * 32;
+  if (ALIGNED && (BLOCK_ROW ? a.cols % (OF_WARP * UNIT) == 0 : a.cols == OF_WARP * UNIT))
+    rms_norm_kernel<T, OUT, UNITS, PLAIN, BLOCK_ROW><<<grid, threads, 0, st>>>(a);
+  else
+    rms_norm_kernel<T, OUT, UNITS, GUARDED, BLOCK_ROW><<<grid, threads, 0, st>>>(a);
+}
+
 template <typename T, int OUT, bool ALIGNED>
 static void launch_norm(const NormArgs& a, cudaStream_t st) {
-  constexpr RowAccess ACCESS = !ALIGNED ? SHIFTED : sizeof(T) == 4 ? SPLIT : WHOLE;
-  const unsigned rows = unsigned(a.rows);
   const int64_t units = ALIGNED ? ceil_div<int64_t>(a.cols, 32 * UNIT) * 32 : std::max<int64_t>(padded(a.cols) / UNIT, (a.cols + 2 * (UNIT - 1)) / UNIT);
   const bool few = a.rows < 2 * sm_count();
-  if (units > MOST_WARPS * 32 * 4) {
-    rms_norm_long_kernel<T, OUT, ALIGNED ? WHOLE : ANY><<<rows, 512, 0, st>>>(a);
-  } else if (units <= 32) {
-    rms_norm_kernel<T, OUT, 1, ACCESS, false><<<(rows + WARP_ROWS - 1) / WARP_ROWS, WARP_ROWS * 32, 0, st>>>(a);
-  } else if (few && units <= MOST_WARPS * 32) {
-    rms_norm_kernel<T, OUT, 1, ACCESS, true><<<rows, unsigned(ceil_div<int64_t>(units, 32)) * 32, 0, st>>>(a);
-  } else if (units <= 64) {
-    rms_norm_kernel<T, OUT, 2, ACCESS, false><<<(rows + WARP_ROWS - 1) / WARP_ROWS, WARP_ROWS * 32, 0, st>>>(a);
-  } else if (units <= 128) {
-    rms_norm_kernel<T, OUT, 4, ACCESS, false><<<(rows + WARP_ROWS - 1) / WARP_ROWS, WARP_ROWS * 32, 0, st>>>(a);
-  } else if (sizeof(T) == 2 && ALIGNED && units <= 1024) {
-    rms_norm_kernel<T, OUT, 2, ACCESS, true><<<rows, unsigned(ceil_div<int64_t>(units, 64)) * 32, 0, st>>>(a);
-  } else {
-    rms_norm_kernel<T, OUT, 4, ACCESS, true><<<rows, unsigned(ceil_div<int64_t>(units, 128)) * 32, 0, st>>>(a);
-  }
+  if (units > MOST_WARPS * 32 * 4) rms_norm_long_kernel<T, OUT, ALIGNED ? WHOLE : ANY><<<unsigned(a.rows), 512, 0, st>>>(a);
+  else if (units <= 32) launch_rows<T, OUT, 1, ALIGNED, false>(a, units, st);
+  else if (few && units <= MOST_WARPS * 32) launch_rows<T, OUT, 1, ALIGNED, true>(a, units, st);
+  else if (units <= 64) launch_rows<T, OUT, 2, ALIGNED, false>(a, units, st);
+  else if (units <= 128) launch_rows<T, OUT, 4, ALIGNED, false>(a, units, st);
+  else launch_rows<T, OUT, 4, ALIGNED, true>(a, units, st);
 }
 
 template <typename T, int OUT>
