@@ -37,6 +37,7 @@ struct Place {
 template <typename T, int FORMAT>
 __global__ void __launch_bounds__(THREADS) quantize_groups_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                                                                   int64_t total, int64_t step) {
+  let_dependents_start();
   const int lane16 = threadIdx.x & 15;
   int64_t index = (int64_t(blockIdx.x) * THREADS + threadIdx.x) >> 4;
   for (; index + (IN_FLIGHT - 1) * step < (total & ~int64_t(1)); index += IN_FLIGHT * step) {        // both half-warps, all units
@@ -63,6 +64,7 @@ __global__ void __launch_bounds__(THREADS) quantize_groups_kernel(const T* __res
 template <typename T, int FORMAT, bool ALIGNED>
 __global__ void __launch_bounds__(THREADS) quantize_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
                                                            int cols, Span span, Walk w) {
+  let_dependents_start();
   Place at(w);
   const int lane16 = threadIdx.x & 15;
   // the two half-warps of a warp may differ by one trip: both run until the first one is past the end

@@ -243,6 +243,11 @@ __device__ __forceinline__ uint32_t scale_code(uint32_t m) {
   return m >= 0x7f800000u ? 255u : uint32_t(max(int(m >> 23) - EMAX, 0));
 }
 
+// A product that reads what a quantising kernel before it writes may be started while that kernel still runs: the first lets it
+// (once all its blocks have begun), the second waits until the kernel before has ended and its writes can be seen.
+__device__ __forceinline__ void let_dependents_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_kernel_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // 2^-e for a scale code below 255 (at most 253: a normal number); 0 for 255
 __device__ __forceinline__ float inverse_scale(uint32_t code) { return __uint_as_float(code == 255u ? 0u : (254u - code) << 23); }
 

@@ -40,6 +40,7 @@ struct Product {
   int y_dtype, vec_scales;
   const void* x;                             // plain activations of a product that quantises them itself
   int whole_rows;                            // their rows are whole, aligned 16-byte pieces
+  bool overlap;                              // the kernel before quantises the activations and lets this one start early
 };
 struct ProductMaps { CUtensorMap w, x; };
 
@@ -128,15 +129,16 @@ __device__ __forceinline__ void warp_mma_stage(uint32_t d, uint64_t a, uint64_t 
 }
 
 // 16 scale bytes of a row from 128-element group `group` on; zeros outside the matrix
+// (through the L2 cache: the activations' may have been written while this kernel ran already)
 __device__ __forceinline__ uint4 load_scale_words(const uint8_t* scales, int row, int rows, int group, int groups, bool vec) {
   uint4 v = make_uint4(0u, 0u, 0u, 0u);
   if (row >= rows) return v;
   const uint32_t* p = reinterpret_cast<const uint32_t*>(scales + int64_t(row) * groups * 4) + group;
-  if (vec) return __ldg(reinterpret_cast<const uint4*>(p));
-  v.x = __ldg(p);
-  if (group + 1 < groups) v.y = __ldg(p + 1);
-  if (group + 2 < groups) v.z = __ldg(p + 2);
-  if (group + 3 < groups) v.w = __ldg(p + 3);
+  if (vec) return __ldcg(reinterpret_cast<const uint4*>(p));
+  v.x = __ldcg(p);
+  if (group + 1 < groups) v.y = __ldcg(p + 1);
+  if (group + 2 < groups) v.z = __ldcg(p + 2);
+  if (group + 3 < groups) v.w = __ldcg(p + 3);
   return v;
 }
 
@@ -342,13 +344,21 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
     if (lane == 0) {
       // a spreading copy counts the bytes it reads, half of those it fills
       constexpr uint32_t TX = (RAW ? 0 : L::X_BYTES) + (XF == NES_MXFP8 && WF == NES_MXFP4 ? L::W_BYTES / 2 : L::W_BYTES);
-      int s = 0;
-      uint32_t ph = 0;
-      for (int kt = kt0; kt < kt1; ++kt) {
+      // first coordinate: bytes of codes, or elements of a copy that spreads 4-bit codes.  The weights of the first stages do not
+      // depend on the kernel before; the activations may.
+      const int ready = RAW ? 0 : min(int(L::STAGES), kt1 - kt0);
+      for (int i = 0; i < ready; ++i) {
+        mbar_expect_tx(&full[i], TX);
+        tma_load_2d(tiles + size_t(i) * L::STAGE, &maps.w, &full[i], (kt0 + i) * ROW_BYTES, n0);
+      }
+      wait_for_kernel_before();
+      for (int i = 0; i < ready; ++i) tma_load_2d(tiles + size_t(i) * L::STAGE + L::W_BYTES, &maps.x, &full[i], (kt0 + i) * ROW_BYTES, m0);
+      int s = ready % L::STAGES;
+      uint32_t ph = ready == L::STAGES;
+      for (int kt = kt0 + ready; kt < kt1; ++kt) {
         if (!mbar_wait(&empty[s], ph ^ 1, 1)) break;
         unsigned char* st = tiles + size_t(s) * L::STAGE;
         mbar_expect_tx(&full[s], TX);
-        // first coordinate: bytes of codes, or elements of a copy that spreads 4-bit codes
         const int c = kt * ROW_BYTES;
         tma_load_2d(st, &maps.w, &full[s], c, n0);
         if (!RAW) tma_load_2d(st + L::W_BYTES, &maps.x, &full[s], c, m0);
@@ -400,6 +410,7 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
     const uint32_t lanes = uint32_t(q * 32) << 16;
     const int t = threadIdx.x - 64, row = scale_row(t);
     uint4 wv[4], xv[4];                              // four steps in flight
+    wait_for_kernel_before();
     auto load = [&](int step, uint4& wo, uint4& xo) {
       if (step >= step1) return;
       wo = load_scale_words(p.w_scales, n0 + row, p.N, step * CHUNKS, p.groups, p.vec_scales);
@@ -623,12 +634,24 @@ mx_pair_kernel(const __grid_constant__ PairMaps maps, const Product p, int ftile
     if (lane == 0) {
       constexpr uint32_t W_TX = XF == NES_MXFP8 && WF == NES_MXFP4 ? L::W_BYTES / 2 : L::W_BYTES;   // a spreading copy counts what it reads
       const uint32_t full0 = map_rank(smem_u32(full), 0);
-      int s = 0;
-      uint32_t ph = 0;
+      // the weights of the first stages do not depend on the kernel before; the activations may
+      const int ready = pair < tiles ? min(int(L::STAGES), kts) : 0;
+      {
+        const int2 at = tile_place(pair, ftiles, ttiles);
+        const int n0 = at.x * PAIR_FEATURES + rank * FEATURES, m0 = at.y * PAIR_TOKENS + rank * (PAIR_TOKENS / 2);
+        for (int i = 0; i < ready; ++i) {
+          if (rank == 0) mbar_expect_tx(&full[i], 2 * (W_TX + L::X_BYTES));
+          tma_load_pair(stages + size_t(i) * L::STAGE, &maps.w, full0 + uint32_t(i) * 8u, i * ROW_BYTES, n0);
+        }
+        wait_for_kernel_before();
+        for (int i = 0; i < ready; ++i) tma_load_pair(stages + size_t(i) * L::STAGE + L::W_BYTES, &maps.x, full0 + uint32_t(i) * 8u, i * ROW_BYTES, m0);
+      }
+      int s = ready % L::STAGES;
+      uint32_t ph = ready == L::STAGES;
       for (int tile = pair; tile < tiles && ok; tile += pairs) {
         const int2 at = tile_place(tile, ftiles, ttiles);
         const int n0 = at.x * PAIR_FEATURES + rank * FEATURES, m0 = at.y * PAIR_TOKENS + rank * (PAIR_TOKENS / 2);
-        for (int kt = 0; kt < kts; ++kt) {
+        for (int kt = tile == pair ? ready : 0; kt < kts; ++kt) {
           ok = mbar_wait(&empty[s], ph ^ 1, 1);
           if (!ok) break;
           unsigned char* st = stages + size_t(s) * L::STAGE;
@@ -718,6 +741,7 @@ mx_pair_kernel(const __grid_constant__ PairMaps maps, const Product p, int ftile
       o[2] = load_scale_words(p.x_scales, m0 + 128 + row, p.M, step * CHUNKS, p.groups, p.vec_scales);
       if (++step == steps) { step = 0; tile += pairs; }
     };
+    wait_for_kernel_before();
 #pragma unroll
     for (int i = 0; i < 4; ++i) load(v[i]);
     const int64_t total = pair < tiles ? int64_t((tiles - 1 - pair) / pairs + 1) * steps : 0;
@@ -862,12 +886,14 @@ static int launch_product(const Product& p, const void* x, const void* w, cudaSt
   cfg.blockDim = dim3(THREADS_TC);
   cfg.dynamicSmemBytes = L::SMEM;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = splits;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = p.overlap ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, mx_product_kernel<XF, WF, TOKENS, X>, maps, p, splits);
   if (e != cudaSuccess) return fail(NES_ERR_LAUNCH, "mx_linear_fwd: %s", cudaGetErrorString(e));
   return check_launch("mx_linear_fwd");
@@ -898,7 +924,18 @@ static int launch_pair(const Product& p, const void* x, const void* w, cudaStrea
   NES_REQUIRE(tiles <= INT32_MAX / 16, NES_ERR_UNSUPPORTED, "mx_linear_fwd: too large");
   if ((rc = allow_smem<mx_pair_kernel<XF, WF>>(L::SMEM)) != NES_OK) return rc;
   const int64_t pairs = tiles < sm_count() / 2 ? tiles : sm_count() / 2;
-  mx_pair_kernel<XF, WF><<<unsigned(pairs * 2), THREADS_PAIR, L::SMEM, st>>>(maps, p, int(ftiles), int(ttiles), tma_out);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(pairs * 2));
+  cfg.blockDim = dim3(THREADS_PAIR);
+  cfg.dynamicSmemBytes = L::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = p.overlap ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, mx_pair_kernel<XF, WF>, maps, p, int(ftiles), int(ttiles), tma_out);
+  if (e != cudaSuccess) return fail(NES_ERR_LAUNCH, "mx_linear_fwd: %s", cudaGetErrorString(e));
   return check_launch("mx_linear_fwd");
 }
 
@@ -970,7 +1007,7 @@ extern "C" int nes_mx_linear_fwd(const void* x, const uint8_t* x_scales, int x_d
               "mx_linear_fwd: scales must be 4-byte aligned");
   cudaStream_t st = as_stream(stream);
   Product p;
-  p.x_scales = x_scales; p.w_scales = w_scales; p.bias = bias; p.y = y; p.x = x; p.whole_rows = 0;
+  p.x_scales = x_scales; p.w_scales = w_scales; p.bias = bias; p.y = y; p.x = x; p.whole_rows = 0; p.overlap = false;
   p.M = int(M); p.N = int(N); p.K = int(K); p.groups = int(padded(K) / GROUP); p.y_dtype = y_dtype;
   p.vec_scales = p.groups % CHUNKS == 0 && aligned16(x_scales) && aligned16(w_scales);
   if (!x_scales && quantises_itself(M, N, K)) {
@@ -989,6 +1026,7 @@ extern "C" int nes_mx_linear_fwd(const void* x, const uint8_t* x_scales, int x_d
     if (rc != NES_OK) return rc;
     x = codes;
     p.x_scales = scales;
+    p.overlap = true;
   }
   if (x_format == NES_MXFP4) return launch_tokens<NES_MXFP4, NES_MXFP4>(p, x, w_codes, st);
   if (w_format == NES_MXFP4) return launch_tokens<NES_MXFP8, NES_MXFP4>(p, x, w_codes, st);
