@@ -46,13 +46,17 @@ struct ProductMaps { CUtensorMap w, x; };
 
 constexpr int RAW_STEPS = 8;                 // steps of K whose quantised activations a CTA keeps
 
+// PUSH: partial results go straight to the CTA that adds them up, which has room for them beside its stages (one barrier of the
+// cluster and local reads: 1 token of 4096x4096 8.0 -> 7.2 us).  Otherwise they lie in the stages until they are fetched: of
+// 128 tokens the room costs two of six stages, which pays from four CTAs to a tile on (128 tokens, 4096x1024: 10.3 -> 7.7 us;
+// 1024x1024 in halves: 8.2 -> 9.0 us).
 // RAW: the activations of all the CTA's stages lie behind the stages, which hold weights only; so do their scales
-template <int TOKENS, bool RAW, int STAGES_PER_STEP>
+template <int TOKENS, bool RAW, int STAGES_PER_STEP, bool PUSH>
 struct Layout {
   static constexpr int W_BYTES = FEATURES * ROW_BYTES;
   static constexpr int X_BYTES = TOKENS * ROW_BYTES;
   static constexpr int STAGE = W_BYTES + (RAW ? 0 : X_BYTES);
-  static constexpr int STAGES = TOKENS >= 128 ? 6 : 8;
+  static constexpr int STAGES = TOKENS >= 128 ? (PUSH ? 4 : 6) : TOKENS >= 64 ? 7 : 8;
   static constexpr int X_COLS = 4;                                         // scale columns of x per 128 elements
   static constexpr int SCALE_COLS = CHUNKS * (4 + X_COLS);                 // one buffer
   static constexpr int SCALE_BASE = TOKENS < 32 ? 32 : TOKENS;
@@ -62,7 +66,8 @@ struct Layout {
   static constexpr int SCALES = (RAW ? 1 : 2) * STEP_SCALES;               // a buffer in shared memory: w, then x
   static constexpr int RAW_X = RAW ? RAW_STEPS * STAGES_PER_STEP * X_BYTES : 0;
   static constexpr int RAW_SCALES = RAW ? RAW_STEPS * STEP_SCALES : 0;
-  static constexpr size_t SMEM = 1024 + size_t(STAGES) * STAGE + RAW_X + RAW_SCALES + 2 * SCALES + (2 * STAGES + 6) * sizeof(uint64_t) + 16;
+  static constexpr int PARTS = PUSH ? TOKENS * FEATURES * 4 : 0;
+  static constexpr size_t SMEM = 1024 + size_t(STAGES) * STAGE + RAW_X + RAW_SCALES + 2 * SCALES + PARTS + (2 * STAGES + 6) * sizeof(uint64_t) + 16;
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
@@ -187,6 +192,8 @@ __device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("m
 __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 __device__ __forceinline__ uint32_t map_rank(uint32_t addr, uint32_t rank) {
   uint32_t remote;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
@@ -196,6 +203,20 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t remote) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
   return v;
+}
+__device__ __forceinline__ void st_cluster(uint32_t remote, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(remote), "f"(v) : "memory");
+}
+
+__device__ __forceinline__ float4 four_biases(const Product& p, int n, int left) {
+  float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (p.bias) {
+    b.x = __ldg(p.bias + n);
+    if (left > 1) b.y = __ldg(p.bias + n + 1);
+    if (left > 2) b.z = __ldg(p.bias + n + 2);
+    if (left > 3) b.w = __ldg(p.bias + n + 3);
+  }
+  return b;
 }
 
 // Four neighbouring features of one token; `left` of them exist.
@@ -219,16 +240,10 @@ __device__ __forceinline__ void store_four(T* y, const float4& v, int left, bool
 // Adds the partial tiles ([token][feature] fp32 at the same shared-memory address of every CTA of the cluster) in rank
 // order and stores this CTA's share of the tokens: token = rank + splits * i, four features per lane.
 template <typename T>
-__device__ __forceinline__ void join_tiles(const Product& p, uint32_t part, int n0, int m0, int tokens, int rank, int splits, int warp, int lane) {
+__device__ __forceinline__ void pull_tiles(const Product& p, uint32_t part, int n0, int m0, int tokens, int rank, int splits, int warp, int lane) {
   const int n = n0 + lane * 4, left = p.N - n;
   if (left <= 0) return;
-  float4 bias = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (p.bias) {
-    bias.x = __ldg(p.bias + n);
-    if (left > 1) bias.y = __ldg(p.bias + n + 1);
-    if (left > 2) bias.z = __ldg(p.bias + n + 2);
-    if (left > 3) bias.w = __ldg(p.bias + n + 3);
-  }
+  const float4 bias = four_biases(p, n, left);
   uint32_t source[8];
 #pragma unroll
   for (int r = 0; r < 8; ++r) source[r] = r < splits ? map_rank(part, r) : 0u;
@@ -257,6 +272,33 @@ __device__ __forceinline__ void join_tiles(const Product& p, uint32_t part, int 
       store_four(static_cast<T*>(p.y) + int64_t(m0 + t) * p.N + n, sum[i], left, vec);
     }
   }
+}
+
+// Adds the partial results of this CTA's share of the tokens (token = rank + splits * i; [source rank][i][feature] fp32 in shared
+// memory) in rank order and stores them, four features per lane.
+template <typename T>
+__device__ __forceinline__ void join_parts(const Product& p, const float* parts, int n0, int m0, int tokens, int share, int rank, int splits,
+                                           int warp, int lane) {
+  const int n = n0 + lane * 4, left = p.N - n;
+  if (left <= 0) return;
+  const float4 bias = four_biases(p, n, left);
+  const bool vec = p.N % 4 == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15u) == 0;
+  for (int i = warp; rank + i * splits < tokens; i += 4) {
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int r = 0; r < splits; ++r) {
+      const float4 v = *reinterpret_cast<const float4*>(parts + (r * share + i) * FEATURES + lane * 4);
+      sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+    }
+    sum.x += bias.x; sum.y += bias.y; sum.z += bias.z; sum.w += bias.w;
+    store_four(static_cast<T*>(p.y) + int64_t(m0 + rank + i * splits) * p.N + n, sum, left, vec);
+  }
+}
+
+template <typename T, bool PUSH, int TOKENS>
+__device__ __forceinline__ void join(const Product& p, const float* parts, const unsigned char* tiles, int n0, int m0, int tokens, int rank, int splits,
+                                     int warp, int lane) {
+  if (PUSH) join_parts<T>(p, parts, n0, m0, tokens, TOKENS / splits, rank, splits, warp, lane);
+  else pull_tiles<T>(p, smem_u32(tiles), n0, m0, tokens, rank, splits, warp, lane);
 }
 
 // Quantises columns c0 ... c0 + width - 1 of all (at most 16) tokens with 128 threads: codes into the 128-byte-swizzled rows of
@@ -298,12 +340,12 @@ __device__ __forceinline__ void quantize_tokens(const Product& p, int c0, int wi
 }
 
 // X: void for activations that are quantised already, else the type of plain ones
-template <int XF, int WF, int TOKENS, typename X>
+template <int XF, int WF, int TOKENS, typename X, bool PUSH>
 __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_constant__ ProductMaps maps, const Product p, int splits) {
   constexpr bool RAW = !std::is_same<X, void>::value;
   constexpr int STAGE_GROUPS = XF == NES_MXFP4 ? 2 : 1;                  // 128-element groups per stage
   constexpr int STAGES_PER_STEP = CHUNKS / STAGE_GROUPS;
-  using L = Layout<TOKENS, RAW, STAGES_PER_STEP>;
+  using L = Layout<TOKENS, RAW, STAGES_PER_STEP, PUSH>;
   extern __shared__ unsigned char dyn_raw[];
   const unsigned int timeouts_at_start = timeouts_so_far();
   const uint32_t raw = smem_u32(dyn_raw);
@@ -311,7 +353,8 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
   unsigned char* raw_tiles = tiles + size_t(L::STAGES) * L::STAGE;
   unsigned char* raw_scales = raw_tiles + L::RAW_X;
   unsigned char* scale_tiles = raw_scales + L::RAW_SCALES;
-  uint64_t* full = reinterpret_cast<uint64_t*>(scale_tiles + 2 * L::SCALES);
+  float* parts = reinterpret_cast<float*>(scale_tiles + 2 * L::SCALES);
+  uint64_t* full = reinterpret_cast<uint64_t*>(reinterpret_cast<unsigned char*>(parts) + L::PARTS);
   uint64_t* empty = full + L::STAGES;
   uint64_t* sf_full = empty + L::STAGES;
   uint64_t* sf_empty = sf_full + 2;
@@ -339,6 +382,7 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   bool ok = true;
+  if (PUSH && splits > 1) cluster_arrive();              // waited for before the first store into another CTA's shared memory
 
   if (warp == 0) {
     if (lane == 0) {
@@ -366,6 +410,7 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
       }
     }
     __syncwarp();
+    if (PUSH && splits > 1) cluster_wait();
   } else if (warp == 1) {
     constexpr uint32_t idesc = idesc_scaled<XF, WF>(FEATURES, TOKENS);
     const uint64_t desc0 = smem_desc_sw128(smem_u32(tiles));
@@ -405,6 +450,7 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
       }
     }
     warp_mma_commit(accum);
+    if (PUSH && splits > 1) cluster_wait();
   } else {
     const int q = warp & 3;
     const uint32_t lanes = uint32_t(q * 32) << 16;
@@ -416,13 +462,13 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
       wo = load_scale_words(p.w_scales, n0 + row, p.N, step * CHUNKS, p.groups, p.vec_scales);
       if (!RAW) xo = load_scale_words(p.x_scales, row < TOKENS ? m0 + row : p.M, p.M, step * CHUNKS, p.groups, p.vec_scales);
     };
+#pragma unroll
+    for (int u = 0; u < 4; ++u) load(step0 + u, wv[u], xv[u]);
     if (RAW) {
       quantize_tokens<typename std::conditional<RAW, X, float>::type, XF>(p, step0 * STEP, (step1 - step0) * STEP, raw_tiles, raw_scales, t);
       __syncwarp();
       if (lane == 0) mbar_arrive(raw_full);
     }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) load(step0 + u, wv[u], xv[u]);
     for (int step = step0; step < step1 && ok; step += 4) {
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
@@ -441,6 +487,10 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
     ok = warp_mbar_wait(accum, 0, 3) && ok;
     tc_fence_after();
     const bool good = __all_sync(0xffffffffu, ok && timeouts_so_far() == timeouts_at_start);
+    if (PUSH && splits > 1) cluster_wait();
+    // PUSH: to the CTA that adds up the token, each rank into a part of its own
+    const int share = TOKENS / splits, half = __ffs(splits) - 1;             // splits is a power of two
+    const uint32_t mine = smem_u32(parts) + uint32_t(rank * share * FEATURES + q * 32 + lane) * 4u;
     float* part = reinterpret_cast<float*>(tiles) + q * 32 + lane;           // every stage has been consumed
 #pragma unroll 1
     for (int c = 0; c < TOKENS; c += 16) {
@@ -449,19 +499,23 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
       tmem_ld16_nowait(tmem + lanes + c, r);
       tmem_ld_wait();
 #pragma unroll
-      for (int j = 0; j < 16; ++j) part[(c + j) * FEATURES] = good ? __uint_as_float(r[j]) : 0.f;
+      for (int j = 0; j < 16; ++j) {
+        const float v = good ? __uint_as_float(r[j]) : 0.f;
+        if (PUSH) st_cluster(map_rank(mine + uint32_t(((c + j) >> half) * FEATURES) * 4u, (c + j) & (splits - 1)), v);
+        else part[(c + j) * FEATURES] = v;
+      }
     }
   }
   __syncwarp();
   if (splits > 1) cluster_sync_all(); else __syncthreads();
   if (warp >= 2 && timeouts_so_far() == timeouts_at_start) {
     const int tokens = min(TOKENS, p.M - m0);
-    if (p.y_dtype == NES_F32) join_tiles<float>(p, smem_u32(tiles), n0, m0, tokens, rank, splits, warp - 2, lane);
-    else if (p.y_dtype == NES_BF16) join_tiles<__nv_bfloat16>(p, smem_u32(tiles), n0, m0, tokens, rank, splits, warp - 2, lane);
-    else join_tiles<__half>(p, smem_u32(tiles), n0, m0, tokens, rank, splits, warp - 2, lane);
+    if (p.y_dtype == NES_F32) join<float, PUSH, TOKENS>(p, parts, tiles, n0, m0, tokens, rank, splits, warp - 2, lane);
+    else if (p.y_dtype == NES_BF16) join<__nv_bfloat16, PUSH, TOKENS>(p, parts, tiles, n0, m0, tokens, rank, splits, warp - 2, lane);
+    else join<__half, PUSH, TOKENS>(p, parts, tiles, n0, m0, tokens, rank, splits, warp - 2, lane);
   }
   __syncwarp();
-  if (splits > 1) cluster_sync_all();                          // partial tiles stay until everyone has read them
+  if (!PUSH && splits > 1) cluster_sync_all();              // partial tiles stay until everyone has read them
   tc_fence_before();
   __syncthreads();
   if (warp == 1) {
@@ -868,19 +922,17 @@ static int allow_smem(size_t bytes) {
   return NES_OK;
 }
 
-template <int XF, int WF, int TOKENS, typename X = void>
-static int launch_product(const Product& p, const void* x, const void* w, cudaStream_t st) {
-  using L = Layout<TOKENS, !std::is_same<X, void>::value, XF == NES_MXFP4 ? 2 : 4>;
+template <int XF, int WF, int TOKENS, typename X, bool PUSH>
+static int launch_product(const Product& p, const void* x, const void* w, int splits, cudaStream_t st) {
+  using L = Layout<TOKENS, !std::is_same<X, void>::value, XF == NES_MXFP4 ? 2 : 4, PUSH>;
   ProductMaps maps;
   int rc = code_map(&maps.w, w, p.N, p.groups, WF == NES_MXFP4, WF == NES_MXFP4 && XF == NES_MXFP8, FEATURES);
   if (rc != NES_OK) return rc;
   maps.x = maps.w;
   if (std::is_same<X, void>::value && (rc = code_map(&maps.x, x, p.M, p.groups, XF == NES_MXFP4, false, TOKENS)) != NES_OK) return rc;
   const int64_t ftiles = ceil_div<int64_t>(p.N, FEATURES), ttiles = ceil_div<int64_t>(p.M, TOKENS);
-  const int steps = ceil_div(p.groups, CHUNKS);
-  const int splits = choose_splits(ftiles * ttiles, steps);
   NES_REQUIRE(ttiles <= 65535 && ftiles * splits <= INT32_MAX, NES_ERR_UNSUPPORTED, "mx_linear_fwd: too large");
-  if ((rc = allow_smem<mx_product_kernel<XF, WF, TOKENS, X>>(L::SMEM)) != NES_OK) return rc;
+  if ((rc = allow_smem<mx_product_kernel<XF, WF, TOKENS, X, PUSH>>(L::SMEM)) != NES_OK) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(ftiles * splits), unsigned(ttiles));
   cfg.blockDim = dim3(THREADS_TC);
@@ -894,7 +946,7 @@ static int launch_product(const Product& p, const void* x, const void* w, cudaSt
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = p.overlap ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, mx_product_kernel<XF, WF, TOKENS, X>, maps, p, splits);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, mx_product_kernel<XF, WF, TOKENS, X, PUSH>, maps, p, splits);
   if (e != cudaSuccess) return fail(NES_ERR_LAUNCH, "mx_linear_fwd: %s", cudaGetErrorString(e));
   return check_launch("mx_linear_fwd");
 }
@@ -939,6 +991,15 @@ static int launch_pair(const Product& p, const void* x, const void* w, cudaStrea
   return check_launch("mx_linear_fwd");
 }
 
+template <int XF, int WF, int TOKENS, typename X = void>
+static int launch_single(const Product& p, const void* x, const void* w, cudaStream_t st) {
+  const int splits = choose_splits(ceil_div<int64_t>(p.N, FEATURES) * ceil_div<int64_t>(p.M, TOKENS), ceil_div(p.groups, CHUNKS));
+  if constexpr (TOKENS >= 128) {
+    if (splits < 4) return launch_product<XF, WF, TOKENS, X, false>(p, x, w, splits, st);
+  }
+  return launch_product<XF, WF, TOKENS, X, true>(p, x, w, splits, st);
+}
+
 // Whether the product quantises its plain activations itself: few tokens, and a part of K per CTA that fits its shared memory.
 // Every feature tile's CTAs do so before their first product, at about 0.23 us per 8 elements of a thread (of 128); a
 // launch of its own costs the device 1.8 us and the host 4 us (1 token of 4096x4096: 7.9 us, else 8.6; 16 tokens: 11.3 and 9.0).
@@ -951,16 +1012,16 @@ static bool quantises_itself(int64_t M, int64_t N, int64_t K) {
 
 template <int XF, int WF>
 static int launch_raw(const Product& p, int x_dtype, const void* w, cudaStream_t st) {
-  if (x_dtype == NES_F32) return launch_product<XF, WF, 16, float>(p, nullptr, w, st);
-  if (x_dtype == NES_BF16) return launch_product<XF, WF, 16, __nv_bfloat16>(p, nullptr, w, st);
-  return launch_product<XF, WF, 16, __half>(p, nullptr, w, st);
+  if (x_dtype == NES_F32) return launch_single<XF, WF, 16, float>(p, nullptr, w, st);
+  if (x_dtype == NES_BF16) return launch_single<XF, WF, 16, __nv_bfloat16>(p, nullptr, w, st);
+  return launch_single<XF, WF, 16, __half>(p, nullptr, w, st);
 }
 
 template <int XF, int WF>
 static int launch_tokens(const Product& p, const void* x, const void* w, cudaStream_t st) {
-  if (p.M <= 16) return launch_product<XF, WF, 16>(p, x, w, st);
-  if (p.M <= 32) return launch_product<XF, WF, 32>(p, x, w, st);
-  if (p.M <= 64) return launch_product<XF, WF, 64>(p, x, w, st);
+  if (p.M <= 16) return launch_single<XF, WF, 16>(p, x, w, st);
+  if (p.M <= 32) return launch_single<XF, WF, 32>(p, x, w, st);
+  if (p.M <= 64) return launch_single<XF, WF, 64>(p, x, w, st);
   // Single CTAs on 128 x 128 tiles, or pairs on 256 x 256: what either takes in ns, from its waves over the SMs.  Measured
   // with 8-bit activations: a wave of either kind takes 2.5 us per 1024 of K, a wave of single CTAs 4.5 us besides (its
   // epilogue runs under nothing), the pairs 8 us in all.  512x4096x4096: 14.9 us single, 20.7 us in pairs; 1024x4096x4096:
@@ -972,7 +1033,7 @@ static int launch_tokens(const Product& p, const void* x, const void* w, cudaStr
     const int64_t single_ns = ceil_div<int64_t>(single * splits, sms) * (4500 + k / splits);
     if (8000 + ceil_div<int64_t>(pairs, sms / 2) * k < single_ns) return launch_pair<XF, WF>(p, x, w, st);
   }
-  return launch_product<XF, WF, 128>(p, x, w, st);
+  return launch_single<XF, WF, 128>(p, x, w, st);
 }
 
 static int64_t align256(int64_t v) { return (v + 255) & ~int64_t(255); }
