@@ -609,8 +609,8 @@ int nes_mx_elements(const void* codes, uint8_t* y, int64_t rows, int64_t cols, n
 
 /* y[t, n] = sum_k x[t, k] w[n, k] + bias[n] with microscaled operands, fp32 accumulation, rounded once to `y_dtype`.
  * w: codes and scales of (N, K).  x: with x_scales given, codes and scales of (M, K) in x_format; with x_scales NULL,
- * a (M, K) matrix of nes_dtype x_dtype, which is quantised to x_format into `scratch` first (scratch_bytes() of it;
- * none is needed otherwise).  Formats (x, w): (4, 4), (8, 4), (8, 8).  bias (N) may be NULL. */
+ * a (M, K) matrix of nes_dtype x_dtype, which is quantised to x_format on the way: by the product itself where
+ * scratch_bytes() is 0, into `scratch` (32-byte aligned) otherwise.  Formats (x, w): (4, 4), (8, 4), (8, 8).  bias (N) may be NULL. */
 int64_t nes_mx_linear_fwd_scratch_bytes(int64_t M, int64_t N, int64_t K, int x_format);
 int nes_mx_linear_fwd(const void* x, const uint8_t* x_scales, int x_dtype, int x_format, const void* w_codes,
                       const uint8_t* w_scales, int w_format, const float* bias, void* y, int y_dtype,
