@@ -67,7 +67,8 @@ def _compile_host():
 
 def _link_host(obj):
     cmd = ["g++", "-shared", "-o", HOST_PATH, obj, "-L" + LIB_DIR, "-lnesgpu_b200", "-Wl,-rpath,$ORIGIN/lib",
-           "-L" + os.path.join(_torch_dir(), "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10"]
+           "-L" + os.path.join(_torch_dir(), "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
+           "-lc10_cuda", "-lc10"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError("link failed:\n%s\n%s" % (res.stdout, res.stderr))

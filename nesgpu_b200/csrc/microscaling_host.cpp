@@ -3,10 +3,11 @@
 //
 // A call of these operators on a few rows takes the device 2 to 8 us; checked, allocated and launched from Python through
 // ctypes it took the host 11 us (a torch.empty 2 us, a ctypes call with its arguments 1.2 us beside the launch, the checks the
-// rest).  Functions take positional arguments only and are called by nesgpu_b200/microscaling.py, which documents them.
+// rest), from here 4 to 8.  Functions take positional arguments only and are called by nesgpu_b200/microscaling.py, which documents them.
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -91,7 +92,11 @@ struct Rows {
   }
 };
 
-at::Tensor bytes(const at::Tensor& like, int64_t rows, int64_t width) { return at::empty({rows, width}, like.options().dtype(at::kByte)); }
+// uninitialised, contiguous, on the device of `like`: the caching allocator without the dispatcher's way to it
+at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+at::Tensor bytes(const at::Tensor& like, int64_t rows, int64_t width) { return empty({rows, width}, at::kByte, like); }
 
 // Makes a tensor's device current for a launch and gives the stream that is current there.
 struct Launch {
@@ -146,6 +151,21 @@ PyObject* blocks_tuple(const at::Tensor& codes, const at::Tensor& scales, const 
   return Py_BuildValue("(NNLLN)", THPVariable_Wrap(codes), THPVariable_Wrap(scales), (long long)x.rows, (long long)x.cols, lead);
 }
 
+// (codes, scales, cols, format) -> (codes, scales, rows): checked, contiguous and aligned as the kernels read them
+PyObject* blocks(PyObject* const* a) {
+  at::Tensor codes = of_type(a[0], "codes", at::kByte), scales = of_type(a[1], "scales", at::kByte);
+  const int64_t cols = whole(a[2]), format = whole(a[3]);
+  if (cols < 1) refuse(PyExc_RuntimeError, "a microscaled tensor needs at least one column");
+  same_device(scales, codes.device(), "scales");
+  if (codes.dim() != 2 || scales.dim() != 2 || codes.size(1) != pitch(cols, format) || scales.size(1) != scale_pitch(cols) ||
+      codes.size(0) != scales.size(0))
+    refuse(PyExc_RuntimeError, "codes and scales of %lld columns in %s must be (rows, %lld) and (rows, %lld)", (long long)cols,
+           format == NES_MXFP4 ? "mxfp4" : "mxfp8", (long long)pitch(cols, format), (long long)scale_pitch(cols));
+  if (reinterpret_cast<uintptr_t>(codes.data_ptr()) % 32) codes = codes.clone();       // read in aligned 16- and 32-byte pieces
+  if (reinterpret_cast<uintptr_t>(scales.data_ptr()) % 4) scales = scales.clone();
+  return Py_BuildValue("(NNL)", THPVariable_Wrap(codes), THPVariable_Wrap(scales), (long long)codes.size(0));
+}
+
 PyObject* quantize(PyObject* const* a) {
   const Rows x(a[0], "input");
   const int64_t format = whole(a[1]);
@@ -172,7 +192,7 @@ PyObject* elements(PyObject* const* a) {
   const at::Tensor& codes = cuda_tensor(a[0], "codes");
   const int64_t cols = whole(a[1]);
   if (whole(a[3]) == NES_MXFP8) return view_rows(codes, a[2], cols, at::kFloat8_e4m3fn);
-  at::Tensor out = at::empty(sizes_of(a[2], cols), codes.options().dtype(at::kFloat8_e4m3fn));
+  at::Tensor out = empty(sizes_of(a[2], cols), at::kFloat8_e4m3fn, codes);
   const Launch launch(codes.device());
   check("nes_mx_elements", nes_mx_elements(codes.data_ptr(), static_cast<uint8_t*>(out.data_ptr()), codes.size(0), cols, launch.stream));
   return THPVariable_Wrap(out);
@@ -194,7 +214,7 @@ PyObject* dequantize(PyObject* const* a) {
   const int64_t cols = whole(a[2]);
   const at::ScalarType type = dtype_argument(a[5]);
   const int kind = kind_of(type, "the result");
-  at::Tensor out = at::empty(sizes_of(a[3], cols), codes.options().dtype(type));
+  at::Tensor out = empty(sizes_of(a[3], cols), type, codes);
   const Launch launch(codes.device());
   check("nes_mx_dequantize", nes_mx_dequantize(codes.data_ptr(), scales.data_ptr<uint8_t>(), out.data_ptr(), kind, codes.size(0), cols,
                                                int(whole(a[4])), launch.stream));
@@ -234,17 +254,17 @@ PyObject* linear(PyObject* const* a) {
       refuse(PyExc_RuntimeError, "out must be a contiguous %S tensor of %lld elements on %s", dtype_object(type), (long long)(rows * out_features),
              device.str().c_str());
   } else if (microscaled) {
-    y = at::empty(sizes_of(a[2], out_features), x.options().dtype(type));
+    y = empty(sizes_of(a[2], out_features), type, x);
   } else {
     std::vector<int64_t> sizes(x.sizes().begin(), x.sizes().end());
     sizes.back() = out_features;
-    y = at::empty(sizes, x.options().dtype(type));
+    y = empty(sizes, type, x);
   }
   const Launch launch(device);
   // a workspace of this call's own: calls captured into different graphs share nothing
   at::Tensor scratch;
   const int64_t need = microscaled ? 0 : nes_mx_linear_fwd_scratch_bytes(rows, out_features, in_features, int(x_format));
-  if (need) scratch = at::empty({need}, x.options().dtype(at::kByte));
+  if (need) scratch = empty({need}, at::kByte, x);
   check("nes_mx_linear_fwd",
         nes_mx_linear_fwd(x.data_ptr(), microscaled ? cuda_tensor(a[1], "scales").data_ptr<uint8_t>() : nullptr, microscaled ? 0 : plain->kind,
                           int(x_format), w.data_ptr(), w_scales.data_ptr<uint8_t>(), int(whole(a[8])), bias.defined() ? bias.data_ptr<float>() : nullptr,
@@ -265,7 +285,7 @@ PyObject* rms_norm(PyObject* const* a) {
     if (!THPVariable_Check(a[3]) || THPVariable_Unpack(a[3]).sizes() != x.t.sizes()) refuse(PyExc_RuntimeError, "residual must have the input's shape");
     residual = aligned(of_type(a[3], "residual", x.t.scalar_type()));
     same_device(residual, device, "residual");
-    h = at::empty(x.t.sizes(), x.t.options());
+    h = empty(x.t.sizes(), x.t.scalar_type(), x.t);
   }
   if (a[1] != Py_None) {
     weight = aligned(of_type(a[1], "weight", at::kFloat));
@@ -287,7 +307,7 @@ PyObject* rms_norm(PyObject* const* a) {
     y = bytes(x.t, x.rows, pitch(x.cols, format));
     scales = bytes(x.t, x.rows, scale_pitch(x.cols));
   } else {
-    y = at::empty(x.t.sizes(), x.t.options());
+    y = empty(x.t.sizes(), x.t.scalar_type(), x.t);
   }
   const Launch launch(device);
   auto data = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
@@ -322,7 +342,7 @@ PyMethodDef method(const char* name) {
   return {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<F, N>)), METH_FASTCALL, nullptr};
 }
 
-PyMethodDef methods[] = {method<quantize, 2>("quantize"), method<elements, 4>("elements"), method<block_scales, 3>("block_scales"),
+PyMethodDef methods[] = {method<blocks, 4>("blocks"), method<quantize, 2>("quantize"), method<elements, 4>("elements"), method<block_scales, 3>("block_scales"),
                          method<dequantize, 6>("dequantize"), method<linear, 12>("linear"), method<rms_norm, 7>("rms_norm"), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "nesgpu_b200._host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -14,7 +14,7 @@ import math
 import torch
 from torch import nn
 
-from . import _cabi as C         # loads the library that the extension module is linked with
+from . import _cabi  # noqa: F401  (loads the library that the extension module is linked with)
 
 try:
     from . import _host
@@ -49,27 +49,11 @@ class MicroscaledTensor:
     __slots__ = ("codes", "scales", "rows", "cols", "format", "_lead")
 
     def __init__(self, codes, scales, cols, format="mxfp4", shape=None):
-        _format(format)
-        cols = int(cols)
-        if cols < 1:
-            raise RuntimeError("a microscaled tensor needs at least one column")
-        codes = C.require_cuda(codes, "codes", torch.uint8)
-        scales = C.require_cuda(scales, "scales", torch.uint8)
-        if scales.device != codes.device:
-            raise RuntimeError("nesgpu_b200: scales is on %s, expected %s" % (scales.device, codes.device))
-        pitch, spitch = _pitches(cols, format)
-        rows = codes.shape[0] if codes.dim() else 0
-        if codes.shape != (rows, pitch) or scales.shape != (rows, spitch):
-            raise RuntimeError("codes and scales of %d columns in %s must be (rows, %d) and (rows, %d), got %s and %s"
-                               % (cols, format, pitch, spitch, tuple(codes.shape), tuple(scales.shape)))
-        if codes.data_ptr() % 32:                # the kernels read codes in aligned 16- and 32-byte pieces
-            codes = codes.clone()
-        if scales.data_ptr() % 4:
-            scales = scales.clone()
+        self.codes, self.scales, rows = _host.blocks(codes, scales, cols, _format(format))
         lead = (rows,) if shape is None else tuple(int(s) for s in shape)
         if math.prod(lead) != rows:
             raise RuntimeError("leading dimensions %s do not match %d rows" % (lead, rows))
-        self.codes, self.scales, self.rows, self.cols, self.format, self._lead = codes, scales, rows, cols, format, lead
+        self.rows, self.cols, self.format, self._lead = rows, cols, format, lead
 
     @property
     def shape(self):
