@@ -40,13 +40,13 @@ __device__ __forceinline__ float2 rsqrt_pair(double v) {
   return make_float2(r, 0.5f * r * float(1.0 - v * (double(r) * double(r))));
 }
 
-// h * (r.x + r.y) * g with the products' rounding errors carried along: s + se is the row's scale times the gain to 48 bits.
+// h * (r.x + r.y) * (g + gl) with the rounding errors carried along: s + se is the row's scale times the gain to 48 bits.
 // SHARP leaves the fp32 result rounded to odd (cut off, lowest bit set), so that a rounding to fewer bits afterwards
 // decides as it would on the unrounded value; a value exactly on a border does not occur except for a zero.  Otherwise
 // the result is rounded to nearest.
 template <bool SHARP>
-__device__ __forceinline__ float scaled(float h, float2 r, float g) {
-  const float s = r.x * g, se = fmaf(r.y, g, fmaf(r.x, g, -s));
+__device__ __forceinline__ float scaled(float h, float2 r, float g, float gl) {
+  const float s = r.x * g, se = fmaf(r.x, gl, fmaf(r.y, g, fmaf(r.x, g, -s)));
   if (SHARP) return __uint_as_float(__float_as_uint(__fmaf_rz(h, s, h * se)) | 1u);
   return fmaf(h, s, h * se);
 }
@@ -222,10 +222,15 @@ __device__ __forceinline__ void emit(const NormArgs& a, const Row<T>& row, int64
     float n[UNIT];
     load_gain<ACCESS, MOVED>(row.noise, c, cols, span_of(a.noise, a.members * a.cols), false, n);
 #pragma unroll
-    for (int i = 0; i < UNIT; ++i) g[i] = fmaf(row.sign, n[i], g[i]);
-  }
+    for (int i = 0; i < UNIT; ++i) {
+      // gain + noise as a sum and what it rounds away
+      const float e = row.sign * n[i], sum = g[i] + e, back = sum - g[i], lost = (g[i] - (sum - back)) + (e - back);
+      y[i] = scaled<OUT != 0>(h[i], r, sum, OUT != 0 ? lost : 0.f);
+    }
+  } else {
 #pragma unroll
-  for (int i = 0; i < UNIT; ++i) y[i] = scaled<OUT != 0>(h[i], r, g[i]);
+    for (int i = 0; i < UNIT; ++i) y[i] = scaled<OUT != 0>(h[i], r, g[i], 0.f);
+  }
   if (OUT == 0) {
     store_at<ACCESS>(row.y, c, cols, values_raw(y, T()));
     return;
