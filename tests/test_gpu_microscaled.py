@@ -155,7 +155,9 @@ def _check_norm(y, want, form, dtype):
     (4, 512, 0, True, False), (12, 1000, 4, True, True), (3, 1024, 0, True, False), (2, 2048, 1, False, False), (1, 4096, 0, True, False),
     (3, 4097, 0, True, False), (2, 8192, 2, True, False), (2, 16384, 0, True, False), (3, 16389, 0, True, False), (2, 40000, 2, True, True),
     (9, 16383, 0, True, False), (3, 17400, 0, True, False), (4, 17411, 2, False, False), (700, 515, 7, True, True), (601, 1023, 0, True, False),
-    (600, 1009, 0, True, False), (500, 250, 5, True, False), (420, 4099, 3, True, True), (300, 4350, 0, True, False), (640, 127, 0, True, False)])
+    (600, 1009, 0, True, False), (500, 250, 5, True, False), (420, 4099, 3, True, True), (300, 4350, 0, True, False), (640, 127, 0, True, False),
+    (304, 256, 4, True, True), (310, 512, 0, False, False), (300, 1024, 3, True, False), (297, 2048, 0, True, False), (320, 4096, 5, True, True),
+    (300, 8192, 0, True, False), (300, 1000, 6, False, True), (302, 2056, 2, True, False), (297, 5000, 0, True, False), (298, 17408, 0, False, False)])
 def test_rms_norm(rows, cols, members, with_residual, antithetic, dtype, form):
     ms = _ms()
     x = _inputs(rows, cols, dtype, rows + cols)

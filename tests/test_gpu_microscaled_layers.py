@@ -271,6 +271,31 @@ def test_two_graphs_replayed_at_once():
                 assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("rows", [1, 40, 200, 900])
+def test_calls_back_to_back(rows):
+    """Weights quantised right before the product that reads them, activations quantised by the kernel before it, results consumed
+    by the next call, in a row without a pause: what the same calls give one at a time."""
+    from nesgpu_b200 import microscaling as ms
+    W = [_rows(384, 512, 50 + i) for i in range(2)]
+    V = [_rows(512, 384, 60 + i) for i in range(2)]
+    X = [_rows(rows, 512, 70 + i, torch.bfloat16) for i in range(2)]
+
+    def chain(i, pause):
+        w = ms.quantize(W[i]); pause()
+        y = ms.linear(X[i], w); pause()
+        q = ms.rms_norm(y, output="mxfp8"); pause()
+        v = ms.quantize(V[i], "mxfp8"); pause()
+        z = ms.linear(q, v, dtype=torch.bfloat16); pause()
+        return y, z, ms.linear(z, w, activations="mxfp4")
+
+    want = [chain(i, torch.cuda.synchronize) for i in range(2)]
+    torch.cuda.synchronize()
+    got = [chain(i % 2, lambda: None) for i in range(40)]
+    for i, g in enumerate(got):
+        for a, b in zip(g, want[i % 2]):
+            assert torch.equal(a, b), i
+
+
 def test_calls_on_another_stream():
     from nesgpu_b200 import microscaling as ms
     w = ms.quantize(_rows(300, 640, 1), "mxfp8")
