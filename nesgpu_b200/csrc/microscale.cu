@@ -35,9 +35,9 @@ struct Place {
 
 // Rows of whole groups have no padding: the plain matrix is one row of groups.
 template <typename T, int FORMAT>
-__global__ void __launch_bounds__(THREADS) quantize_groups_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+__global__ void __launch_bounds__(THREADS) quantize_groups_kernel(const T* x, uint8_t* codes, uint8_t* scales,
                                                                   int64_t total, int64_t step) {
-  let_dependents_start();
+  take_turn();
   const int lane16 = threadIdx.x & 15;
   int64_t index = (int64_t(blockIdx.x) * THREADS + threadIdx.x) >> 4;
   for (; index + (IN_FLIGHT - 1) * step < (total & ~int64_t(1)); index += IN_FLIGHT * step) {        // both half-warps, all units
@@ -62,9 +62,9 @@ __global__ void __launch_bounds__(THREADS) quantize_groups_kernel(const T* __res
 }
 
 template <typename T, int FORMAT, bool ALIGNED>
-__global__ void __launch_bounds__(THREADS) quantize_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales,
+__global__ void __launch_bounds__(THREADS) quantize_kernel(const T* x, uint8_t* codes, uint8_t* scales,
                                                            int cols, Span span, Walk w) {
-  let_dependents_start();
+  take_turn();
   Place at(w);
   const int lane16 = threadIdx.x & 15;
   // the two half-warps of a warp may differ by one trip: both run until the first one is past the end
@@ -87,8 +87,9 @@ __global__ void __launch_bounds__(THREADS) quantize_kernel(const T* __restrict__
 }
 
 template <typename T, int FORMAT, bool ALIGNED>
-__global__ void __launch_bounds__(THREADS) dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ y,
+__global__ void __launch_bounds__(THREADS) dequantize_kernel(const uint8_t* codes, const uint8_t* scales, T* y,
                                                              int cols, Walk w) {
+  take_turn();
   Place at(w);
   const int lane16 = threadIdx.x & 15;
   while (__any_sync(0xffffffffu, at.index < w.total)) {
@@ -101,7 +102,7 @@ __global__ void __launch_bounds__(THREADS) dequantize_kernel(const uint8_t* __re
       s[u] = 0;
       if (index < w.total) {
         q[u] = load_codes<FORMAT>(codes, unit);
-        s[u] = __ldg(scales + (unit >> 2));
+        s[u] = fetch(scales + (unit >> 2));
       }
     }
 #pragma unroll
@@ -118,12 +119,13 @@ __global__ void __launch_bounds__(THREADS) dequantize_kernel(const uint8_t* __re
 }
 
 // e2m1 codes -> e4m3 bytes of the same values, where there is no padding: 16 codes of 8 bytes at a time
-__global__ void __launch_bounds__(THREADS) elements_groups_kernel(const uint2* __restrict__ codes, uint4* __restrict__ y, int64_t total) {
+__global__ void __launch_bounds__(THREADS) elements_groups_kernel(const uint2* codes, uint4* y, int64_t total) {
+  take_turn();
   const int64_t step = int64_t(gridDim.x) * THREADS;
   for (int64_t i = int64_t(blockIdx.x) * THREADS + threadIdx.x; i < total; i += IN_FLIGHT * step) {
     uint2 q[IN_FLIGHT];
 #pragma unroll
-    for (int u = 0; u < IN_FLIGHT; ++u) if (i + u * step < total) q[u] = __ldg(codes + i + u * step);
+    for (int u = 0; u < IN_FLIGHT; ++u) if (i + u * step < total) q[u] = fetch(codes + i + u * step);
 #pragma unroll
     for (int u = 0; u < IN_FLIGHT; ++u)
       if (i + u * step < total)
@@ -133,7 +135,8 @@ __global__ void __launch_bounds__(THREADS) elements_groups_kernel(const uint2* _
 
 // e2m1 codes -> e4m3 bytes of the same values, without the padding
 template <bool ALIGNED>
-__global__ void __launch_bounds__(THREADS) elements_kernel(const uint8_t* __restrict__ codes, uint8_t* __restrict__ y, int cols, Walk w) {
+__global__ void __launch_bounds__(THREADS) elements_kernel(const uint8_t* codes, uint8_t* y, int cols, Walk w) {
+  take_turn();
   Place at(w);
   const int lane16 = threadIdx.x & 15;
   while (__any_sync(0xffffffffu, at.index < w.total)) {
@@ -171,9 +174,9 @@ static void launch_quantize(const void* x, void* codes, uint8_t* scales, int64_t
   const T* in = static_cast<const T*>(x);
   const Span span = {static_cast<const uint8_t*>(x), reinterpret_cast<const uint8_t*>(in + rows * cols)};
   uint8_t* out = static_cast<uint8_t*>(codes);
-  if (aligned16(x) && cols % GROUP == 0) quantize_groups_kernel<T, FORMAT><<<grid, THREADS, 0, st>>>(in, out, scales, w.total, w.step);
-  else if (aligned16(x) && (cols * sizeof(T)) % 16 == 0) quantize_kernel<T, FORMAT, true><<<grid, THREADS, 0, st>>>(in, out, scales, int(cols), span, w);
-  else quantize_kernel<T, FORMAT, false><<<grid, THREADS, 0, st>>>(in, out, scales, int(cols), span, w);
+  if (aligned16(x) && cols % GROUP == 0) launch_in_turn(quantize_groups_kernel<T, FORMAT>, grid, THREADS, st, in, out, scales, w.total, w.step);
+  else if (aligned16(x) && (cols * sizeof(T)) % 16 == 0) launch_in_turn(quantize_kernel<T, FORMAT, true>, grid, THREADS, st, in, out, scales, int(cols), span, w);
+  else launch_in_turn(quantize_kernel<T, FORMAT, false>, grid, THREADS, st, in, out, scales, int(cols), span, w);
 }
 
 template <typename T, int FORMAT>
@@ -182,8 +185,8 @@ static void launch_dequantize(const void* codes, const uint8_t* scales, void* y,
   const Walk w = plan(rows, cols, &grid);
   const uint8_t* in = static_cast<const uint8_t*>(codes);
   T* out = static_cast<T*>(y);
-  if (aligned16(y) && (cols * sizeof(T)) % 16 == 0) dequantize_kernel<T, FORMAT, true><<<grid, THREADS, 0, st>>>(in, scales, out, int(cols), w);
-  else dequantize_kernel<T, FORMAT, false><<<grid, THREADS, 0, st>>>(in, scales, out, int(cols), w);
+  if (aligned16(y) && (cols * sizeof(T)) % 16 == 0) launch_in_turn(dequantize_kernel<T, FORMAT, true>, grid, THREADS, st, in, scales, out, int(cols), w);
+  else launch_in_turn(dequantize_kernel<T, FORMAT, false>, grid, THREADS, st, in, scales, out, int(cols), w);
 }
 
 }  // namespace mx
@@ -236,8 +239,8 @@ extern "C" int nes_mx_elements(const void* codes, uint8_t* y, int64_t rows, int6
   if (aligned16(y) && cols % GROUP == 0) {
     const int64_t total = rows * cols / 16;
     const int64_t blocks = std::min<int64_t>(ceil_div<int64_t>(total, THREADS), int64_t(sm_count()) * 8);
-    elements_groups_kernel<<<unsigned(blocks), THREADS, 0, as_stream(stream)>>>(static_cast<const uint2*>(codes), reinterpret_cast<uint4*>(y), total);
-  } else if ((reinterpret_cast<uintptr_t>(y) & 7u) == 0 && cols % UNIT == 0) elements_kernel<true><<<grid, THREADS, 0, as_stream(stream)>>>(in, y, int(cols), w);
-  else elements_kernel<false><<<grid, THREADS, 0, as_stream(stream)>>>(in, y, int(cols), w);
+    launch_in_turn(elements_groups_kernel, unsigned(blocks), THREADS, as_stream(stream), static_cast<const uint2*>(codes), reinterpret_cast<uint4*>(y), total);
+  } else if ((reinterpret_cast<uintptr_t>(y) & 7u) == 0 && cols % UNIT == 0) launch_in_turn(elements_kernel<true>, grid, THREADS, as_stream(stream), in, y, int(cols), w);
+  else launch_in_turn(elements_kernel<false>, grid, THREADS, as_stream(stream), in, y, int(cols), w);
   return check_launch("mx_elements");
 }

@@ -30,6 +30,10 @@ inline bool known_dtype(int t) { return t == NES_F32 || t == NES_BF16 || t == NE
 inline bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
 inline int64_t dtype_bytes(int t) { return t == NES_F32 ? 4 : 2; }
 
+// An ordinary load.  Not __ldg and no __restrict__ inputs in these kernels: a load of memory that is taken to be constant for the
+// whole kernel could be moved ahead of the wait for the kernel before (take_turn below), which may just be writing it.
+template <typename V> __device__ __forceinline__ V fetch(const V* p) { return *p; }
+
 template <typename T> __device__ __forceinline__ float to_float(T v);
 template <> __device__ __forceinline__ float to_float<float>(float v) { return v; }
 template <> __device__ __forceinline__ float to_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
@@ -79,7 +83,7 @@ struct Span { const uint8_t *begin, *end; };                      // of a whole 
 // the aligned 16-byte word at `at`, bytes outside the tensor read as zero without being touched
 template <typename T>
 __device__ __forceinline__ uint4 load_word(const Span& s, const uint8_t* at) {
-  if (at >= s.begin && at + 16 <= s.end) return __ldg(reinterpret_cast<const uint4*>(at));
+  if (at >= s.begin && at + 16 <= s.end) return fetch(reinterpret_cast<const uint4*>(at));
   uint32_t w[4] = {0u, 0u, 0u, 0u};
 #pragma unroll
   for (int i = 0; i < int(16 / sizeof(T)); ++i) {
@@ -104,7 +108,7 @@ __device__ __forceinline__ Raw<T> load_raw(const T* row, int c, int cols, const 
 #pragma unroll
     for (int i = 0; i < NW; i += 4) {
       if (i && !inside(c + 4, cols)) break;                       // an fp32 unit may lie half inside
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(at) + i / 4);
+      const uint4 v = fetch(reinterpret_cast<const uint4*>(at) + i / 4);
       r.w[i] = v.x; r.w[i + 1] = v.y; r.w[i + 2] = v.z; r.w[i + 3] = v.w;
     }
     return r;
@@ -115,7 +119,7 @@ __device__ __forceinline__ Raw<T> load_raw(const T* row, int c, int cols, const 
 #pragma unroll
   for (int i = 0; i < NW + 4; i += 4) {
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (i < NW || shift) v = interior ? __ldg(reinterpret_cast<const uint4*>(at - shift + 4 * i)) : load_word<T>(span, at - shift + 4 * i);
+    if (i < NW || shift) v = interior ? fetch(reinterpret_cast<const uint4*>(at - shift + 4 * i)) : load_word<T>(span, at - shift + 4 * i);
     e[i] = v.x; e[i + 1] = v.y; e[i + 2] = v.z; e[i + 3] = v.w;
   }
   const bool two = shift & 8u, one = shift & 4u;
@@ -243,10 +247,31 @@ __device__ __forceinline__ uint32_t scale_code(uint32_t m) {
   return m >= 0x7f800000u ? 255u : uint32_t(max(int(m >> 23) - EMAX, 0));
 }
 
-// A product that reads what a quantising kernel before it writes may be started while that kernel still runs: the first lets it
-// (once all its blocks have begun), the second waits until the kernel before has ended and its writes can be seen.
-__device__ __forceinline__ void let_dependents_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// Kernels of a chain are started while the one before still runs, and wait for it before they touch memory: what is saved is the
+// launch and the set-up, a microsecond or two of the few that calls on few rows take.  take_turn() waits until the kernel
+// before has ended and its writes can be seen, and only then lets the next one start: what a kernel finds done when it starts
+// is everything but the kernel just before it.
 __device__ __forceinline__ void wait_for_kernel_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void take_turn() {
+  wait_for_kernel_before();
+  let_next_start();
+}
+
+// Launches a kernel that takes its turn as above; an error is left to check_launch.
+template <typename... P, typename... A>
+inline void launch_in_turn(void (*kernel)(P...), unsigned grid, unsigned threads, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
 
 // 2^-e for a scale code below 255 (at most 253: a normal number); 0 for 255
 __device__ __forceinline__ float inverse_scale(uint32_t code) { return __uint_as_float(code == 255u ? 0u : (254u - code) << 23); }
@@ -327,8 +352,8 @@ __device__ __forceinline__ float2 e4m3x2_to_float(uint32_t two) {
 // The eight elements of a unit as e4m3 bytes, and their values before the scale.
 template <int FORMAT>
 __device__ __forceinline__ uint2 load_codes(const uint8_t* codes_row, int64_t unit) {
-  if (FORMAT == NES_MXFP8) return __ldg(reinterpret_cast<const uint2*>(codes_row) + unit);
-  const uint32_t c = __ldg(reinterpret_cast<const uint32_t*>(codes_row) + unit);
+  if (FORMAT == NES_MXFP8) return fetch(reinterpret_cast<const uint2*>(codes_row) + unit);
+  const uint32_t c = fetch(reinterpret_cast<const uint32_t*>(codes_row) + unit);
   return make_uint2(e2m1x4_to_e4m3(c), e2m1x4_to_e4m3(c >> 16));
 }
 __device__ __forceinline__ void unit_elements(const uint2& q, float (&v)[UNIT]) {

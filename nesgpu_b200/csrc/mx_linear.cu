@@ -12,13 +12,13 @@
 //     column per 32 rows and 128 elements, repeated in each quarter of the lanes.  Four warps load them for STEP = 512
 //     elements of K at a time, 16 bytes per row and thread, transpose them on the way into shared memory, and tcgen05.cp
 //     brings them over in the order of the products.
-//   * Plain activations are quantised into scratch first; a few tokens are quantised by the product itself, every CTA
+//   * Plain activations are quantised into scratch first, under which the product starts and loads its first weights; a few tokens are quantised by the product itself, every CTA
 //     its own part of K straight into the operand's place in shared memory.
 //   * Few output tiles: a cluster of up to eight CTAs splits K and adds its partial tiles in a fixed order through
 //     distributed shared memory.
 //
-// Few tokens are bound by the launch, the latencies of one load - product - store chain and then the weights' bytes: 1 token of
-// 4096x4096 takes 7.2 us with 8.9 MB to read (1.4 us), 24 tokens of 8192x8192 10.9 us (35.7 MB, 5.5 us).  Many are bound by
+// Few tokens are bound by the latencies of one load - product - store chain and then the weights' bytes: 1 token of
+// 4096x4096 takes 6.0 us with 8.9 MB to read (1.4 us), 24 tokens of 8192x8192 9.8 us (35.7 MB, 5.5 us).  Many are bound by
 // the tensor pipe and the power limit: 8192x4096x16384 in 4 bits takes 254 us in a burst (4.3 PFLOP/s) and 300 us back to back
 // at 1.64 GHz, with 8-bit activations 394 and 472 us (2.8 and 2.3 PFLOP/s at 1.4 GHz).
 #include <type_traits>
@@ -45,7 +45,7 @@ struct Product {
   int y_dtype, vec_scales;
   const void* x;                             // plain activations of a product that quantises them itself
   int whole_rows;                            // their rows are whole, aligned 16-byte pieces
-  bool overlap;                              // the kernel before quantises the activations and lets this one start early
+  bool overlap;                              // the kernel before quantises the activations: the weights have been there before it
 };
 struct ProductMaps { CUtensorMap w, x; };
 
@@ -216,10 +216,10 @@ __device__ __forceinline__ void st_cluster(uint32_t remote, float v) {
 __device__ __forceinline__ float4 four_biases(const Product& p, int n, int left) {
   float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
   if (p.bias) {
-    b.x = __ldg(p.bias + n);
-    if (left > 1) b.y = __ldg(p.bias + n + 1);
-    if (left > 2) b.z = __ldg(p.bias + n + 2);
-    if (left > 3) b.w = __ldg(p.bias + n + 3);
+    b.x = fetch(p.bias + n);
+    if (left > 1) b.y = fetch(p.bias + n + 1);
+    if (left > 2) b.z = fetch(p.bias + n + 2);
+    if (left > 3) b.w = fetch(p.bias + n + 3);
   }
   return b;
 }
@@ -396,6 +396,7 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
       // first coordinate: bytes of codes, or elements of a copy that spreads 4-bit codes.  The weights of the first stages do not
       // depend on the kernel before; the activations may.
       const int ready = RAW ? 0 : min(int(L::STAGES), kt1 - kt0);
+      if (!p.overlap) wait_for_kernel_before();
       for (int i = 0; i < ready; ++i) {
         mbar_expect_tx(&full[i], TX);
         tma_load_2d(tiles + size_t(i) * L::STAGE, &maps.w, &full[i], (kt0 + i) * ROW_BYTES, n0);
@@ -423,6 +424,7 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
     int s = 0;
     uint32_t ph = 0, sf_ph = 0, accumulate = 0;
     int kt = kt0;
+    wait_for_kernel_before();                         // the bounded waits count from here
     if (RAW) ok = warp_mbar_wait(raw_full, 0, 2);
     for (int step = step0; step < step1 && ok; ++step) {
       const int b = (step - step0) & 1;
@@ -461,7 +463,7 @@ __global__ void __launch_bounds__(THREADS_TC, 1) mx_product_kernel(const __grid_
     const uint32_t lanes = uint32_t(q * 32) << 16;
     const int t = threadIdx.x - 64, row = scale_row(t);
     uint4 wv[4], xv[4];                              // four steps in flight
-    wait_for_kernel_before();
+    take_turn();
     auto load = [&](int step, uint4& wo, uint4& xo) {
       if (step >= step1) return;
       wo = load_scale_words(p.w_scales, n0 + row, p.N, step * CHUNKS, p.groups, p.vec_scales);
@@ -694,6 +696,7 @@ mx_pair_kernel(const __grid_constant__ PairMaps maps, const Product p, int ftile
       const uint32_t full0 = map_rank(smem_u32(full), 0);
       // the weights of the first stages do not depend on the kernel before; the activations may
       const int ready = pair < tiles ? min(int(L::STAGES), kts) : 0;
+      if (!p.overlap) wait_for_kernel_before();
       {
         const int2 at = tile_place(pair, ftiles, ttiles);
         const int n0 = at.x * PAIR_FEATURES + rank * FEATURES, m0 = at.y * PAIR_TOKENS + rank * (PAIR_TOKENS / 2);
@@ -723,6 +726,7 @@ mx_pair_kernel(const __grid_constant__ PairMaps maps, const Product p, int ftile
     }
     __syncwarp();
   } else if (warp == 1) {
+    wait_for_kernel_before();                                      // the bounded waits count from here
     if (rank == 0) {
       constexpr uint32_t idesc = idesc_scaled<XF, WF>(PAIR_FEATURES, PAIR_TOKENS);
       const uint64_t desc0 = smem_desc_sw128(smem_u32(stages));
@@ -799,7 +803,7 @@ mx_pair_kernel(const __grid_constant__ PairMaps maps, const Product p, int ftile
       o[2] = load_scale_words(p.x_scales, m0 + 128 + row, p.M, step * CHUNKS, p.groups, p.vec_scales);
       if (++step == steps) { step = 0; tile += pairs; }
     };
-    wait_for_kernel_before();
+    take_turn();
 #pragma unroll
     for (int i = 0; i < 4; ++i) load(v[i]);
     const int64_t total = pair < tiles ? int64_t((tiles - 1 - pair) / pairs + 1) * steps : 0;
@@ -823,6 +827,7 @@ mx_pair_kernel(const __grid_constant__ PairMaps maps, const Product p, int ftile
     const uint32_t lanes = uint32_t(q * 32) << 16;
     const uint32_t acc_empty0 = map_rank(smem_u32(acc_empty), 0);
     unsigned char* box = boxes + (warp - 6) * 2 * L::OUT_BYTES;
+    wait_for_kernel_before();
     int acc = 0, side = 0;
     uint32_t ph = 0;
     for (int tile = pair; tile < tiles; tile += pairs) {
@@ -832,7 +837,7 @@ mx_pair_kernel(const __grid_constant__ PairMaps maps, const Product p, int ftile
       if (!ok) break;
       tc_fence_after();
       const bool good = __all_sync(0xffffffffu, timeouts_so_far() == timeouts_at_start);
-      const float bias = p.bias && n0 + lane < p.N ? __ldg(p.bias + n0 + lane) : 0.f;
+      const float bias = p.bias && n0 + lane < p.N ? fetch(p.bias + n0 + lane) : 0.f;
       auto emit = [&](int c, const uint32_t (&r)[32]) {
         if (!good || n0 >= p.N || m0 + c >= p.M) return;
         if (tma_out) {
@@ -949,7 +954,7 @@ static int launch_product(const Product& p, const void* x, const void* w, int sp
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = p.overlap ? 2 : 1;
+  cfg.numAttrs = 2;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, mx_product_kernel<XF, WF, TOKENS, X, PUSH>, maps, p, splits);
   if (e != cudaSuccess) return fail(NES_ERR_LAUNCH, "mx_linear_fwd: %s", cudaGetErrorString(e));
   return check_launch("mx_linear_fwd");
@@ -989,7 +994,7 @@ static int launch_pair(const Product& p, const void* x, const void* w, cudaStrea
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = p.overlap ? 1 : 0;
+  cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, mx_pair_kernel<XF, WF>, maps, p, int(ftiles), int(ttiles), tma_out);
   if (e != cudaSuccess) return fail(NES_ERR_LAUNCH, "mx_linear_fwd: %s", cudaGetErrorString(e));
   return check_launch("mx_linear_fwd");

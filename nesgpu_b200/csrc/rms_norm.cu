@@ -91,7 +91,7 @@ __device__ __forceinline__ Raw<T> load_boundary(const T* row, int c, int cols, c
   if (c >= 0 && c + UNIT <= cols) {
 #pragma unroll
     for (int i = 0; i < NW; i += 4) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + c) + i / 4);
+      const uint4 v = fetch(reinterpret_cast<const uint4*>(row + c) + i / 4);
       r.w[i] = v.x; r.w[i + 1] = v.y; r.w[i + 2] = v.z; r.w[i + 3] = v.w;
     }
   } else if (c < cols && c + UNIT > 0) {
@@ -132,7 +132,7 @@ __device__ __forceinline__ Raw<float> load_split(const float* row, int c, int co
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (inside(c + h * HALF_APART, cols)) v = __ldg(reinterpret_cast<const uint4*>(row + c + h * HALF_APART));
+    if (inside(c + h * HALF_APART, cols)) v = fetch(reinterpret_cast<const uint4*>(row + c + h * HALF_APART));
     r.w[4 * h] = v.x; r.w[4 * h + 1] = v.y; r.w[4 * h + 2] = v.z; r.w[4 * h + 3] = v.w;
   }
   return r;
@@ -299,6 +299,7 @@ template <typename T, int OUT, int UNITS, RowAccess ACCESS, bool BLOCK_ROW>
 __global__ void __launch_bounds__(BLOCK_ROW ? MOST_WARPS * 32 : WARP_ROWS * 32) rms_norm_kernel(const NormArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t index = BLOCK_ROW ? int64_t(blockIdx.x) : int64_t(blockIdx.x) * WARP_ROWS + warp;
+  take_turn();
   if (index >= a.rows) return;
   const Row<T> row(a, index);
   const int base = BLOCK_ROW ? warp * UNITS * 32 * UNIT : 0, first = base + lane * (is_split(ACCESS) ? 4 : UNIT);
@@ -334,6 +335,7 @@ __global__ void __launch_bounds__(BLOCK_ROW ? MOST_WARPS * 32 : WARP_ROWS * 32) 
 template <typename T, int OUT, RowAccess ACCESS>
 __global__ void __launch_bounds__(512) rms_norm_long_kernel(const NormArgs a) {
   const int64_t index = blockIdx.x;
+  take_turn();
   const Row<T> row(a, index);
   const int end = int(padded(a.cols)), step = blockDim.x * UNIT;
   float s = 0.f;
@@ -362,16 +364,16 @@ static void launch_rows(const NormArgs& a, int64_t units, cudaStream_t st) {
   const unsigned grid = unsigned(BLOCK_ROW ? a.rows : ceil_div<int64_t>(a.rows, WARP_ROWS));
   const unsigned threads = unsigned(BLOCK_ROW ? ceil_div<int64_t>(units, OF_WARP) : WARP_ROWS) * 32;
   if (ALIGNED && (BLOCK_ROW ? a.cols % (OF_WARP * UNIT) == 0 : a.cols == OF_WARP * UNIT))
-    rms_norm_kernel<T, OUT, UNITS, PLAIN, BLOCK_ROW><<<grid, threads, 0, st>>>(a);
+    launch_in_turn(rms_norm_kernel<T, OUT, UNITS, PLAIN, BLOCK_ROW>, grid, threads, st, a);
   else
-    rms_norm_kernel<T, OUT, UNITS, GUARDED, BLOCK_ROW><<<grid, threads, 0, st>>>(a);
+    launch_in_turn(rms_norm_kernel<T, OUT, UNITS, GUARDED, BLOCK_ROW>, grid, threads, st, a);
 }
 
 template <typename T, int OUT, bool ALIGNED>
 static void launch_norm(const NormArgs& a, cudaStream_t st) {
   const int64_t units = ALIGNED ? ceil_div<int64_t>(a.cols, 32 * UNIT) * 32 : std::max<int64_t>(padded(a.cols) / UNIT, (a.cols + 2 * (UNIT - 1)) / UNIT);
   const bool few = a.rows < 2 * sm_count();
-  if (units > MOST_WARPS * 32 * 4) rms_norm_long_kernel<T, OUT, ALIGNED ? WHOLE : ANY><<<unsigned(a.rows), 512, 0, st>>>(a);
+  if (units > MOST_WARPS * 32 * 4) launch_in_turn(rms_norm_long_kernel<T, OUT, ALIGNED ? WHOLE : ANY>, unsigned(a.rows), 512, st, a);
   else if (units <= 32) launch_rows<T, OUT, 1, ALIGNED, false>(a, units, st);
   else if (few && units <= MOST_WARPS * 32) launch_rows<T, OUT, 1, ALIGNED, true>(a, units, st);
   else if (units <= 64) launch_rows<T, OUT, 2, ALIGNED, false>(a, units, st);
