@@ -593,7 +593,8 @@ int nes_binarized_int_threshold(const uint16_t* bias_half, const uint16_t* bias_
  * infinity has c = 255 and zero elements.
  * Layout: row-major, rows padded with zero codes and zero scales to whole groups of 128 elements: with
  * G = ceil(cols / 128), codes (rows, 64 G | 128 G) bytes, 16-byte aligned, scales (rows, 4 G) bytes; the product
- * wants codes 32-byte and scales 4-byte aligned. */
+ * wants codes 32-byte and scales 4-byte aligned.  An output that overlaps an input of the same call is refused
+ * (NES_ERR_BAD_ARG). */
 
 enum nes_dtype { NES_F32 = 0, NES_BF16 = 1, NES_F16 = 2 };
 enum nes_mx_format { NES_MXFP4 = 4, NES_MXFP8 = 8 };
@@ -619,7 +620,7 @@ int nes_mx_linear_fwd(const void* x, const uint8_t* x_scales, int x_dtype, int x
 /* RMS norm of population rows, with the residual's addition:
  *   h = x + residual;  y = h / sqrt(mean(h^2) + eps) * (gain + s(r) * noise[d]),  row = r * members + d
  * x, residual, residual_out (rows, cols) of nes_dtype `dtype`; residual and residual_out are both NULL or both given,
- * residual_out receives h rounded to `dtype` and may not overlap x or residual.  gain (cols) and noise
+ * residual_out receives h rounded to `dtype`.  gain (cols) and noise
  * (members, cols) are fp32, either may be NULL (gain 1, no noise).  format 0: y (rows, cols) of `dtype`;
  * otherwise y and y_scales receive the codes and scales of that microscaled format.  All tensors but y_scales start
  * on 16 bytes. */

@@ -203,6 +203,8 @@ extern "C" int nes_mx_quantize(const void* x, int dtype, void* codes, uint8_t* s
   if (rows == 0 || cols == 0) return NES_OK;
   NES_REQUIRE(x && codes && scales, NES_ERR_BAD_ARG, "mx_quantize: null pointer");
   NES_REQUIRE(aligned16(codes), NES_ERR_BAD_ARG, "mx_quantize: codes must be 16-byte aligned");
+  const Bytes outputs[] = {{codes, rows * code_pitch(cols, format)}, {scales, rows * scale_pitch(cols)}}, inputs[] = {{x, rows * cols * dtype_bytes(dtype)}};
+  NES_REQUIRE(!overlap(outputs, inputs), NES_ERR_BAD_ARG, "mx_quantize: the outputs overlap the input");
   cudaStream_t st = as_stream(stream);
   const bool four = format == NES_MXFP4;
   if (dtype == NES_F32) (four ? launch_quantize<float, NES_MXFP4> : launch_quantize<float, NES_MXFP8>)(x, codes, scales, rows, cols, st);
@@ -219,6 +221,8 @@ extern "C" int nes_mx_dequantize(const void* codes, const uint8_t* scales, void*
   if (rows == 0 || cols == 0) return NES_OK;
   NES_REQUIRE(codes && scales && y, NES_ERR_BAD_ARG, "mx_dequantize: null pointer");
   NES_REQUIRE(aligned16(codes), NES_ERR_BAD_ARG, "mx_dequantize: codes must be 16-byte aligned");
+  const Bytes outputs[] = {{y, rows * cols * dtype_bytes(dtype)}}, inputs[] = {{codes, rows * code_pitch(cols, format)}, {scales, rows * scale_pitch(cols)}};
+  NES_REQUIRE(!overlap(outputs, inputs), NES_ERR_BAD_ARG, "mx_dequantize: the output overlaps an input");
   cudaStream_t st = as_stream(stream);
   const bool four = format == NES_MXFP4;
   if (dtype == NES_F32) (four ? launch_dequantize<float, NES_MXFP4> : launch_dequantize<float, NES_MXFP8>)(codes, scales, y, rows, cols, st);
@@ -233,6 +237,7 @@ extern "C" int nes_mx_elements(const void* codes, uint8_t* y, int64_t rows, int6
   if (rows == 0 || cols == 0) return NES_OK;
   NES_REQUIRE(codes && y, NES_ERR_BAD_ARG, "mx_elements: null pointer");
   NES_REQUIRE(aligned16(codes), NES_ERR_BAD_ARG, "mx_elements: codes must be 16-byte aligned");
+  NES_REQUIRE(!overlap(Bytes{y, rows * cols}, Bytes{codes, rows * code_pitch(cols, NES_MXFP4)}), NES_ERR_BAD_ARG, "mx_elements: the output overlaps the input");
   unsigned grid;
   const Walk w = plan(rows, cols, &grid);
   const uint8_t* in = static_cast<const uint8_t*>(codes);

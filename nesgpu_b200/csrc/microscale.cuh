@@ -30,6 +30,20 @@ inline bool known_dtype(int t) { return t == NES_F32 || t == NES_BF16 || t == NE
 inline bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
 inline int64_t dtype_bytes(int t) { return t == NES_F32 ? 4 : 2; }
 
+// What a call reads or writes.  The blocks of a kernel run in any order, so an output that lies over an input is refused.
+struct Bytes { const void* at; int64_t size; };
+inline bool overlap(const Bytes& a, const Bytes& b) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
+  return a.at && b.at && x < y + uintptr_t(b.size) && y < x + uintptr_t(a.size);
+}
+template <int A, int B>
+inline bool overlap(const Bytes (&outputs)[A], const Bytes (&inputs)[B]) {
+  for (const Bytes& o : outputs)
+    for (const Bytes& i : inputs)
+      if (overlap(o, i)) return true;
+  return false;
+}
+
 // An ordinary load.  Not __ldg and no __restrict__ inputs in these kernels: a load of memory that is taken to be constant for the
 // whole kernel could be moved ahead of the wait for the kernel before (take_turn below), which may just be writing it.
 template <typename V> __device__ __forceinline__ V fetch(const V* p) { return *p; }

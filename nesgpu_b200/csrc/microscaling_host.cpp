@@ -108,8 +108,13 @@ struct Launch {
   }
 };
 
-// Status of an entry point -> NotImplementedError or nesgpu_b200._cabi.NesError, as the ctypes binding does
-void check(const char* name, int status) {
+// Calls an entry point without the interpreter's lock, as a ctypes call does (a launch waits while the device's queue is full);
+// status -> NotImplementedError or nesgpu_b200._cabi.NesError.
+template <typename F>
+void run(const char* name, F&& call) {
+  PyThreadState* state = PyEval_SaveThread();
+  const int status = call();
+  PyEval_RestoreThread(state);
   if (status == NES_OK) return;
   PyObject* type = PyExc_NotImplementedError;
   if (status != NES_ERR_UNSUPPORTED) {
@@ -129,11 +134,17 @@ int64_t whole(PyObject* o) {
   return v;
 }
 
-std::vector<int64_t> sizes_of(PyObject* lead, int64_t last) {          // lead: a tuple of whole numbers
+// (lead ..., last); lead: a tuple of whole numbers whose product is `rows`
+std::vector<int64_t> sizes_of(PyObject* lead, int64_t last, int64_t rows) {
   std::vector<int64_t> s;
   const Py_ssize_t n = PyTuple_Size(lead);
   if (n < 0) throw Raised();
-  for (Py_ssize_t i = 0; i < n; ++i) s.push_back(whole(PyTuple_GET_ITEM(lead, i)));
+  int64_t product = 1;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    s.push_back(whole(PyTuple_GET_ITEM(lead, i)));
+    product *= s.back();
+  }
+  if (product != rows) refuse(PyExc_RuntimeError, "leading dimensions %R do not match %lld rows", lead, (long long)rows);
   s.push_back(last);
   return s;
 }
@@ -166,18 +177,29 @@ PyObject* blocks(PyObject* const* a) {
   return Py_BuildValue("(NNL)", THPVariable_Wrap(codes), THPVariable_Wrap(scales), (long long)codes.size(0));
 }
 
+// The tensors of blocks that exist already, looked at again where they are used: the object that holds them may have been given
+// others, or one of them resized, since `blocks` saw them.  `like`: the codes that scales belong to.
+void as_made(const at::Tensor& t, int64_t width, const char* name, const at::Tensor* like = nullptr) {
+  if (t.scalar_type() != at::kByte || t.dim() != 2 || t.size(1) != width || !t.is_contiguous() || (like && t.size(0) != like->size(0)))
+    refuse(PyExc_RuntimeError, "%s of a microscaled tensor must be contiguous uint8 of %lld bytes to a row, and as many rows of codes as of scales", name,
+           (long long)width);
+  if (like) same_device(t, like->device(), name);
+}
+
 PyObject* quantize(PyObject* const* a) {
   const Rows x(a[0], "input");
   const int64_t format = whole(a[1]);
   at::Tensor codes = bytes(x.t, x.rows, pitch(x.cols, format)), scales = bytes(x.t, x.rows, scale_pitch(x.cols));
   const Launch launch(x.t.device());
-  check("nes_mx_quantize", nes_mx_quantize(x.t.data_ptr(), x.kind, codes.data_ptr(), scales.data_ptr<uint8_t>(), x.rows, x.cols, int(format), launch.stream));
+  run("nes_mx_quantize", [&] {
+    return nes_mx_quantize(x.t.data_ptr(), x.kind, codes.data_ptr(), scales.data_ptr<uint8_t>(), x.rows, x.cols, int(format), launch.stream);
+  });
   return blocks_tuple(codes, scales, x);
 }
 
 // the first `width` bytes of every row of `t` with leading dimensions `lead`, as elements of `type`
 PyObject* view_rows(const at::Tensor& t, PyObject* lead, int64_t width, at::ScalarType type) {
-  const std::vector<int64_t> sizes = sizes_of(lead, width);
+  const std::vector<int64_t> sizes = sizes_of(lead, width, t.size(0));
   std::vector<int64_t> strides(sizes.size(), 1);
   int64_t stride = t.size(1);
   for (size_t i = sizes.size() - 1; i-- > 0;) {
@@ -191,16 +213,21 @@ PyObject* view_rows(const at::Tensor& t, PyObject* lead, int64_t width, at::Scal
 PyObject* elements(PyObject* const* a) {
   const at::Tensor& codes = cuda_tensor(a[0], "codes");
   const int64_t cols = whole(a[1]);
-  if (whole(a[3]) == NES_MXFP8) return view_rows(codes, a[2], cols, at::kFloat8_e4m3fn);
-  at::Tensor out = empty(sizes_of(a[2], cols), at::kFloat8_e4m3fn, codes);
+  const int64_t format = whole(a[3]);
+  as_made(codes, pitch(cols, format), "codes");
+  if (format == NES_MXFP8) return view_rows(codes, a[2], cols, at::kFloat8_e4m3fn);
+  at::Tensor out = empty(sizes_of(a[2], cols, codes.size(0)), at::kFloat8_e4m3fn, codes);
   const Launch launch(codes.device());
-  check("nes_mx_elements", nes_mx_elements(codes.data_ptr(), static_cast<uint8_t*>(out.data_ptr()), codes.size(0), cols, launch.stream));
+  run("nes_mx_elements", [&] { return nes_mx_elements(codes.data_ptr(), static_cast<uint8_t*>(out.data_ptr()), codes.size(0), cols, launch.stream); });
   return THPVariable_Wrap(out);
 }
 
 // (scales, cols, lead)
 PyObject* block_scales(PyObject* const* a) {
-  return view_rows(cuda_tensor(a[0], "scales"), a[2], (whole(a[1]) + 31) / 32, at::kFloat8_e8m0fnu);
+  const at::Tensor& scales = cuda_tensor(a[0], "scales");
+  const int64_t cols = whole(a[1]);
+  as_made(scales, scale_pitch(cols), "scales");
+  return view_rows(scales, a[2], (cols + 31) / 32, at::kFloat8_e8m0fnu);
 }
 
 at::ScalarType dtype_argument(PyObject* o) {
@@ -211,25 +238,35 @@ at::ScalarType dtype_argument(PyObject* o) {
 // (codes, scales, cols, lead, format, dtype)
 PyObject* dequantize(PyObject* const* a) {
   const at::Tensor &codes = cuda_tensor(a[0], "codes"), &scales = cuda_tensor(a[1], "scales");
-  const int64_t cols = whole(a[2]);
+  const int64_t cols = whole(a[2]), format = whole(a[4]);
   const at::ScalarType type = dtype_argument(a[5]);
   const int kind = kind_of(type, "the result");
-  at::Tensor out = empty(sizes_of(a[3], cols), type, codes);
+  as_made(codes, pitch(cols, format), "codes");
+  as_made(scales, scale_pitch(cols), "scales", &codes);
+  at::Tensor out = empty(sizes_of(a[3], cols, codes.size(0)), type, codes);
   const Launch launch(codes.device());
-  check("nes_mx_dequantize", nes_mx_dequantize(codes.data_ptr(), scales.data_ptr<uint8_t>(), out.data_ptr(), kind, codes.size(0), cols,
-                                               int(whole(a[4])), launch.stream));
+  run("nes_mx_dequantize", [&] {
+    return nes_mx_dequantize(codes.data_ptr(), scales.data_ptr<uint8_t>(), out.data_ptr(), kind, codes.size(0), cols, int(format), launch.stream);
+  });
   return THPVariable_Wrap(out);
 }
 
 // (input, its scales or None, its lead or None, its cols, its format, weight codes, weight scales, in_features, weight format, bias, dtype, out)
 PyObject* linear(PyObject* const* a) {
   const bool microscaled = a[1] != Py_None;
-  const int64_t x_format = whole(a[4]), in_features = whole(a[7]);
+  const int64_t x_format = whole(a[4]), in_features = whole(a[7]), w_format = whole(a[8]);
   const at::Tensor &w = cuda_tensor(a[5], "weight codes"), &w_scales = cuda_tensor(a[6], "weight scales");
+  as_made(w, pitch(in_features, w_format), "codes");
+  as_made(w_scales, scale_pitch(in_features), "scales", &w);
   const int64_t out_features = w.size(0);
   std::optional<Rows> plain;
   if (!microscaled) plain.emplace(a[0], "input");
   const at::Tensor& x = microscaled ? cuda_tensor(a[0], "codes") : plain->t;
+  const at::Tensor* x_scales = microscaled ? &cuda_tensor(a[1], "scales") : nullptr;
+  if (microscaled) {
+    as_made(x, pitch(whole(a[3]), x_format), "codes");
+    as_made(*x_scales, scale_pitch(whole(a[3])), "scales", &x);
+  }
   const int64_t rows = microscaled ? x.size(0) : plain->rows, cols = microscaled ? whole(a[3]) : plain->cols;
   const bool has_out = a[11] != Py_None;
   at::ScalarType type = microscaled ? at::kFloat : x.scalar_type();
@@ -254,7 +291,7 @@ PyObject* linear(PyObject* const* a) {
       refuse(PyExc_RuntimeError, "out must be a contiguous %S tensor of %lld elements on %s", dtype_object(type), (long long)(rows * out_features),
              device.str().c_str());
   } else if (microscaled) {
-    y = empty(sizes_of(a[2], out_features), type, x);
+    y = empty(sizes_of(a[2], out_features, rows), type, x);
   } else {
     std::vector<int64_t> sizes(x.sizes().begin(), x.sizes().end());
     sizes.back() = out_features;
@@ -265,10 +302,11 @@ PyObject* linear(PyObject* const* a) {
   at::Tensor scratch;
   const int64_t need = microscaled ? 0 : nes_mx_linear_fwd_scratch_bytes(rows, out_features, in_features, int(x_format));
   if (need) scratch = empty({need}, at::kByte, x);
-  check("nes_mx_linear_fwd",
-        nes_mx_linear_fwd(x.data_ptr(), microscaled ? cuda_tensor(a[1], "scales").data_ptr<uint8_t>() : nullptr, microscaled ? 0 : plain->kind,
-                          int(x_format), w.data_ptr(), w_scales.data_ptr<uint8_t>(), int(whole(a[8])), bias.defined() ? bias.data_ptr<float>() : nullptr,
-                          y.data_ptr(), kind, rows, out_features, in_features, need ? scratch.data_ptr() : nullptr, need, launch.stream));
+  run("nes_mx_linear_fwd", [&] {
+    return nes_mx_linear_fwd(x.data_ptr(), x_scales ? x_scales->data_ptr<uint8_t>() : nullptr, microscaled ? 0 : plain->kind, int(x_format), w.data_ptr(),
+                             w_scales.data_ptr<uint8_t>(), int(w_format), bias.defined() ? bias.data_ptr<float>() : nullptr, y.data_ptr(), kind, rows,
+                             out_features, in_features, need ? scratch.data_ptr() : nullptr, need, launch.stream);
+  });
   return THPVariable_Wrap(y);
 }
 
@@ -311,10 +349,12 @@ PyObject* rms_norm(PyObject* const* a) {
   }
   const Launch launch(device);
   auto data = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
-  check("nes_rms_norm_fwd",
-        nes_rms_norm_fwd(in.data_ptr(), data(residual), data(h), static_cast<const float*>(data(weight)), static_cast<const float*>(data(noise)),
-                         y.data_ptr(), static_cast<uint8_t*>(data(scales)), x.rows, x.cols, members, PyObject_IsTrue(a[5]) == 1 ? 1 : 0, x.kind,
-                         int(format), float(eps), launch.stream));
+  const int antithetic = PyObject_IsTrue(a[5]) == 1 ? 1 : 0;
+  run("nes_rms_norm_fwd", [&] {
+    return nes_rms_norm_fwd(in.data_ptr(), data(residual), data(h), static_cast<const float*>(data(weight)), static_cast<const float*>(data(noise)),
+                            y.data_ptr(), static_cast<uint8_t*>(data(scales)), x.rows, x.cols, members, antithetic, x.kind, int(format), float(eps),
+                            launch.stream);
+  });
   PyObject* first = format ? blocks_tuple(y, scales, x) : THPVariable_Wrap(y);
   if (!h.defined()) return first;
   return Py_BuildValue("(NN)", first, THPVariable_Wrap(h));

@@ -636,7 +636,7 @@ __device__ __forceinline__ void box_by_tma(const CUtensorMap* map, unsigned char
   }
 }
 
-// Order of the tiles: eight feature tiles wide down all tokens, so that the pairs that run together share both operands' rows.
+// Order of the tiles: four feature tiles wide down all tokens, so that the pairs that run together share both operands' rows.
 constexpr int RASTER = 4;
 __device__ __forceinline__ int2 tile_place(int tile, int ftiles, int ttiles) {
   const int column = tile / (RASTER * ttiles), within = tile - column * RASTER * ttiles;
@@ -1075,21 +1075,25 @@ extern "C" int nes_mx_linear_fwd(const void* x, const uint8_t* x_scales, int x_d
   NES_REQUIRE(M <= INT32_MAX / 2 && N <= INT32_MAX / 2 && K <= INT32_MAX / 2, NES_ERR_UNSUPPORTED, "mx_linear_fwd: too large");
   NES_REQUIRE((reinterpret_cast<uintptr_t>(x_scales) & 3u) == 0 && (reinterpret_cast<uintptr_t>(w_scales) & 3u) == 0, NES_ERR_BAD_ARG,
               "mx_linear_fwd: scales must be 4-byte aligned");
+  const int64_t need = x_scales ? 0 : nes_mx_linear_fwd_scratch_bytes(M, N, K, x_format);
+  NES_REQUIRE(need == 0 || (scratch && scratch_bytes >= need && aligned32(scratch)), NES_ERR_SCRATCH,
+              "mx_linear_fwd: scratch needs %lld bytes, 32-byte aligned", (long long)need);
+  const Bytes outputs[] = {{y, M * N * dtype_bytes(y_dtype)}, {need ? scratch : nullptr, need}};
+  const Bytes inputs[] = {{x, M * (x_scales ? code_pitch(K, x_format) : K * dtype_bytes(x_dtype))}, {x_scales, M * scale_pitch(K)},
+                          {w_codes, N * code_pitch(K, w_format)}, {w_scales, N * scale_pitch(K)}, {bias, N * 4}};
+  NES_REQUIRE(!overlap(outputs, inputs), NES_ERR_BAD_ARG, "mx_linear_fwd: the output or the scratch overlaps an input");
   cudaStream_t st = as_stream(stream);
   Product p;
   p.x_scales = x_scales; p.w_scales = w_scales; p.bias = bias; p.y = y; p.x = x; p.whole_rows = 0; p.overlap = false;
   p.M = int(M); p.N = int(N); p.K = int(K); p.groups = int(padded(K) / GROUP); p.y_dtype = y_dtype;
   p.vec_scales = p.groups % CHUNKS == 0 && aligned16(x_scales) && aligned16(w_scales);
-  if (!x_scales && quantises_itself(M, N, K)) {
+  if (!x_scales && need == 0) {
     p.whole_rows = aligned16(x) && (K * dtype_bytes(x_dtype)) % 16 == 0;
     if (x_format == NES_MXFP4) return launch_raw<NES_MXFP4, NES_MXFP4>(p, x_dtype, w_codes, st);
     if (w_format == NES_MXFP4) return launch_raw<NES_MXFP8, NES_MXFP4>(p, x_dtype, w_codes, st);
     return launch_raw<NES_MXFP8, NES_MXFP8>(p, x_dtype, w_codes, st);
   }
-  if (!x_scales) {
-    const int64_t need = nes_mx_linear_fwd_scratch_bytes(M, N, K, x_format);
-    NES_REQUIRE(scratch && scratch_bytes >= need && aligned32(scratch), NES_ERR_SCRATCH,
-                "mx_linear_fwd: scratch needs %lld bytes, 32-byte aligned", (long long)need);
+  if (need) {
     uint8_t* codes = static_cast<uint8_t*>(scratch);
     uint8_t* scales = codes + align256(M * code_pitch(K, x_format));
     const int rc = nes_mx_quantize(x, x_dtype, codes, scales, M, K, x_format, stream);

@@ -412,6 +412,10 @@ extern "C" int nes_rms_norm_fwd(const void* x, const void* residual, void* resid
   NES_REQUIRE(rows <= LARGEST_EXTENT && cols <= LARGEST_EXTENT, NES_ERR_UNSUPPORTED, "rms_norm_fwd: too large");
   NES_REQUIRE(aligned16(x) && aligned16(residual) && aligned16(residual_out) && aligned16(gain) && aligned16(noise) && aligned16(y),
               NES_ERR_BAD_ARG, "rms_norm_fwd: tensors must be 16-byte aligned");
+  const int64_t plain = rows * cols * dtype_bytes(dtype);
+  const Bytes outputs[] = {{y, format ? rows * code_pitch(cols, format) : plain}, {format ? y_scales : nullptr, rows * scale_pitch(cols)}, {residual_out, plain}};
+  const Bytes inputs[] = {{x, plain}, {residual, plain}, {gain, cols * 4}, {noise, members * cols * 4}};
+  NES_REQUIRE(!overlap(outputs, inputs), NES_ERR_BAD_ARG, "rms_norm_fwd: an output overlaps an input");
   NormArgs a;
   a.x = x; a.residual = residual; a.h = residual_out; a.gain = gain; a.noise = noise; a.y = y; a.scales = y_scales;
   a.rows = rows; a.cols = cols; a.members = members > 0 ? members : 1; a.antithetic = antithetic;

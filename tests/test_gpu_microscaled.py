@@ -361,3 +361,40 @@ def test_refusals():
         ms.linear(x, q, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="CUDA"):
         ms.linear([1.0], q)
+
+
+def test_refusals_of_blocks_changed_since():
+    """The object's tensors can be replaced; what no longer fits together is refused where it is used."""
+    ms = _ms()
+    x = torch.ones(4, 256, device="cuda")
+    w = ms.quantize(torch.ones(8, 256, device="cuda"))
+    for form in ("mxfp4", "mxfp8"):
+        good = ms.quantize(x, form)
+        more, narrow = ms.quantize(torch.ones(6, 256, device="cuda"), form), ms.quantize(x[:, :128], form)
+        for codes, scales in ((more.codes, more.scales), (more.codes, good.scales), (narrow.codes, good.scales), (good.codes, narrow.scales),
+                              (good.codes.int(), good.scales), (good.codes, good.scales.t().contiguous().t())):
+            q = ms.quantize(x, form)
+            q.codes, q.scales = codes, scales
+            for call in (q.dequantize, lambda: ms.linear(q, w)):
+                with pytest.raises(RuntimeError, match="microscaled tensor must|leading"):
+                    call()
+            if codes is not good.codes:
+                with pytest.raises(RuntimeError, match="microscaled tensor must|leading"):
+                    q.elements()
+        w2 = ms.quantize(torch.ones(8, 256, device="cuda"))
+        w2.scales = good.scales
+        with pytest.raises(RuntimeError, match="microscaled tensor must"):
+            ms.linear(x, w2)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_results_over_inputs_are_refused(rows):
+    ms = _ms()
+    C = pytest.importorskip("nesgpu_b200._cabi")
+    x = torch.ones(rows, 256, device="cuda")
+    w = ms.quantize(torch.ones(256, 256, device="cuda"))
+    with pytest.raises(C.NesError, match="overlap"):
+        ms.linear(x, w, out=x)
+    both = torch.ones(2 * rows, 256, device="cuda")
+    y = ms.linear(both[:rows], w, out=both[rows:])              # next to one another
+    assert torch.equal(y, torch.full_like(y, 256.0))

@@ -342,3 +342,71 @@ def test_offsets_beyond_32_bits():
     y = ms.linear(a, b, dtype=torch.bfloat16)
     want = ms.linear(a, ms.quantize(_rows(cols, 64, 5)[-8:].contiguous()), dtype=torch.bfloat16)
     assert torch.equal(y[:, -8:], want)
+
+
+def test_graph_with_copies_fills_and_branches():
+    """Captured calls that follow a copy, a fill, a join of two branches or another call: each waits for what it reads."""
+    from nesgpu_b200 import microscaling as ms
+    w = ms.quantize(_rows(512, 512, 1))
+    given = _rows(600, 512, 2, torch.bfloat16)
+    static, doubled = torch.empty_like(given), torch.empty_like(given)
+    side = torch.cuda.Stream()
+
+    def call():
+        static.copy_(given)
+        q, h = ms.rms_norm(static, residual=static, output="mxfp8")
+        doubled.copy_(h)
+        y = ms.linear(doubled, w, activations="mxfp4")
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            s = ms.linear(q, w, dtype=torch.bfloat16)
+            back = q.dequantize(torch.bfloat16)
+        z = ms.linear(y, w, dtype=torch.bfloat16)
+        torch.cuda.current_stream().wait_stream(side)
+        total = ms.rms_norm(z, residual=s)[1]
+        z.zero_()
+        return total, back, ms.rms_norm(back), ms.linear(z, w)
+
+    want = [t.clone() for t in call()]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    for i in range(4):
+        given.copy_(torch.roll(given, 1 if i % 2 == 0 else -1, 0))
+        for _ in range(3):
+            graph.replay()
+        ref = [torch.roll(t, 1, 0) if i % 2 == 0 else t for t in want]
+        torch.cuda.synchronize()
+        for a, b in zip(got, ref):
+            assert torch.equal(a, b)
+
+
+def test_calls_from_several_threads():
+    import threading
+    from nesgpu_b200 import microscaling as ms
+    w = ms.quantize(_rows(256, 512, 1))
+    xs = [_rows(rows, 512, 30 + rows, torch.bfloat16) for rows in (1, 40, 300)]
+
+    def chain(x):
+        q, h = ms.rms_norm(x, residual=x, output="mxfp8")
+        return ms.linear(q, w, dtype=torch.bfloat16), ms.linear(h, w, activations="mxfp4")
+
+    want = [[t.clone() for t in chain(x)] for x in xs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(x, ref, stream):
+        with torch.cuda.stream(stream):
+            for _ in range(50):
+                got = chain(x)
+                if not all(torch.equal(a, b) for a, b in zip(got, ref)):
+                    wrong.append(x.shape)
+
+    streams = [torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.current_stream()] * 2
+    threads = [threading.Thread(target=work, args=(xs[i % 3], want[i % 3], s)) for i, s in enumerate(streams)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong

@@ -93,3 +93,25 @@ def test_norm_layer_state_follows_the_other_layers():
         base.PerturbedRMSNorm(8, 2, options={"direct": True})
     pm = base.PerturbedModel(torch.nn.Sequential(layer, base.PerturbedLinear(48, 5, 6, options={"tc": "mxfp4"})), 6)
     assert len(pm.perturbed_layers) == 2
+
+
+def test_outputs_over_inputs_are_refused():
+    """Before anything reaches a device, so the addresses are made up."""
+    from nesgpu_b200 import _cabi as C
+    f32, mx4, mx8 = 0, 4, 8
+    a, b, c, d, e = (n << 40 for n in range(1, 6))
+    over = a + 4 * 128 * 4 - 16                      # the last bytes of a (4, 128) fp32 matrix at a
+    calls = [("nes_mx_quantize", (a, f32, over, b, 4, 128, mx8, 0)),
+             ("nes_mx_quantize", (a, f32, b, over, 4, 128, mx8, 0)),
+             ("nes_mx_dequantize", (a, b, a + 4 * 128 - 16, f32, 4, 128, mx8, 0)),
+             ("nes_mx_dequantize", (a, b, b, f32, 4, 128, mx8, 0)),
+             ("nes_mx_elements", (a, a + 4 * 64 - 16, 4, 128, 0)),
+             ("nes_mx_linear_fwd", (a, None, f32, mx8, b, c, mx4, None, over, f32, 4, 64, 128, None, 0, 0)),
+             ("nes_mx_linear_fwd", (a, d, f32, mx8, b, c, mx4, None, d, f32, 4, 64, 128, None, 0, 0)),
+             ("nes_mx_linear_fwd", (a, d, f32, mx8, b, c, mx4, e, e + 64 * 4 - 4, f32, 4, 64, 128, None, 0, 0)),
+             ("nes_rms_norm_fwd", (a, None, None, None, None, a, None, 4, 128, 0, 0, f32, 0, 1e-6, 0)),
+             ("nes_rms_norm_fwd", (a, b, b, None, None, c, None, 4, 128, 0, 0, f32, 0, 1e-6, 0)),
+             ("nes_rms_norm_fwd", (a, None, None, b, c, c, d, 4, 128, 2, 0, f32, mx8, 1e-6, 0))]
+    for name, args in calls:
+        with pytest.raises(C.NesError, match="overlap"):
+            C.call(name, *args)
