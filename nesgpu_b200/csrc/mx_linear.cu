@@ -12,8 +12,8 @@
 //     column per 32 rows and 128 elements, repeated in each quarter of the lanes.  Four warps load them for STEP = 512
 //     elements of K at a time, 16 bytes per row and thread, transpose them on the way into shared memory, and tcgen05.cp
 //     brings them over in the order of the products.
-//   * Plain activations are quantised into scratch first, under which the product starts and loads its first weights; a few tokens are quantised by the product itself, every CTA
-//     its own part of K straight into the operand's place in shared memory.
+//   * Plain activations are quantised into scratch first, under which the product starts and loads its first weights; a few
+//     tokens are quantised by the product itself, every CTA its own part of K straight into the operand's place in shared memory.
 //   * Few output tiles: a cluster of up to eight CTAs splits K and adds its partial tiles in a fixed order through
 //     distributed shared memory.
 //
@@ -52,9 +52,9 @@ struct ProductMaps { CUtensorMap w, x; };
 constexpr int RAW_STEPS = 8;                 // steps of K whose quantised activations a CTA keeps
 
 // PUSH: partial results go straight to the CTA that adds them up, which has room for them beside its stages (one barrier of the
-// cluster and local reads: 1 token of 4096x4096 8.0 -> 7.2 us).  Otherwise they lie in the stages until they are fetched: of
-// 128 tokens the room costs two of six stages, which pays from four CTAs to a tile on (128 tokens, 4096x1024: 10.3 -> 7.7 us;
-// 1024x1024 in halves: 8.2 -> 9.0 us).
+// cluster and local reads: 1 token of 4096x4096 6.6 -> 6.0 us).  Otherwise they lie in the stages until they are fetched: of
+// 128 tokens the room costs two of six stages, which pays from four CTAs to a tile on (128 tokens, 4096x1024: 9.2 -> 7.0 us;
+// 1024x1024 in halves: 6.9 -> 8.0 us).
 // RAW: the activations of all the CTA's stages lie behind the stages, which hold weights only; so do their scales
 template <int TOKENS, bool RAW, int STAGES_PER_STEP, bool PUSH>
 struct Layout {
@@ -908,8 +908,8 @@ static int code_map(CUtensorMap* map, const void* base, int64_t rows, int64_t gr
 }
 
 // CTAs that share a tile's K: as many as fill the SMs once, each with a step of its own at least.  Clusters of eight do not
-// pack onto all SMs: 16 of them take two waves (1 token, 16384x2048: 15.9 us against 11.7 us in fours), 4 to 8 are faster than
-// fours (8192x512: 6.9 us against 7.9 us).
+// pack onto all SMs: 16 of them take two waves (1 token, 16384x2048: 14.0 us against 10.7 us in fours), 4 to 8 are faster than
+// fours (8192x512: 5.4 us against 7.3 us).
 static int choose_splits(int64_t tiles, int steps) {
   int splits = 1;
   while (splits < 8 && splits * 2 <= steps && tiles * splits * 2 <= (splits == 4 ? sm_count() / 2 : sm_count())) splits *= 2;
@@ -1010,13 +1010,14 @@ static int launch_single(const Product& p, const void* x, const void* w, cudaStr
 }
 
 // Whether the product quantises its plain activations itself: few tokens, and a part of K per CTA that fits its shared memory.
-// Every feature tile's CTAs do so before their first product, at about 0.23 us per 8 elements of a thread (of 128); a
-// launch of its own costs the device 1.8 us and the host 4 us (1 token of 4096x4096: 7.9 us, else 8.6; 16 tokens: 11.3 and 9.0).
+// Every feature tile's CTAs do so before their first product, at about 0.23 us per 8 elements of a thread (of 128); a launch
+// of its own, under which the product starts, costs the device 0.9 us and the host 2.8 us.  4096x4096, 4 bits: 1 token 5.7 us,
+// with a launch of its own 6.6; 4 tokens 6.4 and 6.6; 8 tokens 7.4 and 6.7; 16 tokens 9.2 and 6.7.
 static bool quantises_itself(int64_t M, int64_t N, int64_t K) {
   if (M > 16) return false;
   const int steps = int(ceil_div<int64_t>(K, STEP));
   const int64_t mine = ceil_div<int64_t>(steps, choose_splits(ceil_div<int64_t>(N, FEATURES), steps));
-  return mine <= RAW_STEPS && M * mine * STEP <= 16 * 128 * UNIT;
+  return mine <= RAW_STEPS && M * mine * STEP <= 6 * 128 * UNIT;
 }
 
 template <int XF, int WF>
@@ -1033,8 +1034,8 @@ static int launch_tokens(const Product& p, const void* x, const void* w, cudaStr
   if (p.M <= 64) return launch_single<XF, WF, 64>(p, x, w, st);
   // Single CTAs on 128 x 128 tiles, or pairs on 256 x 256: what either takes in ns, from its waves over the SMs.  Measured
   // with 8-bit activations: a wave of either kind takes 2.5 us per 1024 of K, a wave of single CTAs 4.5 us besides (its
-  // epilogue runs under nothing), the pairs 8 us in all.  512x4096x4096: 14.9 us single, 20.7 us in pairs; 1024x4096x4096:
-  // 28.0 and 21.8 us; 4-bit activations take 1.5 us per 1024 of K.
+  // epilogue runs under nothing), the pairs 8 us in all.  512x4096x4096: 14.8 us single, 18.8 us in pairs; 1024x4096x4096:
+  // 28.5 and 20.4 us; 4-bit activations take 1.5 us per 1024 of K.
   if (p.M > 128) {
     const int64_t sms = sm_count(), k = int64_t(p.groups) * (XF == NES_MXFP4 ? 190 : 310);
     const int64_t single = ceil_div<int64_t>(p.M, 128) * ceil_div(p.N, FEATURES), pairs = ceil_div<int64_t>(p.M, PAIR_TOKENS) * ceil_div(p.N, PAIR_FEATURES);
