@@ -99,7 +99,7 @@ def linear(input, weight, bias=None, activations="mxfp8", dtype=None, out=None):
 
     Products are accumulated in fp32 and rounded once to ``dtype`` (default: the type of a plain input, float32 for a
     microscaled one).  8-bit activations take weights of either format, 4-bit activations 4-bit weights.  ``out``
-    receives the result if given (contiguous, of the result's type and number of elements)."""
+    receives the result if given (contiguous, of the result's type and number of elements, over none of the operands)."""
     if not isinstance(weight, MicroscaledTensor) or len(weight._lead) != 1:
         raise RuntimeError("weight must be a MicroscaledTensor of (out_features, in_features)")
     if isinstance(input, MicroscaledTensor):
@@ -116,7 +116,8 @@ def rms_norm(input, weight=None, eps=1e-6, residual=None, noise=None, antithetic
     call returns ``(y, h)``, ``h`` rounded to that type (``y`` is computed from the unrounded sum).  ``noise``
     ``(members, cols)`` float32 adds ``noise[d]`` to the gain of the rows ``r * members + d`` (its negative for the
     second half of the repeats with ``antithetic``).  ``output`` is None for a ``y`` of the input's type, or
-    ``"mxfp8"`` / ``"mxfp4"`` for a :class:`MicroscaledTensor`."""
+    ``"mxfp8"`` / ``"mxfp4"`` for a :class:`MicroscaledTensor`.  Squares are summed in fp32: a row with magnitudes above
+    1e19 has an infinite mean and is normalised to zeros."""
     if output is None or output == getattr(input, "dtype", None):
         return _host.rms_norm(input, weight, eps, residual, noise, antithetic, 0)
     got = _host.rms_norm(input, weight, eps, residual, noise, antithetic, _format(output, "output"))
