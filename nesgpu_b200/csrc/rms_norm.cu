@@ -18,6 +18,9 @@
 namespace nes {
 namespace mx {
 
+constexpr int MOST_WARPS = 17;                   // of a row: 16384 columns, and one unit more where rows are shifted
+constexpr int WARP_ROWS = 4;                     // rows of a block whose warps take one each
+
 struct NormArgs {
   const void* x;
   const void* residual;
@@ -28,6 +31,7 @@ struct NormArgs {
   uint8_t* scales;
   int64_t rows, cols, members;
   int antithetic;
+  uint32_t minus;                                  // -1
   float eps;
   double inv_cols;
 };
@@ -40,15 +44,36 @@ __device__ __forceinline__ float2 rsqrt_pair(double v) {
   return make_float2(r, 0.5f * r * float(1.0 - v * (double(r) * double(r))));
 }
 
-// h * (r.x + r.y) * (g + gl) with the rounding errors carried along: s + se is the row's scale times the gain to 48 bits.
-// SHARP leaves the fp32 result rounded to odd (cut off, lowest bit set), so that a rounding to fewer bits afterwards
-// decides as it would on the unrounded value; a value exactly on a border does not occur except for a zero.  Otherwise
-// the result is rounded to nearest.
-template <bool SHARP>
+// h * (r.x + r.y) * (g + gl) rounded once: s + se is the row's scale times the gain to 43 bits at least.
+__device__ __forceinline__ float scaled(float h, float2 r, float g) {
+  const float s = r.x * g, se = fmaf(r.y, g, fmaf(r.x, g, -s));
+  return fmaf(h, s, h * se);
+}
 __device__ __forceinline__ float scaled(float h, float2 r, float g, float gl) {
   const float s = r.x * g, se = fmaf(r.x, gl, fmaf(r.y, g, fmaf(r.x, g, -s)));
-  if (SHARP) return __uint_as_float(__float_as_uint(__fmaf_rz(h, s, h * se)) | 1u);
   return fmaf(h, s, h * se);
+}
+
+// A quantised output rounds y a second time.  The first rounding, to fp32, decides that one only where it ends on a border of the second:
+// a number of at most five bits, whether it lies between two codes or begins the binade of a block's scale.  The low 19 bits of such a
+// y are zero, and y and the exact value are told apart in 64 bits: y stays if they are equal (the border's own rule holds), else
+// it becomes its neighbour on the exact value's side.  y times the root is exact where the root is a number of few bits, without
+// which no value but zero can lie on a border.  One y in half a million is such a one, zeros aside: what the kernels do for them
+// is to gather every y's lowest set bit; a unit in which one of these is found is worked out a second time (settle_units).
+constexpr uint32_t BORDER_BITS = 0x7ff80000u;          // of a lowest set bit; a zero has none, or the sign
+// minus: -1, which the compiler does not know of: a product, unlike a negation, leaves the ALU pipe free
+__device__ __forceinline__ uint32_t lowest_bits(const float (&y)[UNIT], uint32_t minus) {
+  uint32_t all = 0;
+#pragma unroll
+  for (int i = 0; i < UNIT; ++i) all |= __float_as_uint(y[i]) & (minus * __float_as_uint(y[i]));
+  return all;
+}
+__device__ __forceinline__ float settled(float y, float h, float g, float gl, double root) {
+  const uint32_t bits = __float_as_uint(y);
+  if (((bits & (0u - bits)) & BORDER_BITS) == 0u) return y;
+  const double past = fma(-double(y), root, double(h) * (double(g) + double(gl)));
+  const int step = past > 0.0 ? 1 : past < 0.0 ? -1 : 0;                  // 0 also for a NaN: an infinite y of an infinite h
+  return __uint_as_float(bits + uint32_t(y < 0.f ? -step : step));
 }
 
 // A row's places in memory.
@@ -206,9 +231,16 @@ __device__ __forceinline__ void load_h(const NormArgs& a, const Row<T>& row, int
   }
 }
 
-// y of the unit at column c; all lanes of a warp call it.  A quantised output is stored from units of whole columns 8 i.
-template <typename T, int OUT, RowAccess ACCESS>
-__device__ __forceinline__ void emit(const NormArgs& a, const Row<T>& row, int64_t index, int c, const float (&h)[UNIT], float2 r) {
+// The sum of squares of this warp's row, kept for settle_units outside the registers.
+__device__ __forceinline__ volatile double& sum_of_row() {
+  __shared__ double sums[MOST_WARPS];
+  return sums[threadIdx.x >> 5];
+}
+
+// y of the unit at column c; all lanes of a warp call it.  A quantised output is stored from units of whole columns 8 i, and its
+// values' lowest bits are added to `lowest`.  SETTLE: values at a border are settled, with the root of mean + eps.
+template <typename T, int OUT, RowAccess ACCESS, bool SETTLE = false>
+__device__ __forceinline__ void emit(const NormArgs& a, const Row<T>& row, int64_t index, int c, const float (&h)[UNIT], float2 r, double root, uint32_t& lowest) {
   constexpr bool MOVED = ACCESS == SHIFTED && OUT != 0;
   const int cols = int(a.cols);
   float g[UNIT], y[UNIT];
@@ -225,12 +257,17 @@ __device__ __forceinline__ void emit(const NormArgs& a, const Row<T>& row, int64
     for (int i = 0; i < UNIT; ++i) {
       // gain + noise as a sum and what it rounds away
       const float e = row.sign * n[i], sum = g[i] + e, back = sum - g[i], lost = (g[i] - (sum - back)) + (e - back);
-      y[i] = scaled<OUT != 0>(h[i], r, sum, OUT != 0 ? lost : 0.f);
+      y[i] = OUT != 0 ? scaled(h[i], r, sum, lost) : scaled(h[i], r, sum);
+      if (SETTLE) y[i] = settled(y[i], h[i], sum, lost, root);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < UNIT; ++i) y[i] = scaled<OUT != 0>(h[i], r, g[i], 0.f);
+    for (int i = 0; i < UNIT; ++i) {
+      y[i] = scaled(h[i], r, g[i]);
+      if (SETTLE) y[i] = settled(y[i], h[i], g[i], 0.f, root);
+    }
   }
+  if (OUT != 0 && !SETTLE) lowest |= lowest_bits(y, a.minus);
   if (OUT == 0) {
     store_at<ACCESS>(row.y, c, cols, values_raw(y, T()));
     return;
@@ -292,11 +329,61 @@ __device__ __forceinline__ float square_sum(const float (&v)[UNIT]) {
   return q;
 }
 
-constexpr int MOST_WARPS = 17;                   // of a row: 16384 columns, and one unit more where rows are shifted
-constexpr int WARP_ROWS = 4;                     // rows of a block whose warps take one each
+// 1 / sqrt(mean + eps)
+template <bool QUANTISED>
+__device__ __forceinline__ float2 row_scale(const NormArgs& a, double sum) {
+  if (QUANTISED) sum_of_row() = sum;                                      // every lane the same: each reads what it wrote itself
+  return rsqrt_pair(sum * a.inv_cols + double(a.eps));
+}
+
+// This lane's unit of 32 neighbouring ones once more, with values at a border settled; x and the residual are read again.  All lanes of
+// the warp call it.
+template <typename T, int OUT, RowAccess ACCESS>
+__device__ __forceinline__ void settle_unit(const NormArgs& a, int64_t index, int c, float2 r) {
+  const Row<T> row(a, index);
+  const double root = sqrt(sum_of_row() / double(a.cols) + double(a.eps));
+  uint32_t lowest = 0;
+  float h[UNIT];
+  if (ACCESS == SHIFTED) {
+    float from[UNIT], next[UNIT];
+    load_h<T, ACCESS>(a, row, c - row.shift, from);
+    load_h<T, ACCESS>(a, row, c - row.shift + 32 * UNIT, next);
+    unshift(from, next, row.shift, h);
+  } else {
+    load_h<T, ACCESS>(a, row, c, h);
+  }
+  emit<T, OUT, ACCESS, true>(a, row, index, c, h, r, root, lowest);
+}
+template <typename T, int OUT, RowAccess ACCESS>
+__device__ __noinline__ void settle_unit_call(const NormArgs a, int64_t index, int c, float2 r) { settle_unit<T, OUT, ACCESS>(a, index, c, r); }
+
+// `units`: a bit for every unit, `step` columns apart, in which a lane has a value at a border.  CALL keeps the kernel's registers
+// free of what a unit takes here.
+template <typename T, int OUT, RowAccess ACCESS, bool CALL>
+__device__ __forceinline__ void settle_units(const NormArgs& a, int64_t index, int first, int step, uint32_t units, float2 r) {
+  units = __reduce_or_sync(0xffffffffu, units);
+#pragma unroll 1
+  for (; units; units &= units - 1) {
+    const int c = first + (__ffs(units) - 1) * step;
+    if (CALL) settle_unit_call<T, OUT, ACCESS>(a, index, c, r);
+    else settle_unit<T, OUT, ACCESS>(a, index, c, r);
+  }
+}
+
+// Whether a kernel calls for the settling, and the blocks that an SM holds at least (0: as many as the registers allow).  Kernels of few
+// units would hold fewer blocks with it in their registers.  Time relative to kernels without any of it: 65536x256 fp32 1.02 with a call
+// and 12 blocks, 1.06 without the call; 16384x1023 fp32 1.12 with a call, 1.02 without; 8192x4096 bf16 1.01 and 0.97.
+constexpr bool calls_settle(int bytes, int units, RowAccess access, bool block_row) {
+  return !block_row && (units < 4 || (access == SHIFTED && bytes == 2));
+}
+constexpr int blocks_held(int out, int bytes, int units, RowAccess access, bool block_row) {
+  if (out == 0 || block_row) return 0;
+  if (access == SHIFTED) return units == 1 ? 10 : units == 2 ? 8 : bytes == 4 ? 6 : 0;
+  return units == 1 ? 12 : units == 2 ? 10 : 7;
+}
 
 template <typename T, int OUT, int UNITS, RowAccess ACCESS, bool BLOCK_ROW>
-__global__ void __launch_bounds__(BLOCK_ROW ? MOST_WARPS * 32 : WARP_ROWS * 32) rms_norm_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(BLOCK_ROW ? MOST_WARPS * 32 : WARP_ROWS * 32, blocks_held(OUT, sizeof(T), UNITS, ACCESS, BLOCK_ROW)) rms_norm_kernel(const NormArgs a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t index = BLOCK_ROW ? int64_t(blockIdx.x) : int64_t(blockIdx.x) * WARP_ROWS + warp;
   take_turn();
@@ -317,23 +404,27 @@ __global__ void __launch_bounds__(BLOCK_ROW ? MOST_WARPS * 32 : WARP_ROWS * 32) 
 #pragma unroll
     for (int u = 0; u < UNITS; ++u) if (is_full(ACCESS) || base + u * 32 * UNIT < int(a.cols) + shift) store_at<ACCESS>(row.h, first - shift + u * 32 * UNIT, int(a.cols), values_raw(v[u], T()));
   }
-  const float2 r = rsqrt_pair(row_sum<BLOCK_ROW>(s) * a.inv_cols + double(a.eps));
+  const float2 r = row_scale<OUT != 0>(a, row_sum<BLOCK_ROW>(s));
+  uint32_t units = 0;
 #pragma unroll
   for (int u = 0; u < UNITS; ++u) {
+    uint32_t lowest = 0;
     if (!is_full(ACCESS) && base + u * 32 * UNIT >= end) break;         // nothing of the row in this warp's unit u
     if (MOVE) {
       float h[UNIT];
       unshift(v[u], v[u + 1], shift, h);
-      emit<T, OUT, ACCESS>(a, row, index, first + u * 32 * UNIT, h, r);
+      emit<T, OUT, ACCESS>(a, row, index, first + u * 32 * UNIT, h, r, 0.0, lowest);
     } else {
-      emit<T, OUT, ACCESS>(a, row, index, first - shift + u * 32 * UNIT, v[u], r);
+      emit<T, OUT, ACCESS>(a, row, index, first - shift + u * 32 * UNIT, v[u], r, 0.0, lowest);
     }
+    if (lowest & BORDER_BITS) units |= 1u << u;
   }
+  if (OUT != 0) settle_units<T, OUT, ACCESS, calls_settle(sizeof(T), UNITS, ACCESS, BLOCK_ROW)>(a, index, first, 32 * UNIT, units, r);
 }
 
 // Rows of any length: the sum of squares in one loop over the row, the outputs in a second one.
 template <typename T, int OUT, RowAccess ACCESS>
-__global__ void __launch_bounds__(512) rms_norm_long_kernel(const NormArgs a) {
+__global__ void __launch_bounds__(512, OUT == 0 ? 0 : ACCESS == ANY ? 3 : 4) rms_norm_long_kernel(const NormArgs a) {
   const int64_t index = blockIdx.x;
   take_turn();
   const Row<T> row(a, index);
@@ -346,13 +437,19 @@ __global__ void __launch_bounds__(512) rms_norm_long_kernel(const NormArgs a) {
     s += square_sum(v);
     if (row.h) store_at<ACCESS>(row.h, c, int(a.cols), values_raw(v, T()));
   }
-  const float2 r = rsqrt_pair(row_sum<true>(s) * a.inv_cols + double(a.eps));
-  for (int c0 = 0; c0 < end; c0 += step) {
+  const float2 r = row_scale<OUT != 0>(a, row_sum<true>(s));
+  uint32_t units = 0;                                             // a bit stands for every 32nd unit
+  int u = 0;
+  for (int c0 = 0; c0 < end; c0 += step, ++u) {
     float v[UNIT];
+    uint32_t lowest = 0;
     const int c = c0 + threadIdx.x * UNIT;
     load_h<T, ACCESS>(a, row, c, v);
-    emit<T, OUT, ACCESS>(a, row, index, c, v, r);
+    emit<T, OUT, ACCESS>(a, row, index, c, v, r, 0.0, lowest);
+    if (lowest & BORDER_BITS) units |= 1u << (u & 31);
   }
+  if constexpr (OUT != 0)
+    for (int c0 = threadIdx.x * UNIT; c0 - int(threadIdx.x) * UNIT < end; c0 += 32 * step) settle_units<T, OUT, ACCESS, true>(a, index, c0, step, units, r);
 }
 
 // Four units per lane keep the most loads in flight where there are rows enough for all SMs; a few rows are spread over more
@@ -419,7 +516,7 @@ extern "C" int nes_rms_norm_fwd(const void* x, const void* residual, void* resid
   NormArgs a;
   a.x = x; a.residual = residual; a.h = residual_out; a.gain = gain; a.noise = noise; a.y = y; a.scales = y_scales;
   a.rows = rows; a.cols = cols; a.members = members > 0 ? members : 1; a.antithetic = antithetic;
-  a.eps = eps; a.inv_cols = 1.0 / double(cols);
+  a.minus = 0xffffffffu; a.eps = eps; a.inv_cols = 1.0 / double(cols);
   cudaStream_t st = as_stream(stream);
   if (dtype == NES_F32) launch_norm_out<float>(a, format, st);
   else if (dtype == NES_BF16) launch_norm_out<__nv_bfloat16>(a, format, st);
