@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/DynamicTypes.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstdarg>
@@ -369,10 +370,8 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
   try {
     return F(args);
   } catch (const Raised&) {
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
   } catch (...) {
-    PyErr_SetString(PyExc_RuntimeError, "nesgpu_b200: unknown C++ exception");
+    torch::translate_exception_to_python(std::current_exception());      // torch.OutOfMemoryError and the like, as PyTorch's own calls raise
   }
   return nullptr;
 }
