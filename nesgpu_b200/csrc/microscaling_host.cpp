@@ -129,6 +129,12 @@ void run(const char* name, F&& call) {
   throw Raised();
 }
 
+bool truth(PyObject* o) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) throw Raised();
+  return v == 1;
+}
+
 int64_t whole(PyObject* o) {
   const long long v = PyLong_AsLongLong(o);
   if (v == -1 && PyErr_Occurred()) throw Raised();
@@ -317,6 +323,7 @@ PyObject* rms_norm(PyObject* const* a) {
   const double eps = PyFloat_AsDouble(a[2]);
   if (eps == -1.0 && PyErr_Occurred()) throw Raised();
   if (!(eps >= 0)) refuse(PyExc_RuntimeError, "eps must not be negative, got %R", a[2]);
+  const bool antithetic = truth(a[5]);
   const at::Device device = x.t.device();
   const int64_t format = whole(a[6]);
   at::Tensor in = aligned(x.t), residual, h, weight, noise;
@@ -350,7 +357,6 @@ PyObject* rms_norm(PyObject* const* a) {
   }
   const Launch launch(device);
   auto data = [](const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
-  const int antithetic = PyObject_IsTrue(a[5]) == 1 ? 1 : 0;
   run("nes_rms_norm_fwd", [&] {
     return nes_rms_norm_fwd(in.data_ptr(), data(residual), data(h), static_cast<const float*>(data(weight)), static_cast<const float*>(data(noise)),
                             y.data_ptr(), static_cast<uint8_t*>(data(scales)), x.rows, x.cols, members, antithetic, x.kind, int(format), float(eps),

@@ -22,3 +22,17 @@ def test_a_failed_allocation_is_out_of_memory():
     y = ms.linear(x[:3], many)                            # and the next call works
     assert y.shape == (3, 1 << 21) and bool((y == 1).all())
 
+
+def test_an_argument_without_a_truth_value_is_refused():
+    from nesgpu_b200 import microscaling as ms
+    x = torch.ones(4, 64, device="cuda")
+    with pytest.raises(RuntimeError, match="ambiguous"):
+        ms.rms_norm(x, noise=torch.zeros(2, 64, device="cuda"), antithetic=torch.ones(2))
+
+    class Without:
+        def __bool__(self):
+            raise KeyError("no truth value")
+
+    with pytest.raises(KeyError, match="no truth value"):
+        ms.rms_norm(x, antithetic=Without())
+    assert bool((ms.rms_norm(x, eps=0.0) == 1).all())
