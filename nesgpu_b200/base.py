@@ -419,6 +419,16 @@ _MX_MODES = {"mxfp4": ("mxfp4", "mxfp4"), "mxfp8": ("mxfp8", "mxfp8"), "mxfp8_mx
 class _LinearMixin:
     MICROSCALED = False        # whether the layer's base product has the microscaled modes
 
+    def _microscaled_mode(self):
+        """The microscaled ``options["tc"]`` of the layer, or None.  Direct storage has no base product to run in it: the
+        population would be evaluated in fp32 and the unperturbed layer in blocks, so the two are refused together."""
+        mode = self.options.get("tc")
+        if not self.MICROSCALED or mode not in _MX_MODES:
+            return None
+        if self.options.get("direct"):
+            raise NotImplementedError('options["tc"] = "%s" is not defined for direct storage' % mode)
+        return mode
+
     def _microscaled_base(self, input, out=None):
         """``x W^T + b`` with both operands in the blocks of ``options["tc"]`` (``"mxfp4"``, ``"mxfp8"`` or
         ``"mxfp8_mxfp4"``: 8-bit activations, 4-bit weights).  The weight is quantised as it is at this call."""
@@ -455,7 +465,7 @@ class _LinearMixin:
 
     def _flatten_rows(self, input):
         if isinstance(input, microscaling.MicroscaledTensor):
-            if not self.MICROSCALED or self.options.get("tc") not in _MX_MODES:
+            if not self._microscaled_mode():
                 raise NotImplementedError('microscaled inputs need a layer with options["tc"] = "mxfp4", "mxfp8" or '
                                           '"mxfp8_mxfp4"')
             input = input.dequantize()
@@ -465,7 +475,7 @@ class _LinearMixin:
         return x.reshape(-1, self.in_features), x.shape[:-1]
 
     def _plain_forward(self, input):
-        if self.MICROSCALED and self.options.get("tc") in _MX_MODES:
+        if self._microscaled_mode():
             mx = isinstance(input, microscaling.MicroscaledTensor)
             return self._microscaled_base(input if mx else C.require_cuda(input, "input", _F32))
         x, lead = self._flatten_rows(input)
@@ -484,8 +494,10 @@ class PerturbedLinear(nn.Linear, _LinearMixin, Perturbed):
     def __init__(self, in_features, out_features, directions, bias=True, antithetic=False, options={}):
         nn.Linear.__init__(self, in_features, out_features, bias)
         Perturbed.__init__(self, directions, antithetic, options)
+        self._microscaled_mode()
 
     def forward(self, input):
+        self._microscaled_mode()
         if not self.perturbed_flag:
             return self._plain_forward(input)
         x, lead = self._flatten_rows(input)

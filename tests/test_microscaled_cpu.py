@@ -115,3 +115,18 @@ def test_outputs_over_inputs_are_refused():
     for name, args in calls:
         with pytest.raises(C.NesError, match="overlap"):
             C.call(name, *args)
+
+
+@pytest.mark.parametrize("mode", ["mxfp4", "mxfp8", "mxfp8_mxfp4"])
+def test_direct_storage_has_no_microscaled_mode(mode):
+    """The population forward would run in fp32, the unperturbed one of the same layer in blocks."""
+    from nesgpu_b200 import base
+    with pytest.raises(NotImplementedError, match="direct storage"):
+        base.PerturbedLinear(32, 8, 2, options={"direct": True, "tc": mode})
+    layer = base.PerturbedLinear(32, 8, 2, options={"direct": True})
+    layer.options["tc"] = mode
+    for population in (False, True):
+        layer.perturbed_flag = population
+        with pytest.raises(NotImplementedError, match="direct storage"):
+            layer(torch.zeros(4, 32))
+    assert base.PerturbedLinear(32, 8, 2, options={"direct": True, "tc": "tf32"}).options["direct"]
