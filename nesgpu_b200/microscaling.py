@@ -9,6 +9,7 @@ infinity has ``c = 255`` and reads as NaN throughout.
 Like the other ops of this package the functions take CUDA tensors, launch on the stream that is current at call time
 on the tensors' device, and record no autograd graph; there is no CPU path.
 """
+import importlib
 import math
 
 import torch
@@ -16,11 +17,23 @@ from torch import nn
 
 from . import _cabi  # noqa: F401  (loads the library that the extension module is linked with)
 
-try:
-    from . import _host
-except ImportError as e:
-    raise RuntimeError("nesgpu_b200: the extension module _host cannot be loaded (%s). Build it with `python -m "
-                       "nesgpu_b200.build`; there is no fallback path." % e) from e
+
+class _Unloaded:
+    """Stands for the extension module until a call needs it: it is built for one PyTorch and one Python, on which the layers
+    without microscaled calls do not depend."""
+
+    def __getattr__(self, name):
+        global _host
+        try:
+            module = importlib.import_module("._host", __package__)
+        except ImportError as e:
+            raise RuntimeError("nesgpu_b200: the extension module _host cannot be loaded (%s). Build it with `python -m "
+                               "nesgpu_b200.build`; there is no fallback path." % e) from e
+        _host = module
+        return getattr(module, name)
+
+
+_host = _Unloaded()
 
 BLOCK = 32
 FORMATS = {"mxfp4": 4, "mxfp8": 8}

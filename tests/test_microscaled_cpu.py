@@ -130,3 +130,30 @@ def test_direct_storage_has_no_microscaled_mode(mode):
         with pytest.raises(NotImplementedError, match="direct storage"):
             layer(torch.zeros(4, 32))
     assert base.PerturbedLinear(32, 8, 2, options={"direct": True, "tc": "tf32"}).options["direct"]
+
+
+def test_the_layers_do_without_the_extension_module():
+    """It is tied to one PyTorch; where it does not load, the microscaled calls say so and everything else works."""
+    import subprocess
+    import sys
+    program = """
+import sys
+sys.modules["nesgpu_b200._host"] = None                  # an import of it fails
+import torch
+from nesgpu_b200 import base, microscaling
+import modules.base, modules.binary
+layer = base.PermutedLinear(8, 8, 2)
+norm = base.PerturbedRMSNorm(8, 2)
+microscaling.MicroscaledLinear(64, 64)
+for call in (lambda: microscaling.quantize(torch.zeros(2, 64)), lambda: norm(torch.zeros(2, 8)), lambda: microscaling.linear(torch.zeros(2, 64), None)):
+    try:
+        call()
+    except RuntimeError as e:
+        print(e)
+"""
+    import os
+    run = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=600,
+                         cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert run.returncode == 0, run.stderr
+    said = run.stdout.splitlines()
+    assert len(said) == 3 and all("python -m nesgpu_b200.build" in line for line in said[:2]) and "MicroscaledTensor" in said[2]
