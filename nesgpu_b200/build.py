@@ -2,7 +2,8 @@
 ``nesgpu_b200/_host.so`` (host code that allocates through PyTorch and calls the library) from ``csrc/*_host.cpp``.
 
 Usage: ``python -m nesgpu_b200.build [--force] [--verbose]``.  nvcc cross-compiles without a
-GPU; the shared library is kept in-tree next to the package.
+GPU; the shared library is kept in-tree next to the package.  What is newer than its sources is left as it is, the extension
+module only if it was also built for this PyTorch and this Python.
 """
 import concurrent.futures
 import os
@@ -16,6 +17,7 @@ LIB_DIR = os.path.join(PKG, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libnesgpu_b200.so")
 HOST_PATH = os.path.join(PKG, "_host.so")
 OBJ_DIR = os.path.join(PKG, "build")
+HOST_TAG = os.path.join(OBJ_DIR, "microscaling_host.tag")      # what the extension module was built for
 INCLUDE = os.path.join(os.path.dirname(PKG), "include")
 
 NVCC_FLAGS = [
@@ -74,27 +76,52 @@ def _link_host(obj):
         raise RuntimeError("link failed:\n%s\n%s" % (res.stdout, res.stderr))
 
 
-def build(force=False, verbose=False):
-    """Compile every CUDA source for sm_100a and link the shared library and the extension module.  Returns the
-    library's path."""
-    os.makedirs(LIB_DIR, exist_ok=True)
-    os.makedirs(OBJ_DIR, exist_ok=True)
-    if not force and all(os.path.exists(p) and os.path.getmtime(p) >= _deps_mtime() for p in (LIB_PATH, HOST_PATH)):
-        return LIB_PATH
-    srcs = sources()
-    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as pool:
-        host = pool.submit(_compile_host)
-        results = list(pool.map(lambda s: _compile(s, verbose), srcs))
-        host_obj = host.result()
-    if verbose:
-        for _, log in results:
-            sys.stderr.write(log)
-    objs = [o for o, _ in results]
+def _link_library(objs):
     cmd = [_nvcc(), "-shared", "-o", LIB_PATH] + objs + ["-gencode", "arch=compute_100a,code=sm_100a"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError("link failed:\n%s\n%s" % (res.stdout, res.stderr))
-    _link_host(host_obj)
+
+
+def _wanted_tag():
+    import torch
+    return "torch %s, python %s" % (torch.__version__, sysconfig.get_config_var("SOABI"))
+
+
+def _built_tag():
+    try:
+        with open(HOST_TAG) as f:
+            return f.read()
+    except OSError:
+        return None
+
+
+def _is_current(path):
+    return os.path.exists(path) and os.path.getmtime(path) >= _deps_mtime()
+
+
+def build(force=False, verbose=False):
+    """Compile every CUDA source for sm_100a and link the shared library, then the extension module.  Returns the
+    library's path."""
+    os.makedirs(LIB_DIR, exist_ok=True)
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    library = force or not _is_current(LIB_PATH)
+    host = library or not _is_current(HOST_PATH) or _built_tag() != _wanted_tag()
+    srcs = sources() if library else []
+    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as pool:
+        host_obj = pool.submit(_compile_host) if host else None
+        results = list(pool.map(lambda s: _compile(s, verbose), srcs))
+    if verbose:
+        for _, log in results:
+            sys.stderr.write(log)
+    if library:
+        _link_library([o for o, _ in results])
+    if host:                                   # last: without it the library still serves all but the microscaled calls
+        if os.path.exists(HOST_TAG):
+            os.remove(HOST_TAG)
+        _link_host(host_obj.result())
+        with open(HOST_TAG, "w") as f:
+            f.write(_wanted_tag())
     return LIB_PATH
 
 

@@ -157,3 +157,47 @@ for call in (lambda: microscaling.quantize(torch.zeros(2, 64)), lambda: norm(tor
     assert run.returncode == 0, run.stderr
     said = run.stdout.splitlines()
     assert len(said) == 3 and all("python -m nesgpu_b200.build" in line for line in said[:2]) and "MicroscaledTensor" in said[2]
+
+
+def test_build_makes_what_is_out_of_date(tmp_path, monkeypatch):
+    """The extension module also when it was built for another PyTorch or Python, the library only for its sources; an extension
+    module that cannot be built leaves the library in place."""
+    import os
+    from nesgpu_b200 import build as B
+    done = []
+
+    def write(path):
+        with open(path, "w") as f:
+            f.write("x")
+        os.utime(path, (B._deps_mtime() + 10,) * 2)
+
+    for name, value in (("LIB_DIR", "lib"), ("OBJ_DIR", "build"), ("LIB_PATH", "lib/l.so"), ("HOST_PATH", "_host.so"), ("HOST_TAG", "build/t")):
+        monkeypatch.setattr(B, name, str(tmp_path / value))
+    monkeypatch.setattr(B, "_compile", lambda src, verbose: (src, ""))
+    monkeypatch.setattr(B, "_compile_host", lambda: "host.o")
+    monkeypatch.setattr(B, "_link_library", lambda objs: (done.append("library"), write(B.LIB_PATH)))
+    monkeypatch.setattr(B, "_link_host", lambda obj: (done.append(obj), write(B.HOST_PATH)))
+
+    def made(**kw):
+        del done[:]
+        assert B.build(**kw) == B.LIB_PATH
+        return list(done)
+
+    assert made() == ["library", "host.o"] and made() == []
+    monkeypatch.setattr(B, "_wanted_tag", lambda: "torch 9.9.9, python cpython-399")
+    assert made() == ["host.o"] and made() == []
+    os.remove(B.HOST_TAG)
+    assert made() == ["host.o"] and made(force=True) == ["library", "host.o"]
+    os.remove(B.HOST_PATH)
+    assert made() == ["host.o"]
+
+    def fails():
+        raise RuntimeError("g++ failed")
+
+    os.remove(B.LIB_PATH)
+    monkeypatch.setattr(B, "_compile_host", fails)
+    with pytest.raises(RuntimeError, match="g\\+\\+ failed"):
+        B.build()
+    assert os.path.exists(B.LIB_PATH) and B._built_tag() is None
+    with pytest.raises(RuntimeError, match="g\\+\\+ failed"):             # and says so again
+        B.build()
