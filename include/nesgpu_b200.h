@@ -593,8 +593,8 @@ int nes_binarized_int_threshold(const uint16_t* bias_half, const uint16_t* bias_
  * infinity has c = 255 and zero elements.
  * Layout: row-major, rows padded with zero codes and zero scales to whole groups of 128 elements: with
  * G = ceil(cols / 128), codes (rows, 64 G | 128 G) bytes, 16-byte aligned, scales (rows, 4 G) bytes; the product
- * wants codes 32-byte and scales 4-byte aligned.  An output that overlaps an input of the same call is refused
- * (NES_ERR_BAD_ARG). */
+ * wants codes 32-byte and scales 4-byte aligned.  An output that overlaps an input or another
+ * output of the same call is refused (NES_ERR_BAD_ARG). */
 
 enum nes_dtype { NES_F32 = 0, NES_BF16 = 1, NES_F16 = 2 };
 enum nes_mx_format { NES_MXFP4 = 4, NES_MXFP8 = 8 };

@@ -204,7 +204,7 @@ extern "C" int nes_mx_quantize(const void* x, int dtype, void* codes, uint8_t* s
   NES_REQUIRE(x && codes && scales, NES_ERR_BAD_ARG, "mx_quantize: null pointer");
   NES_REQUIRE(aligned16(codes), NES_ERR_BAD_ARG, "mx_quantize: codes must be 16-byte aligned");
   const Bytes outputs[] = {{codes, rows * code_pitch(cols, format)}, {scales, rows * scale_pitch(cols)}}, inputs[] = {{x, rows * cols * dtype_bytes(dtype)}};
-  NES_REQUIRE(!overlap(outputs, inputs), NES_ERR_BAD_ARG, "mx_quantize: the outputs overlap the input");
+  NES_REQUIRE(!overlap(outputs, inputs), NES_ERR_BAD_ARG, "mx_quantize: the outputs overlap the input or one another");
   cudaStream_t st = as_stream(stream);
   const bool four = format == NES_MXFP4;
   if (dtype == NES_F32) (four ? launch_quantize<float, NES_MXFP4> : launch_quantize<float, NES_MXFP8>)(x, codes, scales, rows, cols, st);

@@ -30,7 +30,8 @@ inline bool known_dtype(int t) { return t == NES_F32 || t == NES_BF16 || t == NE
 inline bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31u) == 0; }
 inline int64_t dtype_bytes(int t) { return t == NES_F32 ? 4 : 2; }
 
-// What a call reads or writes.  The blocks of a kernel run in any order, so an output that lies over an input is refused.
+// What a call reads or writes.  The blocks of a kernel run in any order, so an output that lies over an input or another output is
+// refused.
 struct Bytes { const void* at; int64_t size; };
 inline bool overlap(const Bytes& a, const Bytes& b) {
   const uintptr_t x = reinterpret_cast<uintptr_t>(a.at), y = reinterpret_cast<uintptr_t>(b.at);
@@ -38,9 +39,12 @@ inline bool overlap(const Bytes& a, const Bytes& b) {
 }
 template <int A, int B>
 inline bool overlap(const Bytes (&outputs)[A], const Bytes (&inputs)[B]) {
-  for (const Bytes& o : outputs)
+  for (int o = 0; o < A; ++o) {
     for (const Bytes& i : inputs)
-      if (overlap(o, i)) return true;
+      if (overlap(outputs[o], i)) return true;
+    for (int other = 0; other < o; ++other)
+      if (overlap(outputs[o], outputs[other])) return true;
+  }
   return false;
 }
 

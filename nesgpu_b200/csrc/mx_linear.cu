@@ -1082,7 +1082,7 @@ extern "C" int nes_mx_linear_fwd(const void* x, const uint8_t* x_scales, int x_d
   const Bytes outputs[] = {{y, M * N * dtype_bytes(y_dtype)}, {need ? scratch : nullptr, need}};
   const Bytes inputs[] = {{x, M * (x_scales ? code_pitch(K, x_format) : K * dtype_bytes(x_dtype))}, {x_scales, M * scale_pitch(K)},
                           {w_codes, N * code_pitch(K, w_format)}, {w_scales, N * scale_pitch(K)}, {bias, N * 4}};
-  NES_REQUIRE(!overlap(outputs, inputs), NES_ERR_BAD_ARG, "mx_linear_fwd: the output or the scratch overlaps an input");
+  NES_REQUIRE(!overlap(outputs, inputs), NES_ERR_BAD_ARG, "mx_linear_fwd: the output or the scratch overlaps an input or the other");
   cudaStream_t st = as_stream(stream);
   Product p;
   p.x_scales = x_scales; p.w_scales = w_scales; p.bias = bias; p.y = y; p.x = x; p.whole_rows = 0; p.overlap = false;

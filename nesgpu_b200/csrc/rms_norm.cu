@@ -512,7 +512,7 @@ extern "C" int nes_rms_norm_fwd(const void* x, const void* residual, void* resid
   const int64_t plain = rows * cols * dtype_bytes(dtype);
   const Bytes outputs[] = {{y, format ? rows * code_pitch(cols, format) : plain}, {format ? y_scales : nullptr, rows * scale_pitch(cols)}, {residual_out, plain}};
   const Bytes inputs[] = {{x, plain}, {residual, plain}, {gain, cols * 4}, {noise, members * cols * 4}};
-  NES_REQUIRE(!overlap(outputs, inputs), NES_ERR_BAD_ARG, "rms_norm_fwd: an output overlaps an input");
+  NES_REQUIRE(!overlap(outputs, inputs), NES_ERR_BAD_ARG, "rms_norm_fwd: an output overlaps an input or another output");
   NormArgs a;
   a.x = x; a.residual = residual; a.h = residual_out; a.gain = gain; a.noise = noise; a.y = y; a.scales = y_scales;
   a.rows = rows; a.cols = cols; a.members = members > 0 ? members : 1; a.antithetic = antithetic;

@@ -201,3 +201,22 @@ def test_build_makes_what_is_out_of_date(tmp_path, monkeypatch):
     assert os.path.exists(B.LIB_PATH) and B._built_tag() is None
     with pytest.raises(RuntimeError, match="g\\+\\+ failed"):             # and says so again
         B.build()
+
+
+def test_outputs_over_one_another_are_refused():
+    """Codes and scales, a norm's output and its residual, a product's output and its scratch; before anything reaches a device."""
+    from nesgpu_b200 import _cabi as C
+    f32, bf16, mx4, mx8 = 0, 1, 4, 8
+    a, b, c, d, e, f = (n << 40 for n in range(1, 7))
+    rows = 4 * 128 * 4                               # bytes of a (4, 128) fp32 matrix
+    need = C.call("nes_mx_linear_fwd_scratch_bytes", 200, 64, 128, mx8)
+    calls = [("nes_mx_quantize", (a, f32, b, b + 4 * 128 - 16, 4, 128, mx8, 0)),
+             ("nes_mx_quantize", (a, f32, b, b, 4, 128, mx4, 0)),
+             ("nes_rms_norm_fwd", (a, b, c, None, None, c, None, 4, 128, 0, 0, f32, 0, 1e-6, 0)),
+             ("nes_rms_norm_fwd", (a, b, c, None, None, c + rows - 16, d, 4, 128, 0, 0, f32, mx8, 1e-6, 0)),
+             ("nes_rms_norm_fwd", (a, b, c, None, None, d, c + rows - 1, 4, 128, 0, 0, f32, mx8, 1e-6, 0)),
+             ("nes_rms_norm_fwd", (a, None, None, None, None, d, d + 16, 4, 128, 0, 0, f32, mx4, 1e-6, 0)),
+             ("nes_mx_linear_fwd", (a, None, bf16, mx8, b, c, mx4, None, d + need - 32, f32, 200, 64, 128, d, need, 0))]
+    for name, args in calls:
+        with pytest.raises(C.NesError, match="overlap"):
+            C.call(name, *args)
