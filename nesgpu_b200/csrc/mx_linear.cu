@@ -18,9 +18,11 @@
 //     distributed shared memory.
 //
 // Few tokens are bound by the latencies of one load - product - store chain and then the weights' bytes: 1 token of
-// 4096x4096 takes 6.0 us with 8.9 MB to read (1.4 us), 24 tokens of 8192x8192 9.8 us (35.7 MB, 5.5 us).  Many are bound by
-// the tensor pipe and the power limit: 8192x4096x16384 in 4 bits takes 254 us in a burst (4.3 PFLOP/s) and 300 us back to back
-// at 1.64 GHz, with 8-bit activations 394 and 472 us (2.8 and 2.3 PFLOP/s at 1.4 GHz).
+// 4096x4096 with 8-bit activations takes 5.9 us with the weights in the L2 cache and 6.3 us out of HBM (8.9 MB, 1.4 us), 24 tokens of
+// 8192x8192 in 4 bits, quantised before, 12.1 us out of HBM (35.7 MB, 5.5 us).  Many are bound by the operands' way from L2 in 4 bits
+// (9.9 TB/s at 45 % tensor activity, where the 8-bit product has the same 9.9 TB/s at 70 %) and by the power limit back to back:
+// 8192x4096x16384 in 4 bits takes 254 us in a burst (4.3 PFLOP/s) and 300 us back to back at 1.64 GHz, with 8-bit activations 394
+// and 472 us (2.8 and 2.3 PFLOP/s at 1.4 GHz).
 #include <type_traits>
 #include "microscale.cuh"
 #include "tc_ptx.cuh"
@@ -89,7 +91,7 @@ __host__ __device__ constexpr uint32_t scale_byte(uint32_t id) { return (id << 2
 
 // The products of one stage: four instructions (two if HALF: a last stage with one 128-element group of 4-bit codes), each 32
 // bytes further along the rows.  They share one elected lane and one asm block: an instruction with an election of its own takes
-// 113 cycles to issue, which is more than a 4-bit product of 192 columns takes to run.
+// 113 cycles to issue, and the widest 4-bit one 170 to run.
 // kind::mxf4: two instructions per scale word (bytes 0-1 and 2-3), words sfa / sfb and sfa1 / sfb1; otherwise four.
 #define NES_MX_STAGE4(GROUP, KIND, VEC)                                                              \
   asm volatile(                                                                                      \

@@ -130,7 +130,8 @@ def rms_norm(input, weight=None, eps=1e-6, residual=None, noise=None, antithetic
     ``(members, cols)`` float32 adds ``noise[d]`` to the gain of the rows ``r * members + d`` (its negative for the
     second half of the repeats with ``antithetic``).  ``output`` is None for a ``y`` of the input's type, or
     ``"mxfp8"`` / ``"mxfp4"`` for a :class:`MicroscaledTensor`.  Squares are summed in fp32: a row with magnitudes above
-    1e19 has an infinite mean and is normalised to zeros."""
+    1e19 has an infinite mean and is normalised to zeros, and magnitudes below 1e-19 lose bits in it, which an ``eps`` above
+    1e-38 hides.  A value of ``y`` exactly between two codes takes the even one."""
     if output is None or output == getattr(input, "dtype", None):
         return _host.rms_norm(input, weight, eps, residual, noise, antithetic, 0)
     got = _host.rms_norm(input, weight, eps, residual, noise, antithetic, _format(output, "output"))
