@@ -59,7 +59,8 @@ __device__ __forceinline__ float scaled(float h, float2 r, float g, float gl) {
 // y are zero, and y and the exact value are told apart in 64 bits: y stays if they are equal (the border's own rule holds), else
 // it becomes its neighbour on the exact value's side.  y times the root is exact where the root is a number of few bits, without
 // which no value but zero can lie on a border.  One y in half a million is such a one, zeros aside: what the kernels do for them
-// is to gather every y's lowest set bit; a unit in which one of these is found is worked out a second time (settle_units).
+// is to gather every y's lowest set bit; a unit in which one of these is found is worked out a second time (settle_units).  A y
+// below 2^-126 has fewer bits than that and keeps its rounding to fp32.
 constexpr uint32_t BORDER_BITS = 0x7ff80000u;          // of a lowest set bit; a zero has none, or the sign
 // minus: -1, which the compiler does not know of: a product, unlike a negation, leaves the ALU pipe free
 __device__ __forceinline__ uint32_t lowest_bits(const float (&y)[UNIT], uint32_t minus) {
